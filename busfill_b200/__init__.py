@@ -10,6 +10,7 @@ Layouts (see include/busfill.h):
   ``wq`` uint8 [N, K/2], ``ws`` fp16 [N, K/32].
 * Q4_K: llama.cpp ``block_q4_K`` rows, uint8 [N, K/256*144].
 * activations fp16 [M, K]; outputs fp16 [M, N] (``busfill_q4``: fp32).
+* the 4-bit K/V cache and the operators around it: :mod:`busfill_b200.kv4`.
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ __all__ = [
     "gemm_q4_0", "gemm_q4k", "gemm_q4_0_ggml", "gemm_q4k_swiglu", "gemm_q4k_sweep", "SweepOp", "gemm_q4k_noalloc", "gemm_q5k", "gemm_q6k", "repack_q6k",
     "busfill_q4", "repack_q4k_planar", "gemm_q4k_planar", "Tensor", "tensor_desc", "mul_mat", "dequant_q4_0", "dequant_q4_0_ggml", "dequant_q4k", "dequant_q5k", "dequant_q6k",
     "stream_status", "stream_status_bits", "noalloc_status", "internal_allocations", "set_pdl", "set_ksplit", "set_prefill_min_m", "set_exact_kquant", "uses_prefill", "gemm_launches", "probe_umma", "version",
+    "KV4_PAGE", "kv4_page_bytes", "kv4_pool", "rope_table", "rope_axes", "kv4_append", "kv4_read", "attn_kv4", "kv4_evict",
 ]
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -32,7 +34,7 @@ _LIB = None
 STATUS = {
     0: "BUSFILL_OK", -1: "BUSFILL_ERR_INVALID_ARG", -2: "BUSFILL_ERR_SHAPE", -3: "BUSFILL_ERR_ALIGNMENT",
     -4: "BUSFILL_ERR_UNSUPPORTED_DEVICE", -5: "BUSFILL_ERR_LAUNCH", -6: "BUSFILL_ERR_ALLOC",
-    -7: "BUSFILL_ERR_DEVICE_TIMEOUT", -8: "BUSFILL_ERR_CUDA",
+    -7: "BUSFILL_ERR_DEVICE_TIMEOUT", -8: "BUSFILL_ERR_CUDA", -9: "BUSFILL_ERR_DEVICE_INDEX",
 }
 
 
@@ -96,6 +98,12 @@ _SIGS = {
     "busfill_ipc_get_handle": [_P, _P],
     "busfill_ipc_open": [_P, ctypes.POINTER(ctypes.c_void_p)],
     "busfill_ipc_close": [_P],
+    "busfill_kv4_page_bytes": [_I],
+    "busfill_rope_axes": [_P, _P],
+    "busfill_kv4_append": [_P, _P, _P],
+    "busfill_kv4_read": [_P, _P, _I, _P, _P, _P],
+    "busfill_attn_kv4": [_P, _P, _P],
+    "busfill_kv4_evict": [_P, _P, _P],
 }
 
 
@@ -548,3 +556,7 @@ def probe_umma(a, b, nb, stream=None):
     d = torch.empty((128, nb), dtype=torch.float32, device=a.device)
     _check(_lib().busfill_probe_umma(_ptr(a), _ptr(b), _ptr(d), nb, _stream(stream)), "busfill_probe_umma")
     return d
+
+
+from .kv4 import (KV4_PAGE, attn_kv4, kv4_append, kv4_evict, kv4_page_bytes, kv4_pool, kv4_read, rope_axes,  # noqa: E402
+                  rope_table)

@@ -20,6 +20,7 @@
 #include "prefill_pair_gemm.cuh"
 #include "sweep_gemm.cuh"
 #include "dequant.cuh"
+#include "host.h"
 
 using namespace busfill;
 
@@ -278,6 +279,10 @@ unsigned* sweep_workspace(int dev, cudaStream_t s, int sm_count) {
   }
   return w;
 }
+
+// The attention calls' workspace (host.h) and how many of its bytes are zero
+// between calls.
+std::map<std::pair<int, cudaStream_t>, std::pair<void*, size_t>> g_work;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -1064,6 +1069,55 @@ int gemm_sweep_impl(const busfill_sweep_op* ops, int nops, int M, cudaStream_t s
 // ===========================================================================
 // C ABI
 // ===========================================================================
+// ---------------------------------------------------------------------------
+// what the other translation units use (host.h)
+// ---------------------------------------------------------------------------
+namespace busfill {
+namespace host {
+
+int context(cudaStream_t s, Context* out) {
+  DeviceInfo di;
+  const int st = current_device(&di, &out->dev);
+  if (st != BUSFILL_OK) return st;
+  out->sms = di.sm_count;
+  std::lock_guard<std::mutex> lk(g_mu);
+  return get_error_words(out->dev, s, &out->error);
+}
+
+int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t zeroed, void** out) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  void*& w = g_work[{c.dev, s}].first;
+  g_work[{c.dev, s}].second = zeroed;
+  if (!w) {
+    if (capturing(s)) return BUSFILL_ERR_ALLOC;
+    if (cudaMalloc(&w, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      w = nullptr;
+      return BUSFILL_ERR_ALLOC;
+    }
+    ++g_internal_allocs;
+    if (cudaMemsetAsync(w, 0, zeroed, s) != cudaSuccess) {
+      cudaGetLastError();
+      cudaFree(w);
+      w = nullptr;
+      return BUSFILL_ERR_CUDA;
+    }
+  }
+  *out = w;
+  return BUSFILL_OK;
+}
+
+int launch(const void* kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, void** args) {
+  if (::launch(kernel, grid, block, smem, s, args, g_use_pdl.load() != 0) != cudaSuccess) {
+    cudaGetLastError();
+    return BUSFILL_ERR_LAUNCH;
+  }
+  return BUSFILL_OK;
+}
+
+}  // namespace host
+}  // namespace busfill
+
 extern "C" {
 
 int busfill_version(void) { return kVersion; }
@@ -1106,6 +1160,7 @@ const char* busfill_status_string(int status) {
     case BUSFILL_ERR_ALLOC: return "workspace allocation failed";
     case BUSFILL_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait expired (kernel gave up)";
     case BUSFILL_ERR_CUDA: return "CUDA runtime error";
+    case BUSFILL_ERR_DEVICE_INDEX: return "an index in device memory was out of range (not followed)";
     default: return "unknown status";
   }
 }
@@ -1474,12 +1529,16 @@ int busfill_stream_status_ex(void* stream, unsigned* bits) {
   }
   if (err == 0) return BUSFILL_OK;
   // a kernel gave up part way: clear the words for the next call, and the
-  // layer-sweep counters (a CTA that gave up may have left some raised)
+  // layer-sweep and attention counters (a CTA that gave up may have left some
+  // raised)
   if (cudaMemset(it->second, 0, kErrorWordsBytes) != cudaSuccess) return BUSFILL_ERR_CUDA;
   auto sw = g_sweep.find({dev, s});
   if (sw != g_sweep.end() && sw->second && cudaMemset(sw->second, 0, (size_t)sweep::kFlagWords * 4) != cudaSuccess)
     return BUSFILL_ERR_CUDA;
-  return BUSFILL_ERR_DEVICE_TIMEOUT;
+  auto wk = g_work.find({dev, s});
+  if (wk != g_work.end() && wk->second.first && cudaMemset(wk->second.first, 0, wk->second.second) != cudaSuccess)
+    return BUSFILL_ERR_CUDA;
+  return err == kErrIndex ? BUSFILL_ERR_DEVICE_INDEX : BUSFILL_ERR_DEVICE_TIMEOUT;
 }
 
 int busfill_probe_umma(const uint16_t* a, const uint16_t* b, float* d, int nb, void* stream) {

@@ -1,0 +1,283 @@
+// Host side of the cache operators in include/busfill.h (rope_axes, kv4_*,
+// attn_kv4): argument checks, the choice of the kernel and its launch shape.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "busfill.h"
+#include "kv4_attn.cuh"
+#include "kv4_cache.cuh"
+
+using namespace busfill;
+using namespace busfill::kv4;
+
+namespace {
+
+bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+bool is16bit(int dtype) { return dtype == BUSFILL_TYPE_F16 || dtype == BUSFILL_TYPE_BF16; }
+
+int check_cache(const busfill_kv4* c) {
+  if (!c || !c->pages || !c->table || !c->kv_len) return BUSFILL_ERR_INVALID_ARG;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return BUSFILL_ERR_SHAPE;
+  if (c->batch < 1 || c->batch > BUSFILL_KV4_MAX_BATCH || c->heads < 1 || c->heads > 65535 || c->num_pages < 1 ||
+      c->table_cols < 1 || c->table_cols > (1 << 24))
+    return BUSFILL_ERR_SHAPE;
+  if (!aligned(c->pages, 16) || !aligned(c->table, 4) || !aligned(c->kv_len, 4)) return BUSFILL_ERR_ALIGNMENT;
+  return BUSFILL_OK;
+}
+
+View view_of(const busfill_kv4* c) {
+  return View{c->pages, c->table, c->kv_len, c->num_pages, c->table_cols, c->batch, c->heads};
+}
+
+// f(std::integral_constant<int, D>) for the cache's head dimension
+template <typename Fn>
+int by_dim(int d, Fn f) {
+  if (d == 64) return f(std::integral_constant<int, 64>());
+  if (d == 128) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 256>());
+}
+
+// Raise a kernel's dynamic shared memory limit, once per device.
+template <typename Kernel>
+bool raise_smem(Kernel kernel, int bytes, int dev, std::once_flag (&once)[64], cudaError_t (&err)[64]) {
+  std::call_once(once[dev & 63], [&] {
+    err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  });
+  return err[dev & 63] == cudaSuccess;
+}
+
+constexpr long long kMaxGrid = 2147483647;
+
+// Query rows of the widest sequence and head from which two row tiles share a
+// warp's pass over the pages.
+constexpr int kTwoTileRows = 9;
+
+// Workspace of the attention calls on a stream: a counter per CTA, then the
+// largest kernel's partial results.
+constexpr size_t kCounterBytes = 4096;
+size_t workspace_bytes(int sms) {
+  size_t f = part_floats<64, 2>();
+  f = std::max(f, part_floats<128, 1>());
+  f = std::max(f, part_floats<128, 2>());
+  f = std::max(f, part_floats<256, 1>());
+  return kCounterBytes + (size_t)sms * f * sizeof(float);
+}
+
+template <int D, int NT>
+int launch_attn(const AttnParams& p, const host::Context& ctx, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  using G = Geo<D, NT>;
+  if (!raise_smem(attn_kernel<D, NT>, G::kBytes, ctx.dev, once, err)) return BUSFILL_ERR_LAUNCH;
+  void* args[] = {const_cast<AttnParams*>(&p)};
+  return host::launch(reinterpret_cast<const void*>(attn_kernel<D, NT>), dim3(ctx.sms), dim3(G::kWarps * 32),
+                      G::kBytes, s, args);
+}
+
+}  // namespace
+
+extern "C" {
+
+int busfill_kv4_page_bytes(int head_dim) {
+  return head_dim == 64 || head_dim == 128 || head_dim == 256 ? 72 * head_dim : BUSFILL_ERR_SHAPE;
+}
+
+int busfill_rope_axes(const busfill_rope* r, void* stream) {
+  if (!r || !r->q || !r->q_out || !r->positions || !r->cos || !r->sin || !r->axis) return BUSFILL_ERR_INVALID_ARG;
+  if (r->k_heads > 0 && (!r->k || !r->k_out)) return BUSFILL_ERR_INVALID_ARG;
+  if (!is16bit(r->dtype)) return BUSFILL_ERR_INVALID_ARG;
+  if (r->tokens < 0 || r->q_heads < 1 || r->k_heads < 0 || r->q_heads > 65535 || r->k_heads > 65535 ||
+      r->head_dim < 2 || r->head_dim > 512 || r->rot < 2 || (r->rot & 1) || r->rot > r->head_dim || r->axes < 1 ||
+      r->axes > 4 || r->max_pos < 1)
+    return BUSFILL_ERR_SHAPE;
+  const int half = r->rot / 2;
+  static_assert(kMaxFreqs == 256, "rot <= 512");
+  RopeParams p{};
+  for (int i = 0; i < half; ++i) {
+    if (r->axis[i] >= r->axes) return BUSFILL_ERR_INVALID_ARG;
+    p.axis[i] = r->axis[i];
+  }
+  const void* ptrs[] = {r->q, r->q_out, r->k_heads ? r->k : r->q, r->k_heads ? r->k_out : r->q_out};
+  const int64_t strides[] = {r->q_token, r->q_head, r->q_out_token, r->q_out_head,
+                             r->k_heads ? r->k_token : 0, r->k_heads ? r->k_head : 0,
+                             r->k_heads ? r->k_out_token : 0, r->k_heads ? r->k_out_head : 0};
+  // 16-byte pieces where every row starts on 16 bytes and the pieces come out even
+  bool vec = r->adjacent ? r->rot % 8 == 0 : half % 8 == 0;
+  vec = vec && (r->head_dim - r->rot) % 8 == 0;
+  for (const void* q : ptrs) {
+    if (!aligned(q, 2)) return BUSFILL_ERR_ALIGNMENT;
+    vec = vec && aligned(q, 16);
+  }
+  if (!aligned(r->positions, 4) || !aligned(r->cos, 4) || !aligned(r->sin, 4)) return BUSFILL_ERR_ALIGNMENT;
+  for (int64_t st : strides) vec = vec && st % 8 == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  host::Context ctx;
+  const int st = host::context(s, &ctx);
+  if (st != BUSFILL_OK || r->tokens == 0) return st;
+  p.q = r->q, p.k = r->k, p.q_out = r->q_out, p.k_out = r->k_out;
+  p.positions = r->positions, p.cos = r->cos, p.sin = r->sin;
+  p.q_token = r->q_token, p.q_head = r->q_head, p.k_token = r->k_token, p.k_head = r->k_head;
+  p.qo_token = r->q_out_token, p.qo_head = r->q_out_head, p.ko_token = r->k_out_token, p.ko_head = r->k_out_head;
+  p.tokens = r->tokens, p.q_heads = r->q_heads, p.k_heads = r->k_heads, p.dim = r->head_dim, p.half = half;
+  p.max_pos = r->max_pos;
+  p.sign = r->inverse ? -1.0f : 1.0f;
+  p.error = ctx.error;
+  const int pairs = vec ? (r->adjacent ? 4 : 8) : 1;
+  const int pieces = half / pairs + (r->head_dim - r->rot) / (vec ? 8 : 1);
+  const int heads = r->q_heads + r->k_heads;
+  // heads of one thread: as many as leave enough threads for the device
+  int per = 8;
+  while (per > 1 && (long long)r->tokens * pieces * ((heads + per - 1) / per) < (long long)ctx.sms * 2048) per /= 2;
+  p.heads_per_thread = per;
+  p.groups = (heads + per - 1) / per;
+  const long long blocks = ((long long)r->tokens * pieces * p.groups + 255) / 256;
+  if (blocks > kMaxGrid) return BUSFILL_ERR_SHAPE;
+  const bool h = r->dtype == BUSFILL_TYPE_F16, adj = r->adjacent != 0;
+  const void* kern;
+#define ROPE_KERNEL(T) \
+  (adj ? (vec ? (const void*)rope_kernel<T, true, true> : (const void*)rope_kernel<T, true, false>) \
+       : (vec ? (const void*)rope_kernel<T, false, true> : (const void*)rope_kernel<T, false, false>))
+  kern = h ? ROPE_KERNEL(__half) : ROPE_KERNEL(__nv_bfloat16);
+#undef ROPE_KERNEL
+  void* args[] = {&p};
+  return host::launch(kern, dim3((unsigned)blocks), dim3(256), 0, s, args);
+}
+
+int busfill_kv4_append(const busfill_kv4* cache, const busfill_kv4_rows* r, void* stream) {
+  int st = check_cache(cache);
+  if (st != BUSFILL_OK) return st;
+  if (!r || !r->k || !r->v || !is16bit(r->dtype)) return BUSFILL_ERR_INVALID_ARG;
+  if (r->tokens < 0 || (!r->q_start && r->tokens != cache->batch)) return BUSFILL_ERR_SHAPE;
+  if (!aligned(r->k, 2) || !aligned(r->v, 2) || !aligned(r->q_start, 4)) return BUSFILL_ERR_ALIGNMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  host::Context ctx;
+  st = host::context(s, &ctx);
+  if (st != BUSFILL_OK || r->tokens == 0) return st;
+  AppendParams p{};
+  p.c = view_of(cache);
+  p.k = r->k, p.v = r->v, p.q_start = r->q_start;
+  p.k_token = r->k_token, p.k_head = r->k_head, p.v_token = r->v_token, p.v_head = r->v_head;
+  p.tokens = r->tokens;
+  p.vec = aligned(r->k, 16) && aligned(r->v, 16) && (r->k_token | r->k_head | r->v_token | r->v_head) % 8 == 0;
+  p.error = ctx.error;
+  p.chunks = (2 * cache->heads * (cache->head_dim / 8) + 31) / 32;
+  const long long blocks = ((long long)p.tokens * p.chunks + 7) / 8;
+  if (blocks > kMaxGrid / 8) return BUSFILL_ERR_SHAPE;   // the kernel counts warps in an int
+  void* args[] = {&p};
+  return by_dim(cache->head_dim, [&](auto d) {
+    const void* kern = r->dtype == BUSFILL_TYPE_F16 ? (const void*)append_kernel<d(), __half>
+                                                    : (const void*)append_kernel<d(), __nv_bfloat16>;
+    return host::launch(kern, dim3((unsigned)blocks), dim3(256), 0, s, args);
+  });
+}
+
+int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_start, int tokens, uint16_t* k, uint16_t* v,
+                     void* stream) {
+  int st = check_cache(cache);
+  if (st != BUSFILL_OK) return st;
+  if (!k || !v) return BUSFILL_ERR_INVALID_ARG;
+  if (tokens < 0 || (!q_start && tokens != cache->batch)) return BUSFILL_ERR_SHAPE;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(q_start, 4)) return BUSFILL_ERR_ALIGNMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  host::Context ctx;
+  st = host::context(s, &ctx);
+  if (st != BUSFILL_OK || tokens == 0) return st;
+  ReadParams p{view_of(cache), q_start, tokens, (2 * cache->heads * (cache->head_dim / 8) + 31) / 32,
+               reinterpret_cast<__half*>(k), reinterpret_cast<__half*>(v), ctx.error};
+  const long long blocks = ((long long)tokens * p.chunks + 7) / 8;
+  if (blocks > kMaxGrid / 8) return BUSFILL_ERR_SHAPE;
+  void* args[] = {&p};
+  return by_dim(cache->head_dim, [&](auto d) {
+    return host::launch((const void*)read_kernel<d()>, dim3((unsigned)blocks), dim3(256), 0, s, args);
+  });
+}
+
+int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stream) {
+  int st = check_cache(cache);
+  if (st != BUSFILL_OK) return st;
+  if (!a || !a->q || !a->out || !is16bit(a->dtype) || (a->weights && !a->lse) || a->window < 0 ||
+      (a->window > 0 && !a->causal) || !(a->scale == a->scale))
+    return BUSFILL_ERR_INVALID_ARG;
+  if (a->tokens < 0 || a->q_heads < 1 || a->q_heads % cache->heads != 0 || a->max_q < 1 ||
+      (!a->q_start && a->tokens != cache->batch) ||
+      (long long)a->max_q * (a->q_heads / cache->heads) > (1 << 30) ||
+      (a->weights && a->weights_cols < (int64_t)64 * cache->table_cols))
+    return BUSFILL_ERR_SHAPE;
+  if (!aligned(a->q, 16) || !aligned(a->out, 16) || (a->q_token | a->q_head | a->out_token | a->out_head) % 8 != 0 ||
+      !aligned(a->lse, 4) || !aligned(a->weights, 4) || !aligned(a->q_start, 4))
+    return BUSFILL_ERR_ALIGNMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  host::Context ctx;
+  st = host::context(s, &ctx);
+  if (st != BUSFILL_OK || a->tokens == 0) return st;
+  void* work = nullptr;
+  st = host::workspace(ctx, s, workspace_bytes(ctx.sms), kCounterBytes, &work);
+  if (st != BUSFILL_OK) return st;
+  AttnParams p{};
+  p.c = view_of(cache);
+  p.q = a->q, p.out = a->out, p.lse = a->lse, p.weights = a->weights, p.q_start = a->q_start;
+  p.q_token = a->q_token, p.q_head = a->q_head, p.o_token = a->out_token, p.o_head = a->out_head;
+  p.weights_cols = a->weights_cols;
+  p.scale_log2 = a->scale * kLog2e;
+  p.tokens = a->tokens, p.q_heads = a->q_heads, p.group = a->q_heads / cache->heads;
+  p.max_q = a->q_start ? a->max_q : 1;
+  p.causal = a->causal != 0, p.window = a->window, p.bf16 = a->dtype == BUSFILL_TYPE_BF16;
+  p.counters = static_cast<unsigned*>(work);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
+  p.error = ctx.error;
+  if (ctx.sms > (int)(kCounterBytes / 4)) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
+  const bool two = p.max_q * p.group >= kTwoTileRows;
+  st = by_dim(cache->head_dim, [&](auto d) {
+    if constexpr (d() < 256) {
+      if (two) return launch_attn<d(), 2>(p, ctx, s);
+    }
+    return launch_attn<d(), 1>(p, ctx, s);
+  });
+  if (st != BUSFILL_OK || !a->weights) return st;
+  void* args[] = {&p};
+  return by_dim(cache->head_dim, [&](auto d) {
+    return host::launch((const void*)weights_kernel<d()>, dim3(ctx.sms * 4), dim3(256), 0, s, args);
+  });
+}
+
+int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, void* stream) {
+  int st = check_cache(cache);
+  if (st != BUSFILL_OK) return st;
+  if (!e || !e->weights || !e->weights_out || !e->index || !e->kv_len_out || !e->out_table ||
+      e->kv_len_out == cache->kv_len)
+    return BUSFILL_ERR_INVALID_ARG;
+  const bool in_place = e->out_table == cache->table;
+  if (e->keep < 1 || e->recent < 0 || e->recent > e->keep || e->weights_cols < (int64_t)64 * cache->table_cols ||
+      e->out_cols < 1 || e->out_cols > (1 << 24) || (int64_t)64 * e->out_cols < e->keep ||
+      (in_place && e->out_cols != cache->table_cols))
+    return BUSFILL_ERR_SHAPE;
+  if (!aligned(e->weights, 4) || !aligned(e->weights_out, 4) || !aligned(e->index, 4) || !aligned(e->kv_len_out, 4) ||
+      !aligned(e->out_table, 4))
+    return BUSFILL_ERR_ALIGNMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  host::Context ctx;
+  st = host::context(s, &ctx);
+  if (st != BUSFILL_OK) return st;
+  EvictParams p{view_of(cache), e->weights, e->weights_out, e->weights_cols, e->index, e->kv_len_out,
+                e->out_table,   e->out_cols, e->keep,       e->recent,       in_place, ctx.error};
+  const int rows = cache->batch * cache->heads;
+  void* args[] = {&p};
+  st = host::launch((const void*)evict_select_kernel, dim3(rows), dim3(kSelectThreads), 0, s, args);
+  if (st != BUSFILL_OK) return st;
+  // CTAs of a row: in place one; else enough to fill the device, as far as there are tokens
+  int per = 1;
+  if (!in_place)
+    per = std::max(1, std::min((e->keep + kMoveThreads / 8 * kMoveRows - 1) / (kMoveThreads / 8 * kMoveRows),
+                               (ctx.sms * 4 + rows - 1) / rows));
+  void* margs[] = {&p, &per};
+  return by_dim(cache->head_dim, [&](auto d) {
+    return host::launch((const void*)evict_move_kernel<d()>, dim3((unsigned)(rows * per)), dim3(kMoveThreads), 0, s,
+                        margs);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,810 @@
+// Attention over the 4-bit cache for few query rows per sequence and head
+// (single tokens, speculated tokens).
+//
+//   out[r] = sum_s p[r,s] v[s],  p = softmax_s(scale * q[r] . k[s])
+//
+// Bound: every cached token costs 9/8 D bytes (K and V codes and scales, once
+// per key/value head) and, for G query heads a group, 4 G D flops: the bytes
+// bound it while the codes can be turned into matrix operands fast enough. So
+// the codes go into the matrix instructions almost as they are:
+//   * A 4-bit code c under zero exponent bits is the fp16 subnormal c 2^-24
+//     (or, four bits up, c 2^-20), exactly, and the tensor core multiplies
+//     subnormals like any other number: one AND per two values. The factor
+//     16 between the nibbles is taken from q (keys: exact in fp16, q is
+//     brought to a row maximum near 2^10 by a power of two first) or from
+//     the sums (values).
+//   * The -8 of (c - 8) d leaves the sums: sum q (c - 8) starts its
+//     accumulator at -8 sum q; sum p d (c - 8) subtracts 8 sum p d, which one
+//     more matrix instruction per block (an operand of ones) adds up from
+//     the same rounded products.
+//   * Scales never touch the codes: the keys' multiply the finished block
+//     sums in fp32, the values' multiply p (fp16, one rounding).
+// The matrix instruction is m16n8k16 with the tokens (scores) or channels
+// (output) as its 16 rows and the query rows as its 8 columns, so that a
+// group of 8 query heads fills it.
+//
+// Work. A unit is one page of one (sequence, head, row group of 8 NT rows).
+// Units are numbered sequence by sequence and dealt out evenly, in ranges, to
+// all warps of a persistent grid: the split follows the lengths on the
+// device, whatever they are. A warp streams its pages with bulk copies into a
+// ring of its own and meets no other warp until its range is done. A range
+// begins and ends inside an item, as a rule: the pieces of an item are joined
+// first inside the CTA, then, by the CTA that comes last (a counter), from
+// the workspace; always in the order of the ranges, so results repeat bit for
+// bit.
+#pragma once
+
+#include "kv4_format.cuh"
+
+namespace busfill {
+namespace kv4 {
+
+constexpr int kMaxBatch = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttnParams {
+  View c;
+  const void* q;
+  void* out;
+  float* lse;        // [tokens][q_heads] or nullptr
+  float* weights;    // [batch][heads][weights_cols] (weights kernel)
+  const int* q_start;
+  long long q_token, q_head, o_token, o_head, weights_cols;
+  float scale_log2;  // scale * log2(e)
+  int tokens, q_heads, group, max_q;
+  int causal, window, bf16;
+  unsigned* counters;   // one per CTA, zero between calls
+  float* part;          // partial results (layout of the kernel)
+  unsigned* error;
+};
+
+// the bulk copy global -> shared (bytes a multiple of 16) counted on an mbarrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ void mma_16816(float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a sequence asks for: its rows, and the pages that some row of it sees.
+struct Span {
+  int first, n;     // rows of the step's tensors
+  int len;          // cached tokens
+  int page0, pages; // pages [page0, page0 + pages)
+};
+__device__ __forceinline__ Span span_of(const AttnParams& p, int b, bool& bad) {
+  Span s;
+  rows_of(p.q_start, b, p.tokens, s.first, s.n, bad);
+  if (s.n > p.max_q) {
+    bad = true;
+    s.n = p.max_q;
+  }
+  s.len = cached(p.c, b, bad);
+  const int lo = p.window > 0 ? max(0, s.len - s.n + 1 - p.window) : 0;
+  s.page0 = lo / kPage;
+  s.pages = s.n > 0 && s.len > 0 ? (s.len + kPage - 1) / kPage - s.page0 : 0;
+  return s;
+}
+// slots [lo, hi) that row i of the span sees
+__device__ __forceinline__ void sees(const AttnParams& p, const Span& s, int i, int& lo, int& hi) {
+  hi = p.causal ? min(s.len, s.len - s.n + i + 1) : s.len;
+  lo = p.window > 0 ? max(0, s.len - s.n + i + 1 - p.window) : 0;
+}
+
+// Query operand of one row group of 8 rows, and per column pair (2j, 2j + 1)
+// of the score fragments: -8 sum(q) of every block, the factor to log2
+// scores, the slots seen.
+template <int D>
+struct QueryTile {
+  uint32_t b[Fmt<D>::kBlocks][4];   // [block][2 * half + reg]
+  float corr[Fmt<D>::kBlocks][2];
+  float factor[2];
+  int lo[2], hi[2];
+};
+
+template <int D>
+__device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s, int head, int r0, int lane,
+                                             QueryTile<D>& t) {
+  constexpr int NB = Fmt<D>::kBlocks;
+  const int n = lane >> 2, j = lane & 3;
+  const int row = r0 + n, i = row / p.group;
+  const bool live = i < s.n;
+  float x[NB][8];
+  float top = 0.0f;
+  const size_t at = live ? (size_t)(s.first + i) * p.q_token + (size_t)(head * p.group + row - i * p.group) * p.q_head : 0;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int ch = 32 * b + 8 * j;
+    if (!live) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[b][e] = 0.0f;
+    } else if (p.bf16) {
+      load8(static_cast<const __nv_bfloat16*>(p.q) + at + ch, true, x[b]);
+    } else {
+      load8(static_cast<const __half*>(p.q) + at + ch, true, x[b]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[b][e]));
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  // power of two that brings the row's maximum to [2^9, 2^10); none for 0 and
+  // non-finite rows
+  int e = 136 - (int)(__float_as_uint(top) >> 23);
+  if (top == 0.0f || !(top <= 3.4e38f)) e = 0;
+  e = max(-126, min(126, e));
+  const float up = __uint_as_float((unsigned)(127 + e) << 23);
+  // codes weigh 2^-24 (see above)
+  const float factor = p.scale_log2 * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.0f;
+  float corr[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      const float y0 = x[b][k] * up, y1 = x[b][k + 1] * up, y2 = x[b][k + 2] * up, y3 = x[b][k + 3] * up;
+      sum += (y0 + y1) + (y2 + y3);
+      t.b[b][k / 2] = h2_as_u32(__floats2half2_rn(y0, y1));
+      t.b[b][k / 2 + 1] = h2_as_u32(__floats2half2_rn(y2 * 0.0625f, y3 * 0.0625f));
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    corr[b] = sum * (-8.0f / 16777216.0f);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int from = 4 * (2 * j + k);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) t.corr[b][k] = __shfl_sync(0xffffffffu, corr[b], from);
+    t.factor[k] = __shfl_sync(0xffffffffu, factor, from);
+    const int ri = (r0 + 2 * j + k) / p.group;
+    t.lo[k] = 0;   // columns without a row see everything, so that they hold up no page
+    t.hi[k] = s.len;
+    if (ri < s.n) sees(p, s, ri, t.lo[k], t.hi[k]);
+  }
+}
+
+// A vector of a lane's 32-bit words of one row: NB words (keys), NB / 2 (values).
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  }
+}
+
+// Scores of 16 tokens (tokens 16 mt .. of the page) for NT row tiles, times
+// nothing: s[nt][0..3] are rows (token tile_perm(lane / 4), and + 8) x column
+// pair. To log2 scores: * factor.
+template <int D, int NT>
+__device__ __forceinline__ void scores_16(const uint8_t* page, int mt, int lane, const QueryTile<D>* q, float (*s)[4]) {
+  using F = Fmt<D>;
+  constexpr int NB = F::kBlocks;
+  const int j = lane & 3, t = 16 * mt + tile_perm(lane >> 2);
+  uint32_t w0[NB], w1[NB], sc0[NB / 2], sc1[NB / 2];
+  lds_words<NB>(page + t * F::kRow + j * 4 * NB, w0);
+  lds_words<NB>(page + (t + 8) * F::kRow + j * 4 * NB, w1);
+  lds_words<NB / 2>(page + F::kKeyScale + t * 2 * NB, sc0);
+  lds_words<NB / 2>(page + F::kKeyScale + (t + 8) * 2 * NB, sc1);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t x0 = w0[b], x1 = w1[b];
+    const uint32_t a0[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u};
+    const uint32_t a1[4] = {x0 >> 8 & 0x000f000fu, x1 >> 8 & 0x000f000fu, x0 >> 8 & 0x00f000f0u,
+                            x1 >> 8 & 0x00f000f0u};
+    const float2 d0 = __half22float2(u32_as_h2(sc0[b / 2])), d1 = __half22float2(u32_as_h2(sc1[b / 2]));
+    const float e0 = b & 1 ? d0.y : d0.x, e1 = b & 1 ? d1.y : d1.x;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float acc[4] = {q[nt].corr[b][0], q[nt].corr[b][1], q[nt].corr[b][0], q[nt].corr[b][1]};
+      mma_16816(acc, a0, q[nt].b[b]);
+      mma_16816(acc, a1, q[nt].b[b] + 2);
+      s[nt][0] = fmaf(e0, acc[0], s[nt][0]);
+      s[nt][1] = fmaf(e0, acc[1], s[nt][1]);
+      s[nt][2] = fmaf(e1, acc[2], s[nt][2]);
+      s[nt][3] = fmaf(e1, acc[3], s[nt][3]);
+    }
+  }
+}
+
+// Running output of NT row tiles: o is channels x rows. Lane (c = lane / 4,
+// j = lane % 4) holds, of block b and half u, the channels 32b + 8(c/2) + 4u +
+// (c%2) (regs 0, 1: rows 2j, 2j + 1; in 2^24 ths) and the same + 2 (regs 2, 3; in
+// 2^20 ths); pd: sum of p d per block.
+template <int D, int NT>
+struct Running {
+  float o[NT][Fmt<D>::kBlocks][2][4];
+  float pd[NT][Fmt<D>::kBlocks][2];
+  float m[NT][2], l[NT][2];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) m[nt][k] = -INFINITY, l[nt][k] = 0.0f;
+#pragma unroll
+      for (int b = 0; b < Fmt<D>::kBlocks; ++b) {
+        pd[nt][b][0] = pd[nt][b][1] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[nt][b][e >> 2][e & 3] = 0.0f;
+      }
+    }
+  }
+};
+
+// One page (64 tokens, slots base .. base + 63) into the running output.
+template <int D, int NT>
+__device__ __forceinline__ void attend_page(const uint8_t* page, int base, int len, int lane, const QueryTile<D>* q,
+                                            Running<D, NT>& run) {
+  using F = Fmt<D>;
+  constexpr int NB = F::kBlocks;
+  const int c = lane >> 2, j = lane & 3;
+  float s[4][NT][4];
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt) scores_16<D, NT>(page, mt, lane, q, s[mt]);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    // the page lies inside what every row of the tile sees?
+    const bool whole = base >= max(q[nt].lo[0], q[nt].lo[1]) && base + kPage <= min(q[nt].hi[0], q[nt].hi[1]);
+    if (!__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int slot = base + 16 * mt + tile_perm(c) + 8 * (e >> 1);
+          const bool seen = slot >= q[nt].lo[e & 1] && slot < q[nt].hi[e & 1];
+          s[mt][nt][e] = seen ? s[mt][nt][e] * q[nt].factor[e & 1] : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][nt][e] *= q[nt].factor[e & 1];
+    }
+    float top[2] = {run.m[nt][0], run.m[nt][1]};
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[mt][nt][e]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], x));
+    float base2[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) base2[k] = top[k] == -INFINITY ? 0.0f : top[k];
+    if (__any_sync(0xffffffffu, top[0] != run.m[nt][0] || top[1] != run.m[nt][1])) {
+      const float f[2] = {exp2_approx(run.m[nt][0] - base2[0]), exp2_approx(run.m[nt][1] - base2[1])};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        run.m[nt][k] = top[k];
+        run.l[nt][k] *= f[k];
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        run.pd[nt][b][0] *= f[0];
+        run.pd[nt][b][1] *= f[1];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) run.o[nt][b][e >> 2][e & 3] *= f[e & 1];
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[mt][nt][e] = exp2_approx(s[mt][nt][e] - base2[e & 1]);
+        run.l[nt][e & 1] += s[mt][nt][e];
+      }
+  }
+  const uint8_t* vals = page + F::kValue;
+  const uint8_t* vsc = page + F::kValueScale;
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt) {
+    uint32_t p0[NT], p1[NT];   // rows (columns of the operand) x tokens 2j, 2j + 1 of each 8-token tile
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      p0[nt] = transpose_8x8(h2_as_u32(__floats2half2_rn(s[mt][nt][0], s[mt][nt][1])));
+      p1[nt] = transpose_8x8(h2_as_u32(__floats2half2_rn(s[mt][nt][2], s[mt][nt][3])));
+    }
+    const int ta = 16 * mt + tile_perm(2 * j), tb = 16 * mt + tile_perm(2 * j + 1);
+    uint32_t w[4][NB / 2];
+    lds_words<NB / 2>(vals + ta * F::kRow + (c ^ value_swizzle<D>(ta)) * 2 * NB, w[0]);
+    lds_words<NB / 2>(vals + tb * F::kRow + (c ^ value_swizzle<D>(tb)) * 2 * NB, w[1]);
+    lds_words<NB / 2>(vals + (ta + 8) * F::kRow + (c ^ value_swizzle<D>(ta + 8)) * 2 * NB, w[2]);
+    lds_words<NB / 2>(vals + (tb + 8) * F::kRow + (c ^ value_swizzle<D>(tb + 8)) * 2 * NB, w[3]);
+    // slots behind the sequence hold anything, non-finite scales too
+    const int left = len - base - 16 * mt;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t d0 = *reinterpret_cast<const uint32_t*>(vsc + (b * kPage + 16 * mt + 2 * j) * 2);
+      uint32_t d1 = *reinterpret_cast<const uint32_t*>(vsc + (b * kPage + 16 * mt + 8 + 2 * j) * 2);
+      if (left < 16) {
+        const int a = tile_perm(2 * j), bb = tile_perm(2 * j + 1);
+        d0 &= (a < left ? 0xffffu : 0u) | (bb < left ? 0xffff0000u : 0u);
+        d1 &= (a + 8 < left ? 0xffffu : 0u) | (bb + 8 < left ? 0xffff0000u : 0u);
+      }
+      const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
+      const uint32_t x0 = prmt(w[0][b / 2], w[1][b / 2], sel), x1 = prmt(w[2][b / 2], w[3][b / 2], sel);
+      const uint32_t a0[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
+      const uint32_t a1[4] = {x0 >> 8 & 0x000f000fu, x0 >> 8 & 0x00f000f0u, x1 >> 8 & 0x000f000fu,
+                              x1 >> 8 & 0x00f000f0u};
+      const uint32_t ones[4] = {0x3C003C00u, 0u, 0x3C003C00u, 0u};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t pb[2] = {h2_as_u32(__hmul2(u32_as_h2(p0[nt]), u32_as_h2(d0))),
+                                h2_as_u32(__hmul2(u32_as_h2(p1[nt]), u32_as_h2(d1)))};
+        mma_16816(run.o[nt][b][0], a0, pb);
+        mma_16816(run.o[nt][b][1], a1, pb);
+        float acc[4] = {run.pd[nt][b][0], run.pd[nt][b][1], 0.0f, 0.0f};
+        mma_16816(acc, ones, pb);
+        run.pd[nt][b][0] = acc[0];
+        run.pd[nt][b][1] = acc[1];
+      }
+    }
+  }
+}
+
+// The finished running output as plain sums: o[channel] = sum p v, and the
+// row sums l over the warp.
+template <int D, int NT>
+__device__ __forceinline__ void settle(Running<D, NT>& run) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) run.l[nt][k] += __shfl_xor_sync(0xffffffffu, run.l[nt][k], x);
+#pragma unroll
+    for (int b = 0; b < Fmt<D>::kBlocks; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        run.o[nt][b][e >> 2][e & 3] =
+            fmaf(run.o[nt][b][e >> 2][e & 3], e & 2 ? 1048576.0f : 16777216.0f, -8.0f * run.pd[nt][b][e & 1]);
+  }
+}
+template <int D>
+__device__ __forceinline__ int channel_of(int lane, int b, int u, int e) {
+  const int c = lane >> 2;
+  return 32 * b + 8 * (c >> 1) + 4 * u + (c & 1) + (e & 2);
+}
+
+template <int D>
+__device__ __forceinline__ void store_out(const AttnParams& p, const Span& s, int head, int row, int ch, float x) {
+  const int i = row / p.group;
+  if (i >= s.n) return;
+  const size_t at = (size_t)(s.first + i) * p.o_token + (size_t)(head * p.group + row - i * p.group) * p.o_head + ch;
+  if (p.bf16)
+    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
+  else
+    static_cast<__half*>(p.out)[at] = __float2half_rn(x);
+}
+__device__ __forceinline__ void store_lse(const AttnParams& p, const Span& s, int head, int row, float m, float l) {
+  const int i = row / p.group;
+  if (!p.lse || i >= s.n) return;
+  p.lse[(size_t)(s.first + i) * p.q_heads + head * p.group + row - i * p.group] =
+      l > 0.0f ? (m + log2f(l)) * kLn2 : l == 0.0f ? -INFINITY : l;
+}
+
+// Geometry by head dimension and row tiles: warps of a CTA (one CTA per SM)
+// and pages of each warp's ring.
+template <int D, int NT>
+struct Geo {
+  static constexpr int kWarps = D == 256 ? 6 : NT == 1 ? 12 : 8;
+  static constexpr int kStages = D == 64 ? 4 : D == 256 ? 2 : NT == 1 ? 2 : 3;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kPieceFloats = kRows * (D + 2);          // o, m, l of a piece
+  static constexpr int kRingBytes = kStages * Fmt<D>::kPageBytes;
+  static constexpr int kPreOff = kWarps * kRingBytes;           // units before each sequence
+  static constexpr int kBarOff = kPreOff + (kMaxBatch + 2) * 4;
+  static constexpr int kMiscOff = kBarOff + kWarps * kStages * 8;
+  static constexpr int kBytes = kMiscOff + 256;
+  static_assert(kPieceFloats * 4 <= kRingBytes, "a piece fits the warp's ring");
+  static_assert(kBytes <= 232448, "dynamic shared memory");
+};
+// workspace, per CTA: every warp's first piece, then the CTA's two partial items
+template <int D, int NT>
+constexpr size_t part_floats() {
+  return (size_t)(Geo<D, NT>::kWarps + 2) * Geo<D, NT>::kPieceFloats;
+}
+
+// Position in the list of units.
+struct Cursor {
+  int b, head, rg, page;    // page: index in the sequence
+  int rgs;                  // row groups of the sequence
+  Span s;
+};
+
+// units before sequence b in pre[b]; sets the cursor to unit u < pre[batch]
+template <int ROWS>
+__device__ __forceinline__ void seek(const AttnParams& p, const int* pre, int u, Cursor& c, bool& bad) {
+  int lo = 0, hi = p.c.batch;   // last b with pre[b] <= u; empty sequences before it share its start
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= u)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  c.b = lo;
+  c.s = span_of(p, lo, bad);
+  c.rgs = (c.s.n * p.group + ROWS - 1) / ROWS;
+  int r = u - pre[lo];
+  c.head = r / (c.rgs * c.s.pages);
+  r -= c.head * c.rgs * c.s.pages;
+  c.rg = r / c.s.pages;
+  c.page = c.s.page0 + r - c.rg * c.s.pages;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const __grid_constant__ AttnParams p) {
+  using F = Fmt<D>;
+  using G = Geo<D, NT>;
+  constexpr int NB = F::kBlocks, ROWS = G::kRows, W = G::kWarps, S = G::kStages, PF = G::kPieceFloats;
+  extern __shared__ __align__(128) uint8_t smem[];
+  int* pre = reinterpret_cast<int*>(smem + G::kPreOff);
+  int* misc = reinterpret_cast<int*>(smem + G::kMiscOff);
+  int* piece_item = misc;            // [2 * W]: first unit of the item, -1: no piece
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = smem + warp * G::kRingBytes;
+  const uint32_t ring_s = smem_u32(ring);
+  const uint32_t bar0 = smem_u32(smem + G::kBarOff) + warp * S * 8;
+  if (lane < S) mbar_init(bar0 + 8 * lane, 1);
+  fence_mbar_init();
+  pdl_wait_prerequisites();
+  pdl_launch_dependents();
+
+  // units of every sequence, then their running sum (warp 0)
+  bool bad = false;
+  const int batch = p.c.batch;
+  for (int b = threadIdx.x; b < batch; b += W * 32) {
+    const Span s = span_of(p, b, bad);
+    const long long n = (long long)p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS) * s.pages;
+    if (n > (1 << 30)) bad = true;
+    pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
+    if (n == 0 && blockIdx.x == 0) {   // rows that see nothing
+      for (int i = 0; i < s.n; ++i)
+        for (int h = 0; h < p.q_heads; ++h) {
+          for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, h / p.group, i * p.group + h % p.group, ch, 0.0f);
+          store_lse(p, s, h / p.group, i * p.group + h % p.group, 0.0f, 0.0f);
+        }
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int total = 0;
+    if (lane == 0) pre[0] = 0;
+    for (int b0 = 0; b0 < batch; b0 += 32) {
+      int x = b0 + lane < batch ? pre[b0 + lane + 1] : 0;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, m);
+        if (lane >= m) x += y;
+      }
+      if (b0 + lane < batch) pre[b0 + lane + 1] = total + x;
+      total += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+  const int T = pre[batch];
+  const long long ctas = min((int)gridDim.x, T);   // every CTA of the split has a unit
+  if ((int)blockIdx.x >= ctas) {
+    if (bad) atomicOr(p.error, kErrIndex);
+    return;
+  }
+  const int c0 = (int)((long long)T * blockIdx.x / ctas), c1 = (int)((long long)T * (blockIdx.x + 1) / ctas);
+  const int u0 = c0 + (int)((long long)(c1 - c0) * warp / W), u1 = c0 + (int)((long long)(c1 - c0) * (warp + 1) / W);
+
+  float* my_part = p.part + (size_t)blockIdx.x * part_floats<D, NT>();
+  if (lane == 0) piece_item[2 * warp] = piece_item[2 * warp + 1] = -1;
+  bool ok = true;
+  if (u0 < u1) {
+    Cursor c;
+    seek<ROWS>(p, pre, u0, c, bad);
+    // the pages ahead: a cursor of its own, the page number one step ahead
+    int ib = c.b, ihead = c.head, irg = c.rg, ipage = c.page, irgs = c.rgs;
+    Span is = c.s;
+    auto next_source = [&]() -> const uint8_t* {
+      const int pg = page_of(p.c, p.c.table, p.c.table_cols, ib, ipage, bad);
+      const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + ihead) * F::kPageBytes;
+      if (++ipage == is.page0 + is.pages) {
+        if (++irg == irgs) {
+          irg = 0;
+          if (++ihead == p.c.heads) {
+            ihead = 0;
+            do ++ib;
+            while (ib < batch && pre[ib + 1] == pre[ib]);
+            if (ib < batch) {
+              is = span_of(p, ib, bad);
+              irgs = (is.n * p.group + ROWS - 1) / ROWS;
+            }
+          }
+        }
+        ipage = is.page0;
+      }
+      return src;
+    };
+    int issued = u0;
+    for (int k = 0; k < S && issued < u1; ++k, ++issued) {
+      const uint8_t* src = next_source();
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar0 + 8 * k, F::kPageBytes);
+        bulk_load(ring_s + k * F::kPageBytes, src, F::kPageBytes, bar0 + 8 * k);
+      }
+    }
+    const uint8_t* ahead = issued < u1 ? next_source() : nullptr;
+
+    QueryTile<D> q[NT];
+    Running<D, NT> run;
+    int stage = 0;
+    uint32_t parity = 0;
+    int item0 = u0 - (c.page - c.s.page0);   // first unit of the current item
+    int begun = u0;                          // first unit of the current piece
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) load_queries<D>(p, c.s, c.head, c.rg * ROWS + 8 * nt, lane, q[nt]);
+    run.clear();
+    for (int u = u0; u < u1; ++u) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, parity));
+      if (!ok) break;
+      attend_page<D, NT>(ring + stage * F::kPageBytes, c.page * kPage, c.s.len, lane, q, run);
+      __syncwarp();
+      if (ahead) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar0 + 8 * stage, F::kPageBytes);
+          bulk_load(ring_s + stage * F::kPageBytes, ahead, F::kPageBytes, bar0 + 8 * stage);
+        }
+        ++issued;
+        ahead = issued < u1 ? next_source() : nullptr;
+      }
+      if (++stage == S) {
+        stage = 0;
+        parity ^= 1;
+      }
+      const bool ends = c.page + 1 == c.s.page0 + c.s.pages;
+      if (!ends && u + 1 < u1) {
+        ++c.page;
+        continue;
+      }
+      // a piece is done
+      settle<D, NT>(run);
+      if (ends && begun == item0) {   // the whole item
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float inv[2] = {run.l[nt][0] == 0.0f ? 0.0f : 1.0f / run.l[nt][0],
+                                run.l[nt][1] == 0.0f ? 0.0f : 1.0f / run.l[nt][1]};
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = c.rg * ROWS + 8 * nt + 2 * (lane & 3) + (e & 1);
+              store_out<D>(p, c.s, c.head, row, channel_of<D>(lane, b, e >> 2, e),
+                           run.o[nt][b][e >> 2][e & 3] * inv[e & 1]);
+            }
+          if (lane < 4) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              store_lse(p, c.s, c.head, c.rg * ROWS + 8 * nt + 2 * lane + k, run.m[nt][k], run.l[nt][k]);
+          }
+        }
+      } else {
+        // kept for the join: the last piece in the ring (all of it has
+        // landed and been read), an earlier one in the workspace
+        const bool last = u + 1 == u1;
+        float* to = last ? reinterpret_cast<float*>(ring) : my_part + (size_t)warp * PF;
+        __syncwarp();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              to[(8 * nt + 2 * (lane & 3) + (e & 1)) * D + channel_of<D>(lane, b, e >> 2, e)] =
+                  run.o[nt][b][e >> 2][e & 3];
+          if (lane < 4) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              to[ROWS * D + 8 * nt + 2 * lane + k] = run.m[nt][k];
+              to[ROWS * (D + 1) + 8 * nt + 2 * lane + k] = run.l[nt][k];
+            }
+          }
+        }
+        if (lane == 0) piece_item[2 * warp + (last ? 1 : 0)] = item0;
+      }
+      if (u + 1 < u1) {   // the next item
+        seek<ROWS>(p, pre, u + 1, c, bad);
+        item0 = begun = u + 1;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) load_queries<D>(p, c.s, c.head, c.rg * ROWS + 8 * nt, lane, q[nt]);
+        run.clear();
+      }
+    }
+    if (!ok && lane == 0) {   // gave up: nothing may land after the CTA is gone
+      atomicOr(p.error, 1u);
+      for (int k = 0; k < S; ++k) mbar_wait(bar0 + 8 * k, k < stage ? parity ^ 1 : parity);
+    }
+  }
+  __threadfence_block();
+  __syncthreads();
+
+  // join the CTA's pieces, item by item
+  auto piece = [&](int i) -> const float* {
+    return (i & 1) ? reinterpret_cast<const float*>(smem + (i >> 1) * G::kRingBytes) : my_part + (size_t)(i >> 1) * PF;
+  };
+  // rows x channels of `n` pieces get(i) to the output or to `to`
+  auto join = [&](int n, auto get, const Cursor& c, float* to) {
+    for (int x = threadIdx.x; x < ROWS * D; x += W * 32) {
+      const int row = x / D, ch = x - row * D;
+      float m = -INFINITY, l = 0.0f, o = 0.0f;
+      for (int i = 0; i < n; ++i) m = fmaxf(m, get(i)[ROWS * D + row]);
+      for (int i = 0; i < n; ++i) {
+        const float* s = get(i);
+        const float mi = s[ROWS * D + row];
+        // an empty piece has m = -inf, l = 0 and o = 0; NaN scores leave m at -inf and l NaN
+        const float f = mi == -INFINITY ? 1.0f : exp2_approx(mi - m);
+        l = fmaf(s[ROWS * (D + 1) + row], f, l);
+        o = fmaf(s[x], f, o);
+      }
+      if (to) {
+        to[x] = o;
+        if (ch == 0) {
+          to[ROWS * D + row] = m;
+          to[ROWS * (D + 1) + row] = l;
+        }
+      } else {
+        store_out<D>(p, c.s, c.head, c.rg * ROWS + row, ch, l == 0.0f ? 0.0f : o / l);
+        if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, m, l);
+      }
+    }
+  };
+  int* list = piece_item + 2 * W;   // the pieces there are, in order
+  int* count = list + 2 * W;
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int i = 0; i < 2 * W; ++i)
+      if (piece_item[i] >= 0) list[n++] = i;
+    *count = n;
+  }
+  __syncthreads();
+  const int pieces = *count;
+  for (int i0 = 0; i0 < pieces;) {
+    const int item0 = piece_item[list[i0]];
+    int i1 = i0 + 1;
+    while (i1 < pieces && piece_item[list[i1]] == item0) ++i1;
+    Cursor c;
+    seek<ROWS>(p, pre, item0, c, bad);
+    const int end = item0 + c.s.pages;
+    auto mine = [&](int i) { return piece(list[i0 + i]); };
+    if (item0 >= c0 && end <= c1) {
+      join(i1 - i0, mine, c, nullptr);
+    } else {
+      // split between CTAs: slot 0 for the item that began before this CTA's
+      // range, slot 1 for the one that goes on behind it
+      join(i1 - i0, mine, c, my_part + (size_t)(W + (item0 < c0 ? 0 : 1)) * PF);
+      __threadfence();
+      __syncthreads();
+      const int first = (int)((((long long)item0 + 1) * ctas - 1) / T), last = (int)(((long long)end * ctas - 1) / T);
+      if (threadIdx.x == 0)
+        misc[255 / 4] = atom_add_acq_rel_gpu(p.counters + first, 1u) == (unsigned)(last - first) ? 1 : 0;
+      __syncthreads();
+      if (misc[255 / 4]) {
+        __threadfence();
+        auto theirs = [&](int i) -> const float* {
+          return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(W + (i == 0 ? 1 : 0)) * PF;
+        };
+        join(last - first + 1, theirs, c, nullptr);
+        if (threadIdx.x == 0) p.counters[first] = 0;
+      }
+      __syncthreads();
+    }
+    i0 = i1;
+  }
+  if (bad) atomicOr(p.error, kErrIndex);
+}
+
+// The weight that the call's rows give every cached token, added to the
+// running sums: weights[b][h][s] += sum over the rows r of the group of
+// exp(score[r,s] - lse[r]). Keys only. A warp takes whole pages and walks over
+// the rows that see them, so each sum has one owner and one order.
+template <int D>
+__global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ AttnParams p) {
+  using F = Fmt<D>;
+  __shared__ int pre[kMaxBatch + 1];
+  pdl_wait_prerequisites();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = p.c.batch;
+  bool bad = false;
+  for (int b = threadIdx.x; b < batch; b += blockDim.x) {
+    const Span s = span_of(p, b, bad);
+    const long long n = (long long)p.c.heads * s.pages;
+    pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    pre[0] = 0;
+    for (int b = 0; b < batch; ++b) pre[b + 1] += pre[b];
+  }
+  __syncthreads();
+  const int T = pre[batch];
+  for (int u = blockIdx.x * (blockDim.x >> 5) + warp; u < T; u += gridDim.x * (blockDim.x >> 5)) {
+    int lo = 0, hi = batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (pre[mid] <= u ? lo : hi) = mid;
+    }
+    const Span s = span_of(p, lo, bad);
+    const int r = u - pre[lo], head = r / s.pages, pg = s.page0 + r - head * s.pages, base = pg * kPage;
+    const uint8_t* page =
+        p.c.pages + ((size_t)page_of(p.c, p.c.table, p.c.table_cols, lo, pg, bad) * p.c.heads + head) * F::kPageBytes;
+    float sum[4][2] = {};
+    // rows that see the page: causal rows from the page's first slot on, and
+    // with a window up to the last that still reaches it
+    const int i0 = p.causal ? max(0, base - (s.len - s.n)) : 0;
+    const int i1 = p.window > 0 ? min(s.n, base + kPage - 1 + p.window - (s.len - s.n)) : s.n;
+    for (int r0 = i0 * p.group / 8 * 8; r0 < i1 * p.group; r0 += 8) {
+      QueryTile<D> q;
+      load_queries<D>(p, s, head, r0, lane, q);
+      float norm[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = r0 + 2 * (lane & 3) + k, i = row / p.group;
+        norm[k] = INFINITY;   // no weight from rows that are not there or see nothing
+        if (i < s.n) {
+          const float x = p.lse[(size_t)(s.first + i) * p.q_heads + head * p.group + row - i * p.group] * kLog2e;
+          if (x != -INFINITY) norm[k] = x;
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        float x[1][4];
+        scores_16<D, 1>(page, mt, lane, &q, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int slot = base + 16 * mt + tile_perm(lane >> 2) + 8 * (e >> 1);
+          const bool seen = slot >= q.lo[e & 1] && slot < q.hi[e & 1];
+          if (seen) sum[mt][e >> 1] += exp2_approx(fmaf(x[0][e], q.factor[e & 1], -norm[e & 1]));
+        }
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x = sum[mt][k];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        const int slot = base + 16 * mt + tile_perm(lane >> 2) + 8 * k;
+        if ((lane & 3) == 0 && slot < s.len)
+          p.weights[((size_t)lo * p.c.heads + head) * p.weights_cols + slot] += x;
+      }
+  }
+  if (bad) atomicOr(p.error, kErrIndex);
+}
+
+}  // namespace kv4
+}  // namespace busfill

@@ -41,7 +41,9 @@ typedef enum busfill_status {
   BUSFILL_ERR_LAUNCH = -5,             /* kernel launch failed              */
   BUSFILL_ERR_ALLOC = -6,              /* workspace allocation failed       */
   BUSFILL_ERR_DEVICE_TIMEOUT = -7,     /* a bounded device wait expired     */
-  BUSFILL_ERR_CUDA = -8                /* other CUDA runtime error          */
+  BUSFILL_ERR_CUDA = -8,               /* other CUDA runtime error          */
+  BUSFILL_ERR_DEVICE_INDEX = -9        /* an index in device memory (page, position,
+                                          length) was out of its range      */
 } busfill_status;
 
 /* ---------------------------------------------------------------------------
@@ -272,6 +274,7 @@ BUSFILL_API int busfill_gemm_q4k_planar(const uint8_t* qs, const uint16_t* d, co
 #define BUSFILL_TYPE_Q4_K 12
 #define BUSFILL_TYPE_Q5_K 13
 #define BUSFILL_TYPE_Q6_K 14
+#define BUSFILL_TYPE_BF16 30
 typedef struct busfill_tensor {
   int32_t type;  /* BUSFILL_TYPE_*: the ggml_type numbering */
   int64_t ne[4]; /* elements per dimension, ne[0] innermost */
@@ -355,11 +358,161 @@ BUSFILL_API int busfill_dequant_q5k(const uint8_t* blocks, uint16_t* out, int N,
 BUSFILL_API int busfill_dequant_q6k(const uint8_t* body, const uint16_t* d, uint16_t* out, int N, int K, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Between the QKV and the O projection: rotary positions, a 4-bit K/V cache,
+ * attention over it, eviction. No reference counterpart (the reference stops
+ * at the GEMM, kernels/busfill_v1a.cu:41-104); these are the operators a
+ * decoder layer runs between two of its GEMMs.
+ *
+ * The cache is a pool of pages. A page holds BUSFILL_KV4_PAGE = 64 tokens of
+ * one key/value head, keys and values, in busfill_kv4_page_bytes(D) = 72 D
+ * bytes for head dimension D (64, 128 or 256):
+ *   [0, 32D)     key codes, one row of D/2 bytes per token
+ *   [32D, 36D)   key scales, fp16 [64 tokens][D/32]
+ *   [36D, 68D)   value codes, one row of D/2 bytes per token
+ *   [68D, 72D)   value scales, fp16 [D/32][64 tokens]
+ * Every 32 channels of a token are a block with one scale d; a 4-bit code c
+ * stands for (c - 8) * d, the Q4_0 rule. d is the block's value of largest
+ * magnitude (the first of equals) over -8, rounded to 7 significant bits and
+ * clamped to +-896, so that (c - 8) * d is exact in fp16; c is
+ * floor(x / d + 8.5) clamped to 0..15 (8 where d is 0). Values beyond the
+ * range (7168) and infinities saturate, NaN is stored as 0: what the cache
+ * holds is always finite. With n = D/32 blocks and channel 32b + 8j + m of
+ * token t:
+ *   key:   nibble m/2 + 4(m%2) of the 32-bit word j*n + b of the row
+ *   value: nibble m/2 of the 16-bit word ((2j + m%2) ^ x)*n + b of the row,
+ *          x = 0 (D = 64), 4(t/4%2) (D = 128), 2(t/2%4) (D = 256)
+ *   value scale: entry t ^ (t/2%2) of its block's 64
+ * (nibbles little-endian). The order is the one in which the attention
+ * kernels' threads read their matrix fragments, so a page goes from memory
+ * to the tensor cores without a shuffle.
+ *
+ * Sequence i of a batch owns slots 0 .. kv_len[i] - 1; slot s lives in entry
+ * s % 64 of page table[i * table_cols + s / 64]. `q_start` (device, batch + 1
+ * entries) gives each sequence its rows of the step's tensors: rows
+ * q_start[i] .. q_start[i+1] - 1 are its newest tokens, so row r of a
+ * sequence with n rows belongs to slot kv_len - n + r; NULL means one row per
+ * sequence. kv_len counts the step's tokens. Tables, lengths and starts are
+ * read by the kernels: an entry out of range is not followed (a page index is
+ * taken as page 0, a length is cut to the table, a row is left out or, for
+ * rope, written as NaN), and busfill_stream_status reports
+ * BUSFILL_ERR_DEVICE_INDEX.
+ * `dtype` is BUSFILL_TYPE_F16 or BUSFILL_TYPE_BF16 and holds for every 16-bit
+ * tensor of the call; strides count elements, channels are contiguous.
+ * ------------------------------------------------------------------------- */
+#define BUSFILL_KV4_PAGE 64
+#define BUSFILL_KV4_MAX_BATCH 1024
+typedef struct busfill_kv4 {
+  uint8_t* pages;         /* [num_pages][heads][72 * head_dim], 16-byte aligned */
+  const int32_t* table;   /* [batch][table_cols] page numbers */
+  const int32_t* kv_len;  /* [batch] cached tokens */
+  int num_pages, table_cols;
+  int batch;              /* sequences, 1..BUSFILL_KV4_MAX_BATCH */
+  int heads, head_dim;    /* key/value heads; 64, 128 or 256 */
+} busfill_kv4;
+
+/* Bytes of one page of one head (72 * head_dim), or BUSFILL_ERR_SHAPE. */
+BUSFILL_API int busfill_kv4_page_bytes(int head_dim);
+
+/* Rotary positions with several axes. Frequency i of rot/2 turns the channel
+ * pair (i, i + rot/2), or (2i, 2i + 1) with `adjacent`, of every head by the
+ * angle of position positions[axis[i]][token]:
+ *   y0 = x0 cos - x1 sin,  y1 = x1 cos + x0 sin
+ * with cos/sin [max_pos][rot/2] fp32 tables, in fp32, rounded once. Channels
+ * from rot on are copied. `inverse` turns back (which is also the gradient).
+ * One call takes the queries and the keys; k may be NULL (k_heads 0). Outputs
+ * may be the inputs. `axis` is a HOST array of rot/2 entries below `axes`
+ * (text has one axis; images and video two to four: time, height, width). */
+typedef struct busfill_rope {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const int32_t* positions;   /* [axes][tokens] */
+  const float *cos, *sin;     /* [max_pos][rot / 2] */
+  const uint8_t* axis;        /* host, [rot / 2] */
+  int64_t q_token, q_head, k_token, k_head;                  /* strides, elements */
+  int64_t q_out_token, q_out_head, k_out_token, k_out_head;
+  int tokens, q_heads, k_heads, head_dim; /* head_dim <= 512 */
+  int rot;                    /* even, 2..head_dim and <= 512 */
+  int axes;                   /* 1..4 */
+  int max_pos;
+  int adjacent, inverse;
+  int dtype;
+} busfill_rope;
+BUSFILL_API int busfill_rope_axes(const busfill_rope* r, void* stream);
+
+/* Quantizes the step's keys and values k, v [tokens][heads][head_dim] into
+ * the slots of their sequences' newest tokens. */
+typedef struct busfill_kv4_rows {
+  const void *k, *v;
+  const int32_t* q_start;     /* [batch + 1], or NULL: tokens == batch */
+  int64_t k_token, k_head, v_token, v_head;  /* strides, elements */
+  int tokens;
+  int dtype;
+} busfill_kv4_rows;
+BUSFILL_API int busfill_kv4_append(const busfill_kv4* cache, const busfill_kv4_rows* rows, void* stream);
+
+/* The values that the newest tokens of every sequence have in the cache (the
+ * rows of q_start; for whole sequences, pass the running sum of kv_len): k, v
+ * [tokens][heads][head_dim] fp16, exact. */
+BUSFILL_API int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_start, int tokens, uint16_t* k, uint16_t* v,
+                                 void* stream);
+
+/* Attention of q [tokens][q_heads][head_dim] over the cache; query head h
+ * reads key/value head h / (q_heads / heads).
+ *   out = sum_s p_s v_s,  p = softmax(scale * q k_s)
+ * over the slots that a row sees: all of its sequence, with `causal` those up
+ * to its own, with window > 0 (needs causal) the last `window` of these. A
+ * row that sees nothing is 0 (its lse -inf). Scores, softmax statistics and
+ * sums are fp32. lse (optional, [tokens][q_heads]) gets log(sum exp(score)).
+ * weights (optional, fp32 [batch][heads][weights_cols]): the weight that the
+ * call's rows give slot s of their sequence, summed over rows and over the
+ * heads of the group, is added to weights[.][.][s]; needs lse, and
+ * weights_cols >= 64 * table_cols. All results are bitwise repeatable. The
+ * first call on a stream makes its workspace (not inside a graph capture:
+ * BUSFILL_ERR_ALLOC). */
+typedef struct busfill_attn {
+  const void* q;
+  void* out;
+  float* lse;
+  float* weights;
+  const int32_t* q_start;     /* [batch + 1], or NULL: tokens == batch */
+  int64_t q_token, q_head, out_token, out_head, weights_cols;
+  float scale;
+  int tokens, q_heads;
+  int max_q;                  /* bound on the rows of one sequence */
+  int causal, window;
+  int dtype;
+} busfill_attn;
+BUSFILL_API int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stream);
+
+/* Eviction by accumulated attention weight, for each sequence and head by
+ * itself: of a sequence longer than `keep`, the last `recent` tokens stay and
+ * of the others the keep - recent with the largest weights (the lower slot of
+ * equals; NaN counts as the least). The kept tokens move, in their order, to
+ * slots 0 .. keep - 1 of out_table (the same table as the cache's: in place,
+ * with out_cols == table_cols; or pages that the cache's sequences do not
+ * use). index [batch][heads][keep] gets the slots they came from (-1 behind a
+ * shorter sequence's), weights_out [batch][heads][weights_cols] their weights
+ * with zeros behind (it may be `weights`), kv_len_out [batch] the new lengths
+ * (not the cache's kv_len). */
+typedef struct busfill_kv4_eviction {
+  const float* weights;
+  float* weights_out;
+  int64_t weights_cols;       /* >= 64 * table_cols */
+  int32_t* index;
+  int32_t* kv_len_out;
+  const int32_t* out_table;   /* [batch][out_cols], out_cols * 64 >= keep */
+  int out_cols;
+  int keep, recent;           /* 1 <= keep, 0 <= recent <= keep */
+} busfill_kv4_eviction;
+BUSFILL_API int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Status, options, diagnostics
  * ------------------------------------------------------------------------- */
 
 /* Synchronizes `stream`, then reports (and clears) the device-side error word
- * of the workspace bound to this stream: BUSFILL_OK, BUSFILL_ERR_DEVICE_TIMEOUT
+ * of the workspace bound to this stream: BUSFILL_OK, BUSFILL_ERR_DEVICE_TIMEOUT,
+ * BUSFILL_ERR_DEVICE_INDEX (an out-of-range index was met and not followed)
  * or BUSFILL_ERR_CUDA. The reference has no error reporting at all
  * (kernels/busfill_v1a.cu:155-158 only prints launch/sync strings). */
 BUSFILL_API int busfill_stream_status(void* stream);
@@ -367,7 +520,8 @@ BUSFILL_API int busfill_stream_status(void* stream);
 /* As busfill_stream_status, and also stores the device error word (0 when
  * clean) in *bits if bits is not NULL: one bit per kernel role whose bounded
  * wait expired (1 weight producer, 2 activation producer, 4 MMA issuer,
- * 8 dequant, 16 epilogue, 32 teardown, 64 activation stage). */
+ * 8 dequant, 16 epilogue, 32 teardown, 64 activation stage), or 256 for an
+ * index out of range (BUSFILL_ERR_DEVICE_INDEX if it stands alone). */
 BUSFILL_API int busfill_stream_status_ex(void* stream, unsigned* bits);
 
 /* Detail word of the first bounded wait that expired in the last failing
