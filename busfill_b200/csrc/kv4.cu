@@ -9,6 +9,7 @@
 #include "busfill.h"
 #include "kv4_attn.cuh"
 #include "kv4_cache.cuh"
+#include "kv4_prompt.cuh"
 
 using namespace busfill;
 using namespace busfill::kv4;
@@ -50,6 +51,10 @@ bool raise_smem(Kernel kernel, int bytes, int dev, std::once_flag (&once)[64], c
   return err[dev & 63] == cudaSuccess;
 }
 
+// Query rows of the widest sequence and head from which the tcgen05 kernel
+// takes the call.
+constexpr int kPromptRows = 33;
+
 constexpr long long kMaxGrid = 2147483647;
 
 // Query rows of the widest sequence and head from which two row tiles share a
@@ -64,6 +69,9 @@ size_t workspace_bytes(int sms) {
   f = std::max(f, part_floats<128, 1>());
   f = std::max(f, part_floats<128, 2>());
   f = std::max(f, part_floats<256, 1>());
+  f = std::max(f, (size_t)2 * prompt::Geo<64>::kPartFloats);
+  f = std::max(f, (size_t)2 * prompt::Geo<128>::kPartFloats);
+  f = std::max(f, (size_t)2 * prompt::Geo<256>::kPartFloats);
   return kCounterBytes + (size_t)sms * f * sizeof(float);
 }
 
@@ -76,6 +84,17 @@ int launch_attn(const AttnParams& p, const host::Context& ctx, cudaStream_t s) {
   void* args[] = {const_cast<AttnParams*>(&p)};
   return host::launch(reinterpret_cast<const void*>(attn_kernel<D, NT>), dim3(ctx.sms), dim3(G::kWarps * 32),
                       G::kBytes, s, args);
+}
+
+template <int D>
+int launch_prompt(const AttnParams& p, const host::Context& ctx, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  constexpr int bytes = prompt::Geo<D>::kAlloc;
+  if (!raise_smem(prompt_kernel<D>, bytes, ctx.dev, once, err)) return BUSFILL_ERR_LAUNCH;
+  void* args[] = {const_cast<AttnParams*>(&p)};
+  return host::launch(reinterpret_cast<const void*>(prompt_kernel<D>), dim3(ctx.sms), dim3(prompt::kThreads), bytes, s,
+                      args);
 }
 
 }  // namespace
@@ -230,8 +249,9 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
   p.error = ctx.error;
   if (ctx.sms > (int)(kCounterBytes / 4)) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
-  const bool two = p.max_q * p.group >= kTwoTileRows;
+  const bool many = p.max_q * p.group >= kPromptRows, two = p.max_q * p.group >= kTwoTileRows;
   st = by_dim(cache->head_dim, [&](auto d) {
+    if (many) return launch_prompt<d()>(p, ctx, s);
     if constexpr (d() < 256) {
       if (two) return launch_attn<d(), 2>(p, ctx, s);
     }

@@ -1,0 +1,692 @@
+// Attention over the 4-bit cache for many query rows per sequence and head
+// (prompts), on tcgen05.
+//
+// The same sums as kv4_attn.cuh, in the regime that the tensor pipe bounds:
+// 4 R L D flops for R query rows and L tokens against one pass of 9/8 L D bytes.
+// A work item is 128 or 256 query rows (rows of one key/value head: tokens x
+// heads of the group) against the tokens that they see, in tiles of kTile
+// tokens:
+//   S_i = Q_i K^T    (SS: both operands in shared memory, 128-byte swizzle)
+//   P_i = exp2(S_i f - m)   in registers, one row per thread; fp16 into TMEM
+//                    over S_i's columns
+//   O_i += P_i V     (TS: P from TMEM; V as it lies in the cache, token by
+//                    token, is the MN-major operand)
+// The two row tiles i = 0, 1 take turns: while one's S is in the softmax
+// threads, the tensor pipe works on the other. Codes are dequantized once per
+// tile and CTA into a ring of fp16 operands, exactly ((c - 8) d has at most 11
+// significant bits). O is rescaled only when a row's maximum has grown by more
+// than 2^8 since the last time (p stays below 2^8, far inside fp16).
+//
+// Warps: 0 copies raw pages into a ring (bulk copies); 1 issues the MMAs and
+// owns TMEM; 4-7 and 8-11 softmax of row tile 0 and 1, thread = row; 12-15
+// dequantize. Registers move from the other warps to the softmax.
+//
+// Work split: the list of all items' tiles is cut into equal ranges, one per
+// CTA of a persistent grid, so ragged and causal shapes balance by themselves;
+// an item that is cut leaves fp32 partial sums in the workspace, which the
+// CTA that finishes last joins in the order of the ranges (repeatable).
+//
+// Every wait is bounded (ptx.cuh: kWaitTimeoutNs).
+#pragma once
+
+#include "kv4_attn.cuh"
+
+namespace busfill {
+namespace kv4 {
+
+// D[tmem] (+)= A[smem] B[smem]^T, kind::f16
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// MN-major, 128-byte swizzle: rows of 64 MN values (128 B) per K index, 8-row
+// atoms of 1024 B along K (stride byte offset), blocks of 64 MN values
+// `block_bytes` apart (leading byte offset).
+__device__ __forceinline__ uint64_t make_sdesc_mn_sw128(uint32_t saddr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(block_bytes >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
+
+// 32 consecutive fp32 columns of this warp's lanes
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+namespace prompt {
+
+constexpr int kThreads = 512;
+constexpr int kSoftmaxWarp0 = 4, kDequantWarp0 = 12;
+constexpr float kLag = 8.0f;   // log2 growth of a row's maximum that O is not rescaled for
+
+template <int D>
+struct Geo {
+  using F = Fmt<D>;
+  static constexpr int kTile = D == 256 ? 64 : 128;        // tokens of a tile
+  static constexpr int kRowTiles = D == 256 ? 1 : 2;       // row tiles of 128 rows
+  static constexpr int kRows = 128 * kRowTiles;
+  static constexpr int kChunks = D / 64;                   // 128-byte column chunks
+  static constexpr int kTilePages = kTile / kPage;
+  static constexpr int kHalfPage = 36 * D;                 // keys (or values) of a page, scales behind
+  static constexpr int kRawBytes = kTilePages * kHalfPage;
+  static constexpr int kSlots = 4;                         // dequantized half tiles
+  static constexpr int kRawStages = D == 64 ? 6 : 3;
+  static constexpr int kSlotBytes = kTile * D * 2;
+  static constexpr int kQTileBytes = 128 * D * 2;
+  // shared memory
+  static constexpr int kSlotOff = 0;
+  static constexpr int kQOff = kSlotOff + kSlots * kSlotBytes;
+  static constexpr int kRawOff = kQOff + kRowTiles * kQTileBytes;
+  static constexpr int kFacOff = kRawOff + kRawStages * kRawBytes;      // factor of every row
+  static constexpr int kBarOff = kFacOff + kRows * 4;
+  static constexpr int bRawFull = 0, bRawEmpty = bRawFull + kRawStages, bKvFull = bRawEmpty + kRawStages,
+                       bKvEmpty = bKvFull + kSlots, bS = bKvEmpty + kSlots, bP = bS + 2, bO = bP + 2, bQ = bO + 2,
+                       bFinal = bQ + 2, kBars = bFinal + 1;
+  static constexpr int kMiscOff = kBarOff + kBars * 8;
+  static constexpr int kPreOff = kMiscOff + 16;            // tiles before each sequence
+  static constexpr int kBytes = kPreOff + (kMaxBatch + 1) * 4;
+  static constexpr int kAlloc = kBytes + 1024;
+  static_assert(kAlloc <= 232448, "dynamic shared memory");
+  // TMEM columns
+  static constexpr int kS = 0, kO = kRowTiles * kTile;
+  static_assert(kO + kRowTiles * D <= 512, "TMEM");
+  // a partial result: O [D][rows], m [rows], l [rows]
+  static constexpr int kPartFloats = kRows * (D + 2);
+};
+
+// An item: rows [row0, row0 + kRows) of (sequence, head); tiles [tile0, tile0 + tiles).
+struct Item {
+  int b, head, t;      // t: row tile pair of the sequence
+  int groups;          // of the sequence
+  int tile0, tiles;
+  Span s;
+};
+
+template <int D>
+__device__ __forceinline__ int groups_of(const AttnParams& p, const Span& s) {
+  return s.len > 0 ? (s.n * p.group + Geo<D>::kRows - 1) / Geo<D>::kRows : 0;
+}
+// the tiles that some row of group t sees (one, all masked, if they see nothing)
+template <int D>
+__device__ __forceinline__ int tiles_of(const AttnParams& p, const Span& s, int t, int& tile0) {
+  constexpr int R = Geo<D>::kRows, K = Geo<D>::kTile;
+  const int i0 = t * R / p.group, i1 = min(s.n - 1, (t * R + R - 1) / p.group);
+  int lo, hi, x;
+  sees(p, s, i0, lo, x);
+  sees(p, s, i1, x, hi);
+  tile0 = min(lo, s.len - 1) / K;
+  return max(1, (hi + K - 1) / K - tile0);
+}
+
+}  // namespace prompt
+
+template <int D>
+__global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __grid_constant__ AttnParams p) {
+  using namespace prompt;
+  using G = prompt::Geo<D>;
+  using F = Fmt<D>;
+  constexpr int K = G::kTile, RT = G::kRowTiles, NB = F::kBlocks;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_s = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_s + 1023u) & ~1023u) - raw_s);
+  const uint32_t sbase = smem_u32(smem);
+  auto BAR = [&](int i) { return sbase + G::kBarOff + 8u * (uint32_t)i; };
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + G::kMiscOff);   // [0] TMEM base, [1] "last" flag
+  int* pre = reinterpret_cast<int*>(smem + G::kPreOff);
+  float* factors = reinterpret_cast<float*>(smem + G::kFacOff);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = p.c.batch;
+
+  if (warp == 0) {
+    for (int i = lane; i < G::kBars; i += 32) {
+      const bool warps4 = (i >= G::bRawEmpty && i < G::bKvEmpty) || (i >= G::bP && i < G::bP + 2) ||
+                          (i >= G::bQ && i < G::bQ + 2);
+      mbar_init(BAR(i), warps4 ? 4 : 1);
+    }
+    fence_mbar_init();
+  } else if (warp == 1) {
+    tmem_alloc(sbase + G::kMiscOff, 512);
+    tmem_relinquish();
+  }
+  pdl_wait_prerequisites();
+  pdl_launch_dependents();
+  // tiles of every sequence (a warp each), then their running sum
+  bool bad = false;
+  for (int b = warp; b < batch; b += kThreads / 32) {
+    const Span s = span_of(p, b, bad);
+    const int groups = groups_of<D>(p, s);
+    int n = 0, x;
+    for (int t = lane; t < groups; t += 32) n += tiles_of<D>(p, s, t, x);
+    n = __reduce_add_sync(0xffffffffu, n) * p.c.heads;
+    if (lane == 0) pre[b + 1] = n;
+    if (s.len == 0 && blockIdx.x == 0) {   // nothing cached: rows are 0
+      for (int r = lane; r < s.n * p.q_heads; r += 32) {
+        const int i = r / p.q_heads, h = r - i * p.q_heads;
+        for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, h / p.group, i * p.group + h % p.group, ch, 0.0f);
+        store_lse(p, s, h / p.group, i * p.group + h % p.group, 0.0f, 0.0f);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {
+    int total = 0;
+    if (lane == 0) pre[0] = 0;
+    for (int b0 = 0; b0 < batch; b0 += 32) {
+      int x = b0 + lane < batch ? pre[b0 + lane + 1] : 0;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, m);
+        if (lane >= m) x += y;
+      }
+      if (b0 + lane < batch) pre[b0 + lane + 1] = total + x;
+      total += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = misc[0];
+  const int T = pre[batch];
+  const long long ctas = min((int)gridDim.x, T);
+  const bool idle = (int)blockIdx.x >= ctas;
+  const int u0 = idle ? 0 : (int)((long long)T * blockIdx.x / ctas);
+  const int u1 = idle ? 0 : (int)((long long)T * (blockIdx.x + 1) / ctas);
+
+  // the item of tile u0 and where in it u0 lies (all warps alike)
+  Item first{};
+  int skip = 0;   // tiles of the first item that belong to CTAs before
+  if (u0 < u1) {
+    int lo = 0, hi = batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (pre[mid] <= u0 ? lo : hi) = mid;
+    }
+    first.b = lo;
+    first.s = span_of(p, lo, bad);
+    first.groups = groups_of<D>(p, first.s);
+    const int per_head = (pre[lo + 1] - pre[lo]) / p.c.heads;
+    int r = u0 - pre[lo];
+    first.head = r / per_head;
+    r -= first.head * per_head;
+    for (int t0 = 0;; t0 += 32) {
+      int x0;
+      const int n = t0 + lane < first.groups ? tiles_of<D>(p, first.s, t0 + lane, x0) : 0;
+      int x = n;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, m);
+        if (lane >= m) x += y;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, x > r);
+      if (over) {
+        const int k = __ffs(over) - 1;
+        first.t = t0 + k;
+        skip = r - __shfl_sync(0xffffffffu, x - n, k);
+        break;
+      }
+      r -= __shfl_sync(0xffffffffu, x, 31);
+    }
+    first.tiles = tiles_of<D>(p, first.s, first.t, first.tile0);
+  }
+  // step to the item behind `it`
+  auto next_item = [&](Item& it) {
+    if (++it.t == it.groups) {
+      it.t = 0;
+      if (++it.head == p.c.heads) {
+        it.head = 0;
+        do ++it.b;
+        while (it.b < batch && pre[it.b + 1] == pre[it.b]);
+        if (it.b >= batch) return;
+        it.s = span_of(p, it.b, bad);
+        it.groups = groups_of<D>(p, it.s);
+      }
+    }
+    it.tiles = tiles_of<D>(p, it.s, it.t, it.tile0);
+  };
+  // for every piece (part of an item) of this CTA: f(item, first tile, tiles, whole)
+  auto for_pieces = [&](auto f) {
+    Item it = first;
+    int from = skip;
+    for (int u = u0; u < u1;) {
+      const int n = min(it.tiles - from, u1 - u);
+      if (!f(it, from, n, u)) return;
+      u += n;
+      from = 0;
+      if (u < u1) next_item(it);
+    }
+  };
+  auto row_tiles = [&](const Item& it) { return RT == 2 && it.s.n * p.group - it.t * G::kRows > 128 ? 2 : 1; };
+
+  bool ok = true;
+  auto wait = [&](int bar, uint32_t phase) -> bool {   // the warp waits for completion number `phase` of the barrier
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(BAR(bar), phase & 1));
+    return ok;
+  };
+  auto failed = [&](unsigned bit) {
+    if (lane == 0) atomicOr(p.error, bit);
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 0) {
+      // ---------------- raw pages ----------------
+      uint32_t n = 0;
+      for_pieces([&](const Item& it, int from, int tiles, int) {
+        const int pages = (it.s.len + kPage - 1) / kPage;
+        for (int j = 0; j < tiles; ++j) {
+          const int page0 = (it.tile0 + from + j) * G::kTilePages;
+          const int have = min(G::kTilePages, pages - page0);
+          const uint8_t* src[G::kTilePages];
+#pragma unroll
+          for (int k = 0; k < G::kTilePages; ++k)
+            src[k] = p.c.pages + ((size_t)(k < have ? page_of(p.c, p.c.table, p.c.table_cols, it.b, page0 + k, bad) : 0) *
+                                      p.c.heads + it.head) * F::kPageBytes;
+#pragma unroll
+          for (int half = 0; half < 2; ++half, ++n) {
+            const int st = n % G::kRawStages;
+            if (!wait(G::bRawEmpty + st, n / G::kRawStages + 1)) return false;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(BAR(G::bRawFull + st), have * G::kHalfPage);
+#pragma unroll
+              for (int k = 0; k < G::kTilePages; ++k)
+                if (k < have)
+                  bulk_load(sbase + G::kRawOff + st * G::kRawBytes + k * G::kHalfPage, src[k] + half * G::kHalfPage,
+                            G::kHalfPage, BAR(G::bRawFull + st));
+            }
+            __syncwarp();
+          }
+        }
+        return true;
+      });
+      if (!ok) failed(1u);
+      // nothing may land after the CTA is gone
+      ok = true;
+      for (uint32_t k = n > G::kRawStages ? n - G::kRawStages : 0; k < n; ++k)
+        if (!wait(G::bRawFull + k % G::kRawStages, k / G::kRawStages)) break;
+    } else if (warp == 1) {
+      // ---------------- MMA ----------------
+      constexpr uint32_t kIdescS = make_idesc_f16_f32(128, K), kIdescO = make_idesc_f16_f32(128, D) | kIdescBMnMajor;
+      uint32_t half = 0;             // half tiles consumed
+      uint32_t done[2] = {0, 0};     // tiles of row tile i whose P was waited for
+      uint32_t items[2] = {0, 0};
+      auto issue_s = [&](int i, uint32_t slot) {
+        const uint32_t a = sbase + G::kQOff + i * G::kQTileBytes, b = sbase + G::kSlotOff + slot * G::kSlotBytes;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ss(tmem + G::kS + i * K, make_sdesc_sw128(a + (k / 4) * 128 * 128 + (k % 4) * 32),
+                     make_sdesc_sw128(b + (k / 4) * K * 128 + (k % 4) * 32), kIdescS, k > 0);
+        tc_commit(BAR(G::bS + i));
+      };
+      for_pieces([&](const Item& it, int, int tiles, int) {
+        const int nr = row_tiles(it);
+        for (int i = 0; i < nr; ++i)
+          if (!wait(G::bQ + i, items[i]++)) return false;
+        if (!wait(G::bKvFull + half % G::kSlots, half / G::kSlots)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          for (int i = 0; i < nr; ++i) issue_s(i, half % G::kSlots);
+          tc_commit(BAR(G::bKvEmpty + half % G::kSlots));
+        }
+        __syncwarp();
+        ++half;
+        for (int j = 0; j < tiles; ++j) {
+          const uint32_t vs = half % G::kSlots, ks = (half + 1) % G::kSlots;
+          const bool more = j + 1 < tiles;
+          if (!wait(G::bKvFull + vs, half / G::kSlots)) return false;
+          if (more && !wait(G::bKvFull + ks, (half + 1) / G::kSlots)) return false;
+          for (int i = 0; i < nr; ++i) {
+            if (!wait(G::bP + i, done[i]++)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t b = sbase + G::kSlotOff + vs * G::kSlotBytes;
+#pragma unroll
+              for (int k = 0; k < K / 16; ++k)
+                mma_f16_ts(tmem + G::kO + i * D, tmem + G::kS + i * K + 8 * k,
+                           make_sdesc_mn_sw128(b + k * 16 * 128, K * 128), kIdescO, j > 0 || k > 0);
+              tc_commit(BAR(G::bO + i));
+              if (more) issue_s(i, ks);
+              if (i + 1 == nr) {
+                tc_commit(BAR(G::bKvEmpty + vs));
+                if (more) tc_commit(BAR(G::bKvEmpty + ks));
+              }
+            }
+            __syncwarp();
+          }
+          half += more ? 2 : 1;
+        }
+        return true;
+      });
+      if (!ok) failed(4u);
+      // every MMA has completed before TMEM is freed
+      ok = true;
+      tc_fence_after();
+      if (elect_one()) tc_commit(BAR(G::bFinal));
+      __syncwarp();
+      if (!wait(G::bFinal, 0)) failed(32u);
+    }
+  } else if (warp >= kDequantWarp0) {
+    // ---------------- dequantize ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int w = warp - kDequantWarp0, j = lane & 3;
+    uint32_t n = 0;
+    for_pieces([&](const Item& it, int from, int tiles, int) {
+      for (int tile = 0; tile < tiles; ++tile) {
+        const int base = (it.tile0 + from + tile) * K;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, ++n) {
+          const int st = n % G::kRawStages, slot = n % G::kSlots;
+          if (!wait(G::bRawFull + st, n / G::kRawStages)) return false;
+          if (!wait(G::bKvEmpty + slot, n / G::kSlots + 1)) return false;
+          const uint8_t* raw = smem + G::kRawOff + st * G::kRawBytes;
+          uint8_t* dst = smem + G::kSlotOff + slot * G::kSlotBytes;
+#pragma unroll
+          for (int pass = 0; pass < K / 32; ++pass) {
+            // lane j of a token's four: words j of all its blocks
+            const int tok = w * (K / 4) + pass * 8 + (lane >> 2);
+            const uint8_t* pg = raw + (tok / kPage) * G::kHalfPage;
+            const int t = tok & (kPage - 1);
+            uint32_t x[NB];
+            __half2 d[NB];
+            if (half == 0) {
+              uint32_t sc[NB / 2];
+              lds_words<NB>(pg + t * F::kRow + j * 4 * NB, x);
+              lds_words<NB / 2>(pg + F::kKeyScale + t * 2 * NB, sc);
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                d[b] = b & 1 ? __high2half2(u32_as_h2(sc[b / 2])) : __low2half2(u32_as_h2(sc[b / 2]));
+            } else {
+              uint32_t y[NB];   // value words 2j and 2j + 1 of all blocks
+              lds_words<NB>(pg + t * F::kRow + ((2 * j) ^ value_swizzle<D>(t)) * 2 * NB, y);
+              const bool live = base + tok < it.s.len;   // slots behind the sequence hold anything
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                x[b] = prmt(y[b / 2], y[NB / 2 + b / 2], b & 1 ? 0x7632u : 0x5410u);
+                const __half s = *reinterpret_cast<const __half*>(pg + 32 * D + (b * kPage + tile_perm(t)) * 2);
+                d[b] = __half2half2(live ? s : __ushort_as_half(0));
+              }
+            }
+            // odd tokens write their blocks in swapped pairs, so that the 8
+            // lanes of a store phase cover all banks
+            if (t & 1) {
+#pragma unroll
+              for (int b = 0; b < NB; b += 2) {
+                const uint32_t tx = x[b];
+                x[b] = x[b + 1], x[b + 1] = tx;
+                const __half2 td = d[b];
+                d[b] = d[b + 1], d[b + 1] = td;
+              }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const int blk = b ^ (t & 1);
+              const int piece = 4 * (blk & 1) + j;   // 16-byte piece of the 128-byte row
+              *reinterpret_cast<uint4*>(dst + (b >> 1) * K * 128 + tok * 128 + ((piece ^ (tok & 7)) << 4)) =
+                  dequant_key8(x[b], d[b], minus_72(d[b]));
+            }
+          }
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(BAR(G::bRawEmpty + st));
+            mbar_arrive(BAR(G::bKvFull + slot));
+          }
+        }
+      }
+      return true;
+    });
+    if (!ok) failed(8u);
+  } else {
+    // ---------------- softmax ----------------
+    // A warp whose wait ran out goes on through its pieces without waiting or
+    // writing, so that the named barriers (no timeout) always fill.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const int i = (warp - kSoftmaxWarp0) / 4, q = warp & 3;   // row tile, lane quarter
+    const int my_row = 32 * q + lane;
+    const uint32_t tm = tmem + ((uint32_t)(32 * q) << 16);
+    const uint32_t ts = tm + G::kS + i * K, to = tm + G::kO + i * D;
+    uint32_t done = 0;
+    const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+    float* my_part = p.part + (size_t)blockIdx.x * 2 * G::kPartFloats;
+    for_pieces([&](const Item& it, int from, int tiles, int u) {
+      const bool active = i < row_tiles(it);
+      const int row0 = it.t * G::kRows + i * 128;
+      const int row = row0 + my_row;
+      float m = -INFINITY, l = 0.0f;
+      if (active) {
+        // queries: lanes together on a row, 16 bytes each
+        constexpr int LPR = D / 8, RPI = 32 / LPR;
+        const int c = lane % LPR;
+#pragma unroll 4
+        for (int k = 0; k < 32; k += RPI) {
+          const int r = 32 * q + k + lane / LPR;
+          const int tok = (row0 + r) / p.group;
+          const bool live = tok < it.s.n;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (live)
+            v = __ldg(reinterpret_cast<const uint4*>(
+                static_cast<const uint16_t*>(p.q) + (size_t)(it.s.first + tok) * p.q_token +
+                (size_t)(it.head * p.group + row0 + r - tok * p.group) * p.q_head + 8 * c));
+          float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);
+          float up = sign;
+          if (p.bf16) {
+            float x[8];
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            float top = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              x[2 * y] = __uint_as_float(e[y] << 16);
+              x[2 * y + 1] = __uint_as_float(e[y] & 0xffff0000u);
+              top = fmaxf(top, fmaxf(fabsf(x[2 * y]), fabsf(x[2 * y + 1])));
+            }
+#pragma unroll
+            for (int y = 1; y < LPR; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+            // a power of two brings the row's maximum to [2^9, 2^10): fp16 then
+            // holds what bf16 held
+            int ex = 136 - (int)(__float_as_uint(top) >> 23);
+            if (top == 0.0f || !(top <= 3.4e38f)) ex = 0;
+            ex = max(-126, min(126, ex));
+            up *= __uint_as_float((unsigned)(127 + ex) << 23);
+            fac *= __uint_as_float((unsigned)(127 - ex) << 23);
+            v.x = h2_as_u32(__floats2half2_rn(x[0] * up, x[1] * up));
+            v.y = h2_as_u32(__floats2half2_rn(x[2] * up, x[3] * up));
+            v.z = h2_as_u32(__floats2half2_rn(x[4] * up, x[5] * up));
+            v.w = h2_as_u32(__floats2half2_rn(x[6] * up, x[7] * up));
+          } else if (sign < 0.0f) {
+            v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+          }
+          *reinterpret_cast<uint4*>(smem + G::kQOff + i * G::kQTileBytes + (c / 8) * 128 * 128 + r * 128 +
+                                    (((c & 7) ^ (r & 7)) << 4)) = v;
+          if (c == 0) factors[i * 128 + r] = fac;
+        }
+        fence_proxy_async_shared();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(G::bQ + i));
+        const float f = factors[i * 128 + my_row];
+        int lo = 0, hi = 0x7fffffff;
+        const int tok = row / p.group;
+        if (tok < it.s.n) sees(p, it.s, tok, lo, hi);
+
+        for (int j = 0; j < tiles; ++j, ++done) {
+          const int base = (it.tile0 + from + j) * K;
+          if (!wait(G::bS + i, done)) break;
+          tc_fence_after();
+          float s[K];
+#pragma unroll
+          for (int c2 = 0; c2 < K; c2 += 32) tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(s) + c2);
+          tc_wait_ld();
+          if (!__all_sync(0xffffffffu, lo <= base && base + K <= hi)) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) s[k] = base + k >= lo && base + k < hi ? s[k] : -INFINITY;
+          }
+          float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < K; ++k) top[k & 3] = fmaxf(top[k & 3], s[k]);
+          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+          if (j == 0) {
+            m = mt;
+          } else if (__any_sync(0xffffffffu, mt > m + kLag || (m == -INFINITY && mt > m))) {
+            const float m2 = fmaxf(m, mt);
+            const float a = m == m2 ? 1.0f : exp2_approx(m - m2);
+            m = m2;
+            l *= a;
+            if (!wait(G::bO + i, done - 1)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c2 = 0; c2 < D; c2 += 32) {
+              uint32_t o[32];
+              tmem_ld_x32(to + c2, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
+              tmem_st_x32(to + c2, o);
+            }
+          }
+          const float off = m == -INFINITY ? 0.0f : -m;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c2 = 0; c2 < K; c2 += 64) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int k = 0; k < 64; k += 2) {
+              const float x = exp2_approx(fmaf(s[c2 + k], f, off)), y = exp2_approx(fmaf(s[c2 + k + 1], f, off));
+              sum[k & 2] += x;
+              sum[(k & 2) + 1] += y;
+              pk[k / 2] = h2_as_u32(__floats2half2_rn(x, y));
+            }
+            tmem_st_x32(ts + c2 / 2, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(G::bP + i));
+        }
+        if (ok) wait(G::bO + i, done - 1);
+        tc_fence_after();
+      }
+      // 32 columns of this thread's output row
+      const int my_tok = row / p.group;
+      const bool live = ok && active && my_tok < it.s.n;
+      const size_t out_at = live ? (size_t)(it.s.first + my_tok) * p.o_token +
+                                       (size_t)(it.head * p.group + row - my_tok * p.group) * p.o_head
+                                 : 0;
+      auto put32 = [&](int c2, const float* x, float scale) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          uint32_t e[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float a = x[k + 2 * y] * scale, b = x[k + 2 * y + 1] * scale;
+            if (p.bf16) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+              e[y] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+              e[y] = h2_as_u32(__floats2half2_rn(a, b));
+            }
+          }
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + out_at + c2 + k) = make_uint4(e[0], e[1], e[2], e[3]);
+        }
+      };
+      if (from == 0 && tiles == it.tiles) {
+        if (active) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+          for (int c2 = 0; c2 < D; c2 += 32) {   // TMEM loads take the whole warp
+            float o[32];
+            tmem_ld_x32(to + c2, reinterpret_cast<uint32_t*>(o));
+            tc_wait_ld();
+            if (live) put32(c2, o, inv);
+          }
+          if (live) store_lse(p, it.s, it.head, row, m, l);
+        }
+        return true;
+      }
+      // a cut item: slot 0 if it began before this CTA's range, slot 1 if it goes on behind it
+      const int r = i * 128 + my_row;
+      float* to_part = my_part + (size_t)(from > 0 ? 0 : 1) * G::kPartFloats;
+      if (active) {
+#pragma unroll 1
+        for (int c2 = 0; c2 < D; c2 += 32) {
+          uint32_t o[32];
+          tmem_ld_x32(to + c2, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) to_part[(c2 + k) * G::kRows + r] = __uint_as_float(o[k]);
+        }
+        to_part[D * G::kRows + r] = m;
+        to_part[(D + 1) * G::kRows + r] = l;
+      }
+      __threadfence();
+      named_bar_sync(1, 128 * 2);
+      const int item0 = u - from, end = item0 + it.tiles;
+      const int c_first = (int)((((long long)item0 + 1) * ctas - 1) / T), c_last = (int)(((long long)end * ctas - 1) / T);
+      if (threadIdx.x == 32 * kSoftmaxWarp0)
+        misc[1] = atom_add_acq_rel_gpu(p.counters + c_first, 1u) == (unsigned)(c_last - c_first) ? 1u : 0u;
+      named_bar_sync(1, 128 * 2);
+      if (misc[1]) {
+        __threadfence();
+        const int n = c_last - c_first + 1;
+        auto theirs = [&](int k) {
+          return p.part + ((size_t)(c_first + k) * 2 + (k == 0 ? 1 : 0)) * G::kPartFloats;
+        };
+        if (live) {
+          float mm = -INFINITY, ll = 0.0f;
+          for (int k = 0; k < n; ++k) mm = fmaxf(mm, __ldcg(theirs(k) + D * G::kRows + r));
+          // a piece that saw nothing has m = -inf, l = 0 and o = 0
+          auto share = [&](int k) {
+            const float mk = __ldcg(theirs(k) + D * G::kRows + r);
+            return mk == -INFINITY ? 1.0f : exp2_approx(mk - mm);
+          };
+          for (int k = 0; k < n; ++k) ll = fmaf(__ldcg(theirs(k) + (D + 1) * G::kRows + r), share(k), ll);
+          const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll 1
+          for (int c2 = 0; c2 < D; c2 += 32) {
+            float x[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = 0.0f;
+            for (int y = 0; y < n; ++y) {
+              const float a = share(y);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] = fmaf(__ldcg(theirs(y) + (c2 + k) * G::kRows + r), a, x[k]);
+            }
+            put32(c2, x, inv);
+          }
+          store_lse(p, it.s, it.head, row, mm, ll);
+        }
+        if (threadIdx.x == 32 * kSoftmaxWarp0) p.counters[c_first] = 0;
+      }
+      named_bar_sync(1, 128 * 2);
+      return true;
+    });
+    if (!ok) failed(16u);
+  }
+  if (bad) atomicOr(p.error, kErrIndex);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace kv4
+}  // namespace busfill
