@@ -10,6 +10,7 @@
 #include "kv4_attn.cuh"
 #include "kv4_cache.cuh"
 #include "kv4_prompt.cuh"
+#include "kv4_weights.cuh"
 
 using namespace busfill;
 using namespace busfill::kv4;
@@ -95,6 +96,17 @@ int launch_prompt(const AttnParams& p, const host::Context& ctx, cudaStream_t s)
   void* args[] = {const_cast<AttnParams*>(&p)};
   return host::launch(reinterpret_cast<const void*>(prompt_kernel<D>), dim3(ctx.sms), dim3(prompt::kThreads), bytes, s,
                       args);
+}
+
+template <int D>
+int launch_weights(const AttnParams& p, const host::Context& ctx, cudaStream_t s, bool many) {
+  void* args[] = {const_cast<AttnParams*>(&p)};
+  if (!many) return host::launch((const void*)weights_kernel<D>, dim3(ctx.sms * 4), dim3(256), 0, s, args);
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  constexpr int bytes = wsum::Geo<D>::kAlloc;
+  if (!raise_smem(weights_prompt_kernel<D>, bytes, ctx.dev, once, err)) return BUSFILL_ERR_LAUNCH;
+  return host::launch((const void*)weights_prompt_kernel<D>, dim3(ctx.sms), dim3(wsum::kThreads), bytes, s, args);
 }
 
 }  // namespace
@@ -258,10 +270,7 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
     return launch_attn<d(), 1>(p, ctx, s);
   });
   if (st != BUSFILL_OK || !a->weights) return st;
-  void* args[] = {&p};
-  return by_dim(cache->head_dim, [&](auto d) {
-    return host::launch((const void*)weights_kernel<d()>, dim3(ctx.sms * 4), dim3(256), 0, s, args);
-  });
+  return by_dim(cache->head_dim, [&](auto d) { return launch_weights<d()>(p, ctx, s, many); });
 }
 
 int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, void* stream) {

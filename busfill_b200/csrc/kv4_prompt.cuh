@@ -72,6 +72,37 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 
+// Eight query elements (16-bit pairs in v) as fp16 operands: bf16 is brought to
+// a row maximum in [2^9, 2^10) by a power of two (the row is on LANES
+// neighbouring lanes), so that fp16 holds what bf16 held; fac takes its
+// inverse. sign is the scale's.
+template <int LANES>
+__device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign, float& fac) {
+  if (bf16) {
+    float x[8], up = sign, top = 0.0f;
+    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      x[2 * y] = __uint_as_float(e[y] << 16);
+      x[2 * y + 1] = __uint_as_float(e[y] & 0xffff0000u);
+      top = fmaxf(top, fmaxf(fabsf(x[2 * y]), fabsf(x[2 * y + 1])));
+    }
+#pragma unroll
+    for (int y = 1; y < LANES; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+    int ex = 136 - (int)(__float_as_uint(top) >> 23);
+    if (top == 0.0f || !(top <= 3.4e38f)) ex = 0;
+    ex = max(-126, min(126, ex));
+    up *= __uint_as_float((unsigned)(127 + ex) << 23);
+    fac *= __uint_as_float((unsigned)(127 - ex) << 23);
+    v.x = h2_as_u32(__floats2half2_rn(x[0] * up, x[1] * up));
+    v.y = h2_as_u32(__floats2half2_rn(x[2] * up, x[3] * up));
+    v.z = h2_as_u32(__floats2half2_rn(x[4] * up, x[5] * up));
+    v.w = h2_as_u32(__floats2half2_rn(x[6] * up, x[7] * up));
+  } else if (sign < 0.0f) {
+    v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+  }
+}
+
 namespace prompt {
 
 constexpr int kThreads = 512;
@@ -484,34 +515,8 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
             v = __ldg(reinterpret_cast<const uint4*>(
                 static_cast<const uint16_t*>(p.q) + (size_t)(it.s.first + tok) * p.q_token +
                 (size_t)(it.head * p.group + row0 + r - tok * p.group) * p.q_head + 8 * c));
-          float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);
-          float up = sign;
-          if (p.bf16) {
-            float x[8];
-            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-            float top = 0.0f;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              x[2 * y] = __uint_as_float(e[y] << 16);
-              x[2 * y + 1] = __uint_as_float(e[y] & 0xffff0000u);
-              top = fmaxf(top, fmaxf(fabsf(x[2 * y]), fabsf(x[2 * y + 1])));
-            }
-#pragma unroll
-            for (int y = 1; y < LPR; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
-            // a power of two brings the row's maximum to [2^9, 2^10): fp16 then
-            // holds what bf16 held
-            int ex = 136 - (int)(__float_as_uint(top) >> 23);
-            if (top == 0.0f || !(top <= 3.4e38f)) ex = 0;
-            ex = max(-126, min(126, ex));
-            up *= __uint_as_float((unsigned)(127 + ex) << 23);
-            fac *= __uint_as_float((unsigned)(127 - ex) << 23);
-            v.x = h2_as_u32(__floats2half2_rn(x[0] * up, x[1] * up));
-            v.y = h2_as_u32(__floats2half2_rn(x[2] * up, x[3] * up));
-            v.z = h2_as_u32(__floats2half2_rn(x[4] * up, x[5] * up));
-            v.w = h2_as_u32(__floats2half2_rn(x[6] * up, x[7] * up));
-          } else if (sign < 0.0f) {
-            v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-          }
+          float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
+          normalize_query8<LPR>(v, p.bf16, sign, fac);
           *reinterpret_cast<uint4*>(smem + G::kQOff + i * G::kQTileBytes + (c / 8) * 128 * 128 + r * 128 +
                                     (((c & 7) ^ (r & 7)) << 4)) = v;
           if (c == 0) factors[i * 128 + r] = fac;
