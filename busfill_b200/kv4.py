@@ -16,10 +16,10 @@ Out-of-range device indices are not followed and show in ``stream_status()``.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import struct
 
-from . import _check, _lib, _ptr, _stream, _torch
+from . import _check, _lib, _torch
 
 KV4_PAGE = 64
 
@@ -60,26 +60,48 @@ class Eviction(ctypes.Structure):
                 ("out_table", _P), ("out_cols", _I), ("keep", _I), ("recent", _I)]
 
 
-def _dtype(t):
-    torch = _torch()
-    return {torch.float16: 1, torch.bfloat16: 30}[t.dtype]
+def _packer(cls):
+    """cls's fields as native bytes: several times cheaper to make per call than the ctypes object."""
+    code = {_P: "P", _L: "q", _I: "i", ctypes.c_float: "f"}
+    return struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0q").pack
+
+
+_pack_cache, _pack_rope, _pack_rows, _pack_attn, _pack_eviction = map(_packer, (Cache, Rope, Rows, Attn, Eviction))
+_TYPE = {}   # torch dtype -> BUSFILL_TYPE_*
+
+
+def _dtype(t, name):
+    if not _TYPE:
+        torch = _torch()
+        _TYPE.update({torch.float16: 1, torch.bfloat16: 30})
+    code = _TYPE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be fp16 or bf16, got {t.dtype}")
+    return code
+
+
+def _need_cuda(t, name):
+    if not isinstance(t, _torch().Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
 
 
 def _need_heads(t, name, like=None):
-    """A step's tensor [tokens, heads, D], fp16 or bf16, channels contiguous."""
-    torch = _torch()
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype not in (torch.float16, torch.bfloat16) or (like is not None and t.dtype != like.dtype):
-        raise TypeError(f"{name} must be {'fp16 or bf16' if like is None else like.dtype}, got {t.dtype}")
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise ValueError(f"{name} must be [tokens, heads, D] with contiguous channels")
+    """A step's tensor [tokens, heads, D], fp16 or bf16, channels contiguous; (token, head) strides."""
+    _need_cuda(t, name)
+    if like is None:
+        _dtype(t, name)
+    elif t.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, D], got {tuple(t.shape)}")
+    token, head, channel = t.stride()
+    if channel != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name} must have contiguous channels")
+    return token, head
 
 
 def _need_array(t, dtype, name, ndim):
-    torch = _torch()
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
+    _need_cuda(t, name)
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != ndim or not t.is_contiguous():
@@ -87,33 +109,55 @@ def _need_array(t, dtype, name, ndim):
 
 
 def _cache(pages, table, kv_len):
+    """(busfill_kv4 as bytes, batch, heads, head_dim, table columns)"""
     torch = _torch()
     _need_array(pages, torch.uint8, "pages", 3)
     _need_array(table, torch.int32, "table", 2)
     _need_array(kv_len, torch.int32, "kv_len", 1)
-    dim, rest = divmod(pages.shape[2], 72)
+    num_pages, heads, width = pages.shape
+    batch, cols = table.shape
+    dim, rest = divmod(width, 72)
     if rest or dim not in (64, 128, 256):
         raise ValueError(f"pages must be [num_pages, kv_heads, 72 * D] with D 64, 128 or 256, got {tuple(pages.shape)}")
-    if table.shape[0] != kv_len.shape[0]:
+    if batch != kv_len.shape[0]:
         raise ValueError(f"table {tuple(table.shape)} and kv_len {tuple(kv_len.shape)} differ in batch")
-    return Cache(pages.data_ptr(), table.data_ptr(), kv_len.data_ptr(), pages.shape[0], table.shape[1],
-                 table.shape[0], pages.shape[1], dim)
+    return (_pack_cache(pages.data_ptr(), table.data_ptr(), kv_len.data_ptr(), num_pages, cols, batch, heads, dim),
+            batch, heads, dim, cols)
 
 
-def _need_start(q_start, cache, tokens):
+def _need_start(q_start, batch, tokens):
     if q_start is None:
-        if tokens != cache.batch:
-            raise ValueError(f"{tokens} rows for {cache.batch} sequences: give q_start")
-        return None
+        if tokens != batch:
+            raise ValueError(f"{tokens} rows for {batch} sequences: give q_start")
+        return 0
     _need_array(q_start, _torch().int32, "q_start", 1)
-    if q_start.shape[0] != cache.batch + 1:
-        raise ValueError(f"q_start must have {cache.batch + 1} entries, got {q_start.shape[0]}")
+    if q_start.shape[0] != batch + 1:
+        raise ValueError(f"q_start must have {batch + 1} entries, got {q_start.shape[0]}")
     return q_start.data_ptr()
 
 
-def _on(stream):
-    """Allocations inside belong to the call's stream."""
-    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
+def _need_weights(weights, name, batch, heads, cols):
+    _need_array(weights, _torch().float32, name, 3)
+    b, h, n = weights.shape
+    if b != batch or h != heads or n < KV4_PAGE * cols:
+        raise ValueError(f"{name} must be [{batch}, {heads}, >= {KV4_PAGE * cols}], got {tuple(weights.shape)}")
+    return n
+
+
+def _raw(stream, like):
+    """The cudaStream_t of the call."""
+    if stream is None:
+        return _torch()._C._cuda_getCurrentRawStream(like.get_device())
+    return stream.cuda_stream
+
+
+def _empty(stream, shape, dtype, device):
+    """A tensor that belongs to the call's stream."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def kv4_page_bytes(head_dim: int) -> int:
@@ -149,69 +193,70 @@ def rope_axes(q, k, positions, cos, sin, axis=None, adjacent=False, inverse=Fals
     ``adjacent``; channels from rot on are copied. ``inverse`` turns back, which is also the gradient.
     q_out, k_out may be q, k. Returns (q_out, k_out)."""
     torch = _torch()
-    _need_heads(q, "q")
+    q_token, q_head = _need_heads(q, "q")
+    _need_cuda(positions, "positions")
     if positions.dim() == 1:
         positions = positions[None]
     _need_array(positions, torch.int32, "positions", 2)
     _need_array(cos, torch.float32, "cos", 2)
     _need_array(sin, torch.float32, "sin", 2)
     tokens, heads, dim = q.shape
-    half = cos.shape[1]
-    axis = [0] * half if axis is None else [int(a) for a in axis]
+    max_pos, half = cos.shape
+    axes = positions.shape[0]
+    axis = bytes(half) if axis is None else bytes(axis)
     if cos.shape != sin.shape or len(axis) != half or positions.shape[1] != tokens:
         raise ValueError(f"shape mismatch: cos {tuple(cos.shape)}, sin {tuple(sin.shape)}, axis {len(axis)}, "
                          f"positions {tuple(positions.shape)}, q {tuple(q.shape)}")
-    if any(not 0 <= a < positions.shape[0] for a in axis):
-        raise ValueError(f"axis entries must be in 0..{positions.shape[0] - 1}")
+    if max(axis, default=0) >= axes:
+        raise ValueError(f"axis entries must be in 0..{axes - 1}")
+    if q_out is None:
+        q_out = _empty(stream, q.shape, q.dtype, q.device)
+    elif q_out.shape != q.shape:
+        raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+    qo_token, qo_head = _need_heads(q_out, "q_out", like=q)
+    k_ptr = ko_ptr = k_heads = k_token = k_head = ko_token = ko_head = 0
     if k is not None:
-        _need_heads(k, "k", like=q)
+        k_token, k_head = _need_heads(k, "k", like=q)
+        k_heads = k.shape[1]
         if k.shape[0] != tokens or k.shape[2] != dim:
             raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}")
-    with _on(stream):
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if k is not None and k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    for t, like, name in ((q_out, q, "q_out"), (k_out, k, "k_out")):
-        if like is not None:
-            _need_heads(t, name, like=like)
-            if t.shape != like.shape:
-                raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
-    table = (ctypes.c_uint8 * half)(*axis)
-    r = Rope(q.data_ptr(), None if k is None else k.data_ptr(), q_out.data_ptr(),
-             None if k is None else k_out.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-             ctypes.cast(table, _P), q.stride(0), q.stride(1), 0 if k is None else k.stride(0),
-             0 if k is None else k.stride(1), q_out.stride(0), q_out.stride(1), 0 if k is None else k_out.stride(0),
-             0 if k is None else k_out.stride(1), tokens, heads, 0 if k is None else k.shape[1], dim, 2 * half,
-             positions.shape[0], cos.shape[0], int(adjacent), int(inverse), _dtype(q))
-    _check(_lib().busfill_rope_axes(ctypes.byref(r), _stream(stream)), "busfill_rope_axes")
+        if k_out is None:
+            k_out = _empty(stream, k.shape, k.dtype, k.device)
+        elif k_out.shape != k.shape:
+            raise ValueError(f"k_out must be {tuple(k.shape)}, got {tuple(k_out.shape)}")
+        ko_token, ko_head = _need_heads(k_out, "k_out", like=q)
+        k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
+    table = ctypes.create_string_buffer(axis, half)
+    r = _pack_rope(q.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, positions.data_ptr(), cos.data_ptr(),
+                   sin.data_ptr(), ctypes.addressof(table), q_token, q_head, k_token, k_head, qo_token, qo_head,
+                   ko_token, ko_head, tokens, heads, k_heads, dim, 2 * half, axes, max_pos, bool(adjacent),
+                   bool(inverse), _dtype(q, "q"))
+    _check(_lib().busfill_rope_axes(r, _raw(stream, q)), "busfill_rope_axes")
     return q_out, k_out
 
 
 def kv4_append(pages, table, kv_len, k, v, q_start=None, stream=None):
     """Quantize the step's keys and values [tokens, kv_heads, D] into the slots of their sequences'
     newest tokens (row r of a sequence's n rows goes to slot kv_len - n + r)."""
-    c = _cache(pages, table, kv_len)
-    _need_heads(k, "k")
-    _need_heads(v, "v", like=k)
-    if k.shape != v.shape or k.shape[1] != c.heads or k.shape[2] != c.head_dim:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {c.heads}, {c.head_dim}]")
-    r = Rows(k.data_ptr(), v.data_ptr(), _need_start(q_start, c, k.shape[0]), k.stride(0), k.stride(1), v.stride(0),
-             v.stride(1), k.shape[0], _dtype(k))
-    _check(_lib().busfill_kv4_append(ctypes.byref(c), ctypes.byref(r), _stream(stream)), "busfill_kv4_append")
+    c, batch, heads, dim, _ = _cache(pages, table, kv_len)
+    k_token, k_head = _need_heads(k, "k")
+    v_token, v_head = _need_heads(v, "v", like=k)
+    tokens = k.shape[0]
+    if k.shape != v.shape or k.shape[1] != heads or k.shape[2] != dim:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {heads}, {dim}]")
+    r = _pack_rows(k.data_ptr(), v.data_ptr(), _need_start(q_start, batch, tokens), k_token, k_head, v_token, v_head,
+                   tokens, _dtype(k, "k"))
+    _check(_lib().busfill_kv4_append(c, r, _raw(stream, pages)), "busfill_kv4_append")
 
 
 def kv4_read(pages, table, kv_len, q_start=None, tokens=None, stream=None):
     """The exact fp16 values (k, v) [tokens, kv_heads, D] that the cache holds for the newest tokens
     of every sequence; for whole sequences let q_start be the running sum of kv_len."""
-    torch = _torch()
-    c = _cache(pages, table, kv_len)
-    tokens = c.batch if tokens is None else int(tokens)
-    start = _need_start(q_start, c, tokens)
-    with _on(stream):
-        k = torch.empty((tokens, c.heads, c.head_dim), dtype=torch.float16, device=pages.device)
-        v = torch.empty_like(k)
-    _check(_lib().busfill_kv4_read(ctypes.byref(c), start, tokens, _ptr(k), _ptr(v), _stream(stream)),
+    c, batch, heads, dim, _ = _cache(pages, table, kv_len)
+    tokens = batch if tokens is None else int(tokens)
+    start = _need_start(q_start, batch, tokens)
+    k, v = _empty(stream, (2, tokens, heads, dim), _torch().float16, pages.device).unbind()
+    _check(_lib().busfill_kv4_read(c, start, tokens, k.data_ptr(), v.data_ptr(), _raw(stream, pages)),
            "busfill_kv4_read")
     return k, v
 
@@ -226,36 +271,33 @@ def attn_kv4(q, pages, table, kv_len, q_start=None, max_q=None, scale=None, caus
     ``lse`` fp32 [tokens, q_heads] gets each row's log-sum-exp (-inf for a row that sees nothing).
     To ``weights`` fp32 [batch, kv_heads, cols >= 64 * table columns] the attention weight of every
     cached token, summed over the call's rows and the group's heads, is added."""
-    torch = _torch()
-    c = _cache(pages, table, kv_len)
-    _need_heads(q, "q")
+    c, batch, kv_heads, head_dim, cols = _cache(pages, table, kv_len)
+    q_token, q_head = _need_heads(q, "q")
     tokens, heads, dim = q.shape
-    if dim != c.head_dim or heads % c.heads:
-        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {c.heads} heads of {c.head_dim}")
-    start = _need_start(q_start, c, tokens)
+    if dim != head_dim or heads % kv_heads:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {kv_heads} heads of {head_dim}")
+    start = _need_start(q_start, batch, tokens)
+    w_ptr = w_cols = lse_ptr = 0
     if weights is not None:
-        _need_array(weights, torch.float32, "weights", 3)
-        if weights.shape[:2] != (c.batch, c.heads) or weights.shape[2] < KV4_PAGE * c.table_cols:
-            raise ValueError(f"weights must be [{c.batch}, {c.heads}, >= {KV4_PAGE * c.table_cols}], got "
-                             f"{tuple(weights.shape)}")
-    with _on(stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if lse is None and weights is not None:
-            lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
-    _need_heads(out, "out", like=q)
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        w_cols = _need_weights(weights, "weights", batch, kv_heads, cols)
+        w_ptr = weights.data_ptr()
+        if lse is None:
+            lse = _empty(stream, (tokens, heads), weights.dtype, q.device)
     if lse is not None:
-        _need_array(lse, torch.float32, "lse", 2)
+        _need_array(lse, _torch().float32, "lse", 2)
         if lse.shape != (tokens, heads):
             raise ValueError(f"lse must be [{tokens}, {heads}], got {tuple(lse.shape)}")
-    a = Attn(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-             None if weights is None else weights.data_ptr(), start, q.stride(0), q.stride(1), out.stride(0),
-             out.stride(1), 0 if weights is None else weights.shape[2], dim ** -0.5 if scale is None else float(scale),
-             tokens, heads, max(1, tokens if max_q is None else int(max_q)) if start else 1, int(bool(causal)),
-             int(window), _dtype(q))
-    _check(_lib().busfill_attn_kv4(ctypes.byref(c), ctypes.byref(a), _stream(stream)), "busfill_attn_kv4")
+        lse_ptr = lse.data_ptr()
+    if out is None:
+        out = _empty(stream, q.shape, q.dtype, q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    o_token, o_head = _need_heads(out, "out", like=q)
+    a = _pack_attn(q.data_ptr(), out.data_ptr(), lse_ptr, w_ptr, start, q_token, q_head, o_token, o_head, w_cols,
+                   dim ** -0.5 if scale is None else scale, tokens, heads,
+                   max(1, tokens if max_q is None else int(max_q)) if start else 1, bool(causal), int(window),
+                   _dtype(q, "q"))
+    _check(_lib().busfill_attn_kv4(c, a, _raw(stream, q)), "busfill_attn_kv4")
     return out
 
 
@@ -266,27 +308,24 @@ def kv4_evict(pages, table, kv_len, weights, keep, recent, out_table=None, weigh
     the same table, in place). Returns (index, weights_out, new kv_len): index int32 [batch,
     kv_heads, keep] holds the slots they came from (-1 behind a shorter sequence's)."""
     torch = _torch()
-    c = _cache(pages, table, kv_len)
-    _need_array(weights, torch.float32, "weights", 3)
-    if weights.shape[:2] != (c.batch, c.heads) or weights.shape[2] < KV4_PAGE * c.table_cols:
-        raise ValueError(f"weights must be [{c.batch}, {c.heads}, >= {KV4_PAGE * c.table_cols}], got "
-                         f"{tuple(weights.shape)}")
+    c, batch, heads, _, cols = _cache(pages, table, kv_len)
+    w_cols = _need_weights(weights, "weights", batch, heads, cols)
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"need 1 <= keep and 0 <= recent <= keep, got keep {keep}, recent {recent}")
     out_table = table if out_table is None else out_table
     _need_array(out_table, torch.int32, "out_table", 2)
-    if out_table.shape[0] != c.batch or out_table.shape[1] * KV4_PAGE < keep:
-        raise ValueError(f"out_table must be [{c.batch}, >= {-(-keep // KV4_PAGE)}], got {tuple(out_table.shape)}")
-    with _on(stream):
-        index = torch.empty((c.batch, c.heads, keep), dtype=torch.int32, device=pages.device)
-        kv_len_out = torch.empty_like(kv_len)
-        if weights_out is None:
-            weights_out = torch.empty_like(weights)
-    _need_array(weights_out, torch.float32, "weights_out", 3)
-    if weights_out.shape != weights.shape:
-        raise ValueError(f"weights_out must be {tuple(weights.shape)}, got {tuple(weights_out.shape)}")
-    e = Eviction(weights.data_ptr(), weights_out.data_ptr(), weights.shape[2], index.data_ptr(),
-                 kv_len_out.data_ptr(), out_table.data_ptr(), out_table.shape[1], keep, recent)
-    _check(_lib().busfill_kv4_evict(ctypes.byref(c), ctypes.byref(e), _stream(stream)), "busfill_kv4_evict")
+    if out_table.shape[0] != batch or out_table.shape[1] * KV4_PAGE < keep:
+        raise ValueError(f"out_table must be [{batch}, >= {-(-keep // KV4_PAGE)}], got {tuple(out_table.shape)}")
+    index = _empty(stream, (batch, heads, keep), torch.int32, pages.device)
+    kv_len_out = _empty(stream, (batch,), torch.int32, pages.device)
+    if weights_out is None:
+        weights_out = _empty(stream, weights.shape, torch.float32, pages.device)
+    else:
+        _need_array(weights_out, torch.float32, "weights_out", 3)
+        if weights_out.shape != weights.shape:
+            raise ValueError(f"weights_out must be {tuple(weights.shape)}, got {tuple(weights_out.shape)}")
+    e = _pack_eviction(weights.data_ptr(), weights_out.data_ptr(), w_cols, index.data_ptr(), kv_len_out.data_ptr(),
+                       out_table.data_ptr(), out_table.shape[1], keep, recent)
+    _check(_lib().busfill_kv4_evict(c, e, _raw(stream, pages)), "busfill_kv4_evict")
     return index, weights_out, kv_len_out

@@ -41,3 +41,13 @@ def test_ctypes_mirror_matches_c_layout(c_layout, name):
     assert ctypes.sizeof(cls) == c_layout[(name, "size")], name
     for f, _ in cls._fields_:
         assert getattr(cls, f).offset == c_layout[(name, f)], (name, f)
+
+
+@pytest.mark.parametrize("name", sorted(STRUCTS))
+def test_packed_bytes_are_the_struct(name):
+    cls = STRUCTS[name]
+    values = [float(i) if t is ctypes.c_float else i for i, (_, t) in enumerate(cls._fields_, 1)]
+    data = kv4._packer(cls)(*values)
+    assert len(data) == ctypes.sizeof(cls)
+    back = cls.from_buffer_copy(data)
+    assert [getattr(back, f) for f, _ in cls._fields_] == values
