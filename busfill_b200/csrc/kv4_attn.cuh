@@ -72,6 +72,13 @@ __device__ __forceinline__ void mma_16816(float* d, const uint32_t* a, const uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
+// d = a b + c, c = (c0, c1, c0, c1)
+__device__ __forceinline__ void mma_16816_from(float* d, const uint32_t* a, const uint32_t* b, const float* c) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -223,8 +230,8 @@ __device__ __forceinline__ void scores_16(const uint8_t* page, int mt, int lane,
     const float e0 = b & 1 ? d0.y : d0.x, e1 = b & 1 ? d1.y : d1.x;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float acc[4] = {q[nt].corr[b][0], q[nt].corr[b][1], q[nt].corr[b][0], q[nt].corr[b][1]};
-      mma_16816(acc, a0, q[nt].b[b]);
+      float acc[4];
+      mma_16816_from(acc, a0, q[nt].b[b], q[nt].corr[b]);
       mma_16816(acc, a1, q[nt].b[b] + 2);
       s[nt][0] = fmaf(e0, acc[0], s[nt][0]);
       s[nt][1] = fmaf(e0, acc[1], s[nt][1]);
@@ -405,6 +412,21 @@ __device__ __forceinline__ void store_out(const AttnParams& p, const Span& s, in
   else
     static_cast<__half*>(p.out)[at] = __float2half_rn(x);
 }
+// four channels, ch a multiple of 4
+__device__ __forceinline__ void store_out4(const AttnParams& p, const Span& s, int head, int row, int ch,
+                                           const float4& o, float f) {
+  const int i = row / p.group;
+  if (i >= s.n) return;
+  const size_t at = (size_t)(s.first + i) * p.o_token + (size_t)(head * p.group + row - i * p.group) * p.o_head + ch;
+  uint2 v;
+  if (p.bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(o.x * f, o.y * f), b = __floats2bfloat162_rn(o.z * f, o.w * f);
+    v = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    v = make_uint2(h2_as_u32(__floats2half2_rn(o.x * f, o.y * f)), h2_as_u32(__floats2half2_rn(o.z * f, o.w * f)));
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = v;
+}
 __device__ __forceinline__ void store_lse(const AttnParams& p, const Span& s, int head, int row, float m, float l) {
   const int i = row / p.group;
   if (!p.lse || i >= s.n) return;
@@ -423,8 +445,9 @@ struct Geo {
   static constexpr int kRingBytes = kStages * Fmt<D>::kPageBytes;
   static constexpr int kPreOff = kWarps * kRingBytes;           // units before each sequence
   static constexpr int kBarOff = kPreOff + (kMaxBatch + 2) * 4;
-  static constexpr int kMiscOff = kBarOff + kWarps * kStages * 8;
-  static constexpr int kBytes = kMiscOff + 256;
+  static constexpr int kMetaOff = kBarOff + kWarps * kStages * 8;      // m, then l, of every piece and row
+  static constexpr int kMiscOff = kMetaOff + 2 * 2 * kWarps * kRows * 4;
+  static constexpr int kBytes = kMiscOff + 512;
   static_assert(kPieceFloats * 4 <= kRingBytes, "a piece fits the warp's ring");
   static_assert(kBytes <= 232448, "dynamic shared memory");
 };
@@ -471,6 +494,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   int* pre = reinterpret_cast<int*>(smem + G::kPreOff);
   int* misc = reinterpret_cast<int*>(smem + G::kMiscOff);
   int* piece_item = misc;            // [2 * W]: first unit of the item, -1: no piece
+  float* meta_m = reinterpret_cast<float*>(smem + G::kMetaOff);
+  float* meta_l = meta_m + 2 * W * ROWS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * G::kRingBytes;
   const uint32_t ring_s = smem_u32(ring);
@@ -629,8 +654,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
           if (lane < 4) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              to[ROWS * D + 8 * nt + 2 * lane + k] = run.m[nt][k];
-              to[ROWS * (D + 1) + 8 * nt + 2 * lane + k] = run.l[nt][k];
+              meta_m[(2 * warp + last) * ROWS + 8 * nt + 2 * lane + k] = run.m[nt][k];
+              meta_l[(2 * warp + last) * ROWS + 8 * nt + 2 * lane + k] = run.l[nt][k];
             }
           }
         }
@@ -652,77 +677,114 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   __threadfence_block();
   __syncthreads();
 
-  // join the CTA's pieces, item by item
-  auto piece = [&](int i) -> const float* {
-    return (i & 1) ? reinterpret_cast<const float*>(smem + (i >> 1) * G::kRingBytes) : my_part + (size_t)(i >> 1) * PF;
-  };
-  // rows x channels of `n` pieces get(i) to the output or to `to`
-  auto join = [&](int n, auto get, const Cursor& c, float* to) {
-    for (int x = threadIdx.x; x < ROWS * D; x += W * 32) {
-      const int row = x / D, ch = x - row * D;
-      float m = -INFINITY, l = 0.0f, o = 0.0f;
-      for (int i = 0; i < n; ++i) m = fmaxf(m, get(i)[ROWS * D + row]);
-      for (int i = 0; i < n; ++i) {
-        const float* s = get(i);
-        const float mi = s[ROWS * D + row];
-        // an empty piece has m = -inf, l = 0 and o = 0; NaN scores leave m at -inf and l NaN
-        const float f = mi == -INFINITY ? 1.0f : exp2_approx(mi - m);
-        l = fmaf(s[ROWS * (D + 1) + row], f, l);
-        o = fmaf(s[x], f, o);
-      }
-      if (to) {
-        to[x] = o;
-        if (ch == 0) {
-          to[ROWS * D + row] = m;
-          to[ROWS * (D + 1) + row] = l;
-        }
-      } else {
-        store_out<D>(p, c.s, c.head, c.rg * ROWS + row, ch, l == 0.0f ? 0.0f : o / l);
-        if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, m, l);
-      }
-    }
-  };
+  // Join: first the CTA's own pieces, item by item (their m and l are in
+  // shared memory), then, where this CTA is the last one of an item that is
+  // split between CTAs, all CTAs' parts from the workspace. A task is 32
+  // 4-channel pieces of an item's rows, one per lane of a warp. An empty piece
+  // has m = -inf, l = 0, o = 0; NaN scores leave m at -inf and l NaN.
+  constexpr int QUADS = D / 4, TASKS = ROWS * QUADS / 32;
+  auto share = [](float m, float top) { return m == -INFINITY ? 1.0f : exp2_approx(m - top); };
   int* list = piece_item + 2 * W;   // the pieces there are, in order
-  int* count = list + 2 * W;
-  if (threadIdx.x == 0) {
-    int n = 0;
-    for (int i = 0; i < 2 * W; ++i)
-      if (piece_item[i] >= 0) list[n++] = i;
-    *count = n;
+  int* group = list + 2 * W;        // the first in `list` of every item
+  int* counts = group + 2 * W + 1;  // items, and whether this CTA joins slot 0, slot 1
+  if (warp == 0) {
+    const bool has = lane < 2 * W && piece_item[lane < 2 * W ? lane : 0] >= 0;
+    const unsigned all = __ballot_sync(0xffffffffu, has);
+    if (has) list[__popc(all & ((1u << lane) - 1))] = lane;
+    __syncwarp();
+    const int n = __popc(all);
+    const bool heads = lane < n && (lane == 0 || piece_item[list[lane]] != piece_item[list[lane - 1]]);
+    const unsigned first = __ballot_sync(0xffffffffu, heads);
+    if (heads) group[__popc(first & ((1u << lane) - 1))] = lane;
+    if (lane == 0) {
+      group[__popc(first)] = n;
+      counts[0] = __popc(first);
+      counts[1] = counts[2] = 0;
+    }
   }
   __syncthreads();
-  const int pieces = *count;
-  for (int i0 = 0; i0 < pieces;) {
-    const int item0 = piece_item[list[i0]];
-    int i1 = i0 + 1;
-    while (i1 < pieces && piece_item[list[i1]] == item0) ++i1;
-    Cursor c;
+  const int groups = counts[0];
+  // items that go on outside the CTA's range: slot 0 began before it, slot 1
+  // goes on behind it
+  int split[2] = {-1, -1};
+  Cursor c;
+  for (int task = warp; task < groups * TASKS; task += W) {
+    const int g = task / TASKS, x = (task - g * TASKS) * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
+    const int k0 = group[g], n = group[g + 1] - k0, item0 = piece_item[list[k0]];
     seek<ROWS>(p, pre, item0, c, bad);
-    const int end = item0 + c.s.pages;
-    auto mine = [&](int i) { return piece(list[i0 + i]); };
-    if (item0 >= c0 && end <= c1) {
-      join(i1 - i0, mine, c, nullptr);
-    } else {
-      // split between CTAs: slot 0 for the item that began before this CTA's
-      // range, slot 1 for the one that goes on behind it
-      join(i1 - i0, mine, c, my_part + (size_t)(W + (item0 < c0 ? 0 : 1)) * PF);
-      __threadfence();
-      __syncthreads();
-      const int first = (int)((((long long)item0 + 1) * ctas - 1) / T), last = (int)(((long long)end * ctas - 1) / T);
-      if (threadIdx.x == 0)
-        misc[255 / 4] = atom_add_acq_rel_gpu(p.counters + first, 1u) == (unsigned)(last - first) ? 1 : 0;
-      __syncthreads();
-      if (misc[255 / 4]) {
-        __threadfence();
-        auto theirs = [&](int i) -> const float* {
-          return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(W + (i == 0 ? 1 : 0)) * PF;
-        };
-        join(last - first + 1, theirs, c, nullptr);
-        if (threadIdx.x == 0) p.counters[first] = 0;
-      }
-      __syncthreads();
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < n; ++i) top = fmaxf(top, meta_m[list[k0 + i] * ROWS + row]);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const int id = list[k0 + i];
+      const float* from = id & 1 ? reinterpret_cast<const float*>(smem + (id >> 1) * G::kRingBytes)
+                                 : my_part + (size_t)(id >> 1) * PF;
+      const float4 v = reinterpret_cast<const float4*>(from)[x];
+      const float f = share(meta_m[id * ROWS + row], top);
+      sum = fmaf(meta_l[id * ROWS + row], f, sum);
+      o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
     }
-    i0 = i1;
+    if (item0 >= c0 && item0 + c.s.pages <= c1) {
+      store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o, sum == 0.0f ? 0.0f : 1.0f / sum);
+      if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
+    } else {
+      float* to = my_part + (size_t)(W + (item0 < c0 ? 0 : 1)) * PF;
+      reinterpret_cast<float4*>(to)[x] = o;
+      if (ch == 0) to[ROWS * D + row] = top, to[ROWS * (D + 1) + row] = sum;
+    }
+  }
+  if (groups > 0) {
+    const int lo = piece_item[list[0]], hi = piece_item[list[group[groups - 1]]];
+    if (lo < c0) split[0] = lo;
+    seek<ROWS>(p, pre, hi, c, bad);
+    if (hi >= c0 && hi + c.s.pages > c1) split[1] = hi;
+  }
+  if (split[0] >= 0 || split[1] >= 0) {
+    __threadfence();
+    __syncthreads();
+    // the CTAs [first, last] that hold an item
+    auto holders = [&](int item0, int& first, int& last) {
+      seek<ROWS>(p, pre, item0, c, bad);
+      first = (int)((((long long)item0 + 1) * ctas - 1) / T);
+      last = (int)(((long long)(item0 + c.s.pages) * ctas - 1) / T);
+    };
+    if (threadIdx.x < 2 && split[threadIdx.x] >= 0) {
+      int first, last;
+      holders(split[threadIdx.x], first, last);
+      if (atom_add_acq_rel_gpu(p.counters + first, 1u) == (unsigned)(last - first)) {
+        counts[1 + threadIdx.x] = 1;
+        p.counters[first] = 0;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int slot = 0; slot < 2; ++slot) {
+      if (!counts[1 + slot]) continue;
+      __threadfence();
+      int first, last;
+      holders(split[slot], first, last);
+      const int n = last - first + 1;
+      auto theirs = [&](int i) {
+        return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(W + (i == 0 ? 1 : 0)) * PF;
+      };
+      for (int task = warp; task < TASKS; task += W) {
+        const int x = task * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) top = fmaxf(top, __ldcg(theirs(i) + ROWS * D + row));
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(theirs(i)) + x);
+          const float f = share(__ldcg(theirs(i) + ROWS * D + row), top);
+          sum = fmaf(__ldcg(theirs(i) + ROWS * (D + 1) + row), f, sum);
+          o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+        }
+        store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o, sum == 0.0f ? 0.0f : 1.0f / sum);
+        if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
+      }
+    }
   }
   if (bad) atomicOr(p.error, kErrIndex);
 }
