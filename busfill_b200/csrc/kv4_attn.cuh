@@ -40,6 +40,7 @@ namespace busfill {
 namespace kv4 {
 
 constexpr int kMaxBatch = 1024;
+constexpr float kLag = 4.0f;   // log2 growth of a row's maximum that is not followed
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -66,22 +67,21 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// d += a b
 __device__ __forceinline__ void mma_16816(float* d, const uint32_t* a, const uint32_t* b) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-// d = a b + c, c = (c0, c1, c0, c1)
+// d = a b + c
 __device__ __forceinline__ void mma_16816_from(float* d, const uint32_t* a, const uint32_t* b, const float* c) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -121,7 +121,7 @@ __device__ __forceinline__ void sees(const AttnParams& p, const Span& s, int i, 
 template <int D>
 struct QueryTile {
   uint32_t b[Fmt<D>::kBlocks][4];   // [block][2 * half + reg]
-  float corr[Fmt<D>::kBlocks][2];
+  float corr[Fmt<D>::kBlocks][4];   // as the accumulator's start: columns 2j, 2j + 1 twice
   float factor[2];
   int lo[2], hi[2];
 };
@@ -157,9 +157,11 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s,
   int e = 136 - (int)(__float_as_uint(top) >> 23);
   if (top == 0.0f || !(top <= 3.4e38f)) e = 0;
   e = max(-126, min(126, e));
-  const float up = __uint_as_float((unsigned)(127 + e) << 23);
-  // codes weigh 2^-24 (see above)
-  const float factor = p.scale_log2 * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.0f;
+  // the scale's sign goes to the queries, so that the factor orders scores;
+  // codes weigh 2^-24 (see above); -inf times the factor stays -inf
+  const float up = copysignf(__uint_as_float((unsigned)(127 + e) << 23), p.scale_log2);
+  const float factor =
+      fmaxf(fabsf(p.scale_log2) * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.0f, 1e-37f);
   float corr[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -179,7 +181,10 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s,
   for (int k = 0; k < 2; ++k) {
     const int from = 4 * (2 * j + k);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) t.corr[b][k] = __shfl_sync(0xffffffffu, corr[b], from);
+    for (int b = 0; b < NB; ++b) {
+      t.corr[b][k] = t.corr[b][k + 2] = __shfl_sync(0xffffffffu, corr[b], from);
+      asm("" : "+f"(t.corr[b][k + 2]));   // four registers, ready to be an accumulator
+    }
     t.factor[k] = __shfl_sync(0xffffffffu, factor, from);
     const int ri = (r0 + 2 * j + k) / p.group;
     t.lo[k] = 0;   // columns without a row see everything, so that they hold up no page
@@ -248,7 +253,7 @@ __device__ __forceinline__ void scores_16(const uint8_t* page, int mt, int lane,
 template <int D, int NT>
 struct Running {
   float o[NT][Fmt<D>::kBlocks][2][4];
-  float pd[NT][Fmt<D>::kBlocks][2];
+  float pd[NT][Fmt<D>::kBlocks][4];   // every row alike: a whole accumulator
   float m[NT][2], l[NT][2];
 
   __device__ __forceinline__ void clear() {
@@ -258,7 +263,7 @@ struct Running {
       for (int k = 0; k < 2; ++k) m[nt][k] = -INFINITY, l[nt][k] = 0.0f;
 #pragma unroll
       for (int b = 0; b < Fmt<D>::kBlocks; ++b) {
-        pd[nt][b][0] = pd[nt][b][1] = 0.0f;
+        pd[nt][b][0] = pd[nt][b][1] = pd[nt][b][2] = pd[nt][b][3] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[nt][b][e >> 2][e & 3] = 0.0f;
       }
@@ -286,47 +291,48 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int slot = base + 16 * mt + tile_perm(c) + 8 * (e >> 1);
-          const bool seen = slot >= q[nt].lo[e & 1] && slot < q[nt].hi[e & 1];
-          s[mt][nt][e] = seen ? s[mt][nt][e] * q[nt].factor[e & 1] : -INFINITY;
+          if (slot < q[nt].lo[e & 1] || slot >= q[nt].hi[e & 1]) s[mt][nt][e] = -INFINITY;
         }
-    } else {
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][nt][e] *= q[nt].factor[e & 1];
     }
-    float top[2] = {run.m[nt][0], run.m[nt][1]};
+    float top[2] = {s[0][nt][0], s[0][nt][1]};
+    top[0] = fmaxf(top[0], s[0][nt][2]);
+    top[1] = fmaxf(top[1], s[0][nt][3]);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+    for (int mt = 1; mt < 4; ++mt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[mt][nt][e]);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], x));
-    float base2[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) base2[k] = top[k] == -INFINITY ? 0.0f : top[k];
-    if (__any_sync(0xffffffffu, top[0] != run.m[nt][0] || top[1] != run.m[nt][1])) {
-      const float f[2] = {exp2_approx(run.m[nt][0] - base2[0]), exp2_approx(run.m[nt][1] - base2[1])};
+      top[k] *= q[nt].factor[k];
+    }
+    // The reference m follows the maximum only when that has grown by more
+    // than kLag (p d stays far inside fp16: 2^kLag * 896), as most pages change
+    // some row's maximum a little.
+    if (__any_sync(0xffffffffu, top[0] > run.m[nt][0] + kLag || top[1] > run.m[nt][1] + kLag)) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        run.m[nt][k] = top[k];
-        run.l[nt][k] *= f[k];
-      }
+        const float m = fmaxf(run.m[nt][k], top[k]);
+        const float f = m == run.m[nt][k] ? 1.0f : exp2_approx(run.m[nt][k] - m);
+        run.m[nt][k] = m;
+        run.l[nt][k] *= f;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        run.pd[nt][b][0] *= f[0];
-        run.pd[nt][b][1] *= f[1];
+        for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) run.o[nt][b][e >> 2][e & 3] *= f[e & 1];
+          for (int e = k; e < 8; e += 2) run.o[nt][b][e >> 2][e & 3] *= f;
+          run.pd[nt][b][k] *= f;
+          run.pd[nt][b][k + 2] *= f;
+        }
       }
     }
+    const float off[2] = {run.m[nt][0] == -INFINITY ? 0.0f : -run.m[nt][0],
+                          run.m[nt][1] == -INFINITY ? 0.0f : -run.m[nt][1]};
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[mt][nt][e] = exp2_approx(s[mt][nt][e] - base2[e & 1]);
+        s[mt][nt][e] = exp2_approx(fmaf(s[mt][nt][e], q[nt].factor[e & 1], off[e & 1]));
         run.l[nt][e & 1] += s[mt][nt][e];
       }
   }
@@ -362,17 +368,14 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
       const uint32_t a0[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
       const uint32_t a1[4] = {x0 >> 8 & 0x000f000fu, x0 >> 8 & 0x00f000f0u, x1 >> 8 & 0x000f000fu,
                               x1 >> 8 & 0x00f000f0u};
-      const uint32_t ones[4] = {0x3C003C00u, 0u, 0x3C003C00u, 0u};
+      const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const uint32_t pb[2] = {h2_as_u32(__hmul2(u32_as_h2(p0[nt]), u32_as_h2(d0))),
                                 h2_as_u32(__hmul2(u32_as_h2(p1[nt]), u32_as_h2(d1)))};
         mma_16816(run.o[nt][b][0], a0, pb);
         mma_16816(run.o[nt][b][1], a1, pb);
-        float acc[4] = {run.pd[nt][b][0], run.pd[nt][b][1], 0.0f, 0.0f};
-        mma_16816(acc, ones, pb);
-        run.pd[nt][b][0] = acc[0];
-        run.pd[nt][b][1] = acc[1];
+        mma_16816(run.pd[nt][b], ones, pb);
       }
     }
   }
@@ -434,6 +437,14 @@ __device__ __forceinline__ void store_lse(const AttnParams& p, const Span& s, in
       l > 0.0f ? (m + log2f(l)) * kLn2 : l == 0.0f ? -INFINITY : l;
 }
 
+// Position in the list of units.
+struct Cursor {
+  int b, head, rg, page;    // page: index in the sequence
+  int rgs;                  // row groups of the sequence
+  Span s;
+};
+static_assert(sizeof(Cursor) <= 64, "item slots in shared memory");
+
 // Geometry by head dimension and row tiles: warps of a CTA (one CTA per SM)
 // and pages of each warp's ring.
 template <int D, int NT>
@@ -446,7 +457,8 @@ struct Geo {
   static constexpr int kPreOff = kWarps * kRingBytes;           // units before each sequence
   static constexpr int kBarOff = kPreOff + (kMaxBatch + 2) * 4;
   static constexpr int kMetaOff = kBarOff + kWarps * kStages * 8;      // m, then l, of every piece and row
-  static constexpr int kMiscOff = kMetaOff + 2 * 2 * kWarps * kRows * 4;
+  static constexpr int kItemOff = kMetaOff + 2 * 2 * kWarps * kRows * 4;   // the item of every piece
+  static constexpr int kMiscOff = kItemOff + 2 * kWarps * 64;
   static constexpr int kBytes = kMiscOff + 512;
   static_assert(kPieceFloats * 4 <= kRingBytes, "a piece fits the warp's ring");
   static_assert(kBytes <= 232448, "dynamic shared memory");
@@ -457,12 +469,6 @@ constexpr size_t part_floats() {
   return (size_t)(Geo<D, NT>::kWarps + 2) * Geo<D, NT>::kPieceFloats;
 }
 
-// Position in the list of units.
-struct Cursor {
-  int b, head, rg, page;    // page: index in the sequence
-  int rgs;                  // row groups of the sequence
-  Span s;
-};
 
 // units before sequence b in pre[b]; sets the cursor to unit u < pre[batch]
 template <int ROWS>
@@ -494,6 +500,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   int* pre = reinterpret_cast<int*>(smem + G::kPreOff);
   int* misc = reinterpret_cast<int*>(smem + G::kMiscOff);
   int* piece_item = misc;            // [2 * W]: first unit of the item, -1: no piece
+  auto piece_cursor = [&](int i) { return reinterpret_cast<Cursor*>(smem + G::kItemOff + 64 * i); };
   float* meta_m = reinterpret_cast<float*>(smem + G::kMetaOff);
   float* meta_l = meta_m + 2 * W * ROWS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -552,26 +559,34 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   if (u0 < u1) {
     Cursor c;
     seek<ROWS>(p, pre, u0, c, bad);
-    // the pages ahead: a cursor of its own, the page number one step ahead
-    int ib = c.b, ihead = c.head, irg = c.rg, ipage = c.page, irgs = c.rgs;
-    Span is = c.s;
+    // the pages ahead: a cursor of its own; the lanes hold the next 32 page
+    // numbers of the sequence
+    Cursor in = c;
+    int held = -64, number = 0;   // lane i holds page held + i
     auto next_source = [&]() -> const uint8_t* {
-      const int pg = page_of(p.c, p.c.table, p.c.table_cols, ib, ipage, bad);
-      const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + ihead) * F::kPageBytes;
-      if (++ipage == is.page0 + is.pages) {
-        if (++irg == irgs) {
-          irg = 0;
-          if (++ihead == p.c.heads) {
-            ihead = 0;
-            do ++ib;
-            while (ib < batch && pre[ib + 1] == pre[ib]);
-            if (ib < batch) {
-              is = span_of(p, ib, bad);
-              irgs = (is.n * p.group + ROWS - 1) / ROWS;
+      if (in.page < held || in.page >= held + 32) {
+        held = in.page;
+        number = 0;
+        if (held + lane < in.s.page0 + in.s.pages)
+          number = page_of(p.c, p.c.table, p.c.table_cols, in.b, held + lane, bad);
+      }
+      const int pg = __shfl_sync(0xffffffffu, number, in.page - held);
+      const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + in.head) * F::kPageBytes;
+      if (++in.page == in.s.page0 + in.s.pages) {
+        if (++in.rg == in.rgs) {
+          in.rg = 0;
+          if (++in.head == p.c.heads) {
+            in.head = 0;
+            do ++in.b;
+            while (in.b < batch && pre[in.b + 1] == pre[in.b]);
+            if (in.b < batch) {
+              in.s = span_of(p, in.b, bad);
+              in.rgs = (in.s.n * p.group + ROWS - 1) / ROWS;
             }
+            held = -64;
           }
         }
-        ipage = is.page0;
+        in.page = in.s.page0;
       }
       return src;
     };
@@ -659,7 +674,10 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
             }
           }
         }
-        if (lane == 0) piece_item[2 * warp + (last ? 1 : 0)] = item0;
+        if (lane == 0) {
+          piece_item[2 * warp + last] = item0;
+          *piece_cursor(2 * warp + last) = c;
+        }
       }
       if (u + 1 < u1) {   // the next item
         seek<ROWS>(p, pre, u + 1, c, bad);
@@ -704,18 +722,14 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   }
   __syncthreads();
   const int groups = counts[0];
-  // items that go on outside the CTA's range: slot 0 began before it, slot 1
-  // goes on behind it
-  int split[2] = {-1, -1};
-  Cursor c;
   for (int task = warp; task < groups * TASKS; task += W) {
     const int g = task / TASKS, x = (task - g * TASKS) * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
     const int k0 = group[g], n = group[g + 1] - k0, item0 = piece_item[list[k0]];
-    seek<ROWS>(p, pre, item0, c, bad);
+    const Cursor& c = *piece_cursor(list[k0]);
     float top = -INFINITY, sum = 0.0f;
     for (int i = 0; i < n; ++i) top = fmaxf(top, meta_m[list[k0 + i] * ROWS + row]);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const int id = list[k0 + i];
       const float* from = id & 1 ? reinterpret_cast<const float*>(smem + (id >> 1) * G::kRingBytes)
@@ -729,61 +743,75 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
       store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o, sum == 0.0f ? 0.0f : 1.0f / sum);
       if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
     } else {
+      // slot 0: the item began before this CTA's range; slot 1: it goes on behind it
       float* to = my_part + (size_t)(W + (item0 < c0 ? 0 : 1)) * PF;
       reinterpret_cast<float4*>(to)[x] = o;
       if (ch == 0) to[ROWS * D + row] = top, to[ROWS * (D + 1) + row] = sum;
     }
   }
-  if (groups > 0) {
-    const int lo = piece_item[list[0]], hi = piece_item[list[group[groups - 1]]];
-    if (lo < c0) split[0] = lo;
-    seek<ROWS>(p, pre, hi, c, bad);
-    if (hi >= c0 && hi + c.s.pages > c1) split[1] = hi;
-  }
-  if (split[0] >= 0 || split[1] >= 0) {
-    __threadfence();
-    __syncthreads();
-    // the CTAs [first, last] that hold an item
-    auto holders = [&](int item0, int& first, int& last) {
-      seek<ROWS>(p, pre, item0, c, bad);
-      first = (int)((((long long)item0 + 1) * ctas - 1) / T);
-      last = (int)(((long long)(item0 + c.s.pages) * ctas - 1) / T);
-    };
-    if (threadIdx.x < 2 && split[threadIdx.x] >= 0) {
-      int first, last;
-      holders(split[threadIdx.x], first, last);
+  __syncthreads();
+  // An item in slot 0 or 1 is held by the CTAs [first, last]; the one that
+  // arrives last joins the parts.
+  auto item_of = [&](int slot) { return piece_cursor(list[slot == 0 ? 0 : group[groups - 1]]); };
+  auto holders = [&](int slot, int& first, int& last) {
+    const int item0 = piece_item[list[slot == 0 ? 0 : group[groups - 1]]];
+    first = (int)((((long long)item0 + 1) * ctas - 1) / T);
+    last = (int)(((long long)(item0 + item_of(slot)->s.pages) * ctas - 1) / T);
+    return slot == 0 ? item0 < c0 : item0 >= c0 && item0 + item_of(slot)->s.pages > c1;
+  };
+  if (threadIdx.x < 64 && lane == 0 && groups > 0) {
+    int first, last;
+    if (holders(warp, first, last)) {
+      __threadfence();
       if (atom_add_acq_rel_gpu(p.counters + first, 1u) == (unsigned)(last - first)) {
-        counts[1 + threadIdx.x] = 1;
         p.counters[first] = 0;
+        counts[1 + warp] = 1;
       }
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  for (int slot = 0; slot < 2; ++slot) {
+    if (!counts[1 + slot]) continue;
+    int first, last;
+    holders(slot, first, last);
+    const int n = last - first + 1;
+    const Cursor& c = *item_of(slot);
+    auto theirs = [&](int i) {
+      return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(W + (i == 0 ? 1 : 0)) * PF;
+    };
+    for (int task = warp; task < TASKS; task += W) {
+      const int x = task * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
+      float top = -INFINITY, sum = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      // 16 parts in flight at a time; the reference moves with the parts
+      for (int i0 = 0; i0 < n; i0 += 16) {
+        float4 v[16];
+        float m[16], l[16];
 #pragma unroll
-    for (int slot = 0; slot < 2; ++slot) {
-      if (!counts[1 + slot]) continue;
-      __threadfence();
-      int first, last;
-      holders(split[slot], first, last);
-      const int n = last - first + 1;
-      auto theirs = [&](int i) {
-        return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(W + (i == 0 ? 1 : 0)) * PF;
-      };
-      for (int task = warp; task < TASKS; task += W) {
-        const int x = task * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) top = fmaxf(top, __ldcg(theirs(i) + ROWS * D + row));
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(theirs(i)) + x);
-          const float f = share(__ldcg(theirs(i) + ROWS * D + row), top);
-          sum = fmaf(__ldcg(theirs(i) + ROWS * (D + 1) + row), f, sum);
-          o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+        for (int i = 0; i < 16; ++i) {
+          const float* from = theirs(min(i0 + i, n - 1));
+          v[i] = __ldcg(reinterpret_cast<const float4*>(from) + x);
+          m[i] = __ldcg(from + ROWS * D + row);
+          l[i] = __ldcg(from + ROWS * (D + 1) + row);
         }
-        store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o, sum == 0.0f ? 0.0f : 1.0f / sum);
-        if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
+        float next = top;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next = fmaxf(next, m[i]);
+        const float old = share(top, next);
+        sum *= old;
+        o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+        top = next;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i0 + i < n) {
+            const float f = share(m[i], top);
+            sum = fmaf(l[i], f, sum);
+            o.x = fmaf(v[i].x, f, o.x), o.y = fmaf(v[i].y, f, o.y), o.z = fmaf(v[i].z, f, o.z),
+            o.w = fmaf(v[i].w, f, o.w);
+          }
       }
+      store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o, sum == 0.0f ? 0.0f : 1.0f / sum);
+      if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
     }
   }
   if (bad) atomicOr(p.error, kErrIndex);

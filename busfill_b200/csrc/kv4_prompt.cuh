@@ -107,7 +107,7 @@ namespace prompt {
 
 constexpr int kThreads = 512;
 constexpr int kSoftmaxWarp0 = 4, kDequantWarp0 = 12;
-constexpr float kLag = 8.0f;   // log2 growth of a row's maximum that O is not rescaled for
+constexpr float kLag = 8.0f;   // log2 growth of a row's maximum that O is not rescaled for (p < 2^8)
 
 template <int D>
 struct Geo {
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
           if (j == 0) {
             m = mt;
-          } else if (__any_sync(0xffffffffu, mt > m + kLag || (m == -INFINITY && mt > m))) {
+          } else if (__any_sync(0xffffffffu, mt > m + prompt::kLag || (m == -INFINITY && mt > m))) {
             const float m2 = fmaxf(m, mt);
             const float a = m == m2 ? 1.0f : exp2_approx(m - m2);
             m = m2;
