@@ -449,12 +449,13 @@ static_assert(sizeof(Cursor) <= 64, "item slots in shared memory");
 // and pages of each warp's ring.
 template <int D, int NT>
 struct Geo {
-  static constexpr int kWarps = D == 256 ? 6 : NT == 1 ? 12 : 8;
-  static constexpr int kStages = D == 64 ? 4 : D == 256 ? 2 : NT == 1 ? 2 : 3;
+  static constexpr int kWarps = D == 64 && NT == 1 ? 12 : 8;
+  static constexpr int kStages = D == 64 ? 3 : D == 128 ? 2 : 1;
   static constexpr int kRows = 8 * NT;
   static constexpr int kPieceFloats = kRows * (D + 2);          // o, m, l of a piece
   static constexpr int kRingBytes = kStages * Fmt<D>::kPageBytes;
-  static constexpr int kPreOff = kWarps * kRingBytes;           // units before each sequence
+  static constexpr int kFirstOff = kWarps * kRingBytes;         // o of every warp's first piece
+  static constexpr int kPreOff = kFirstOff + kWarps * kRows * D * 4;   // units before each sequence
   static constexpr int kBarOff = kPreOff + (kMaxBatch + 2) * 4;
   static constexpr int kMetaOff = kBarOff + kWarps * kStages * 8;      // m, then l, of every piece and row
   static constexpr int kItemOff = kMetaOff + 2 * 2 * kWarps * kRows * 4;   // the item of every piece
@@ -463,10 +464,10 @@ struct Geo {
   static_assert(kPieceFloats * 4 <= kRingBytes, "a piece fits the warp's ring");
   static_assert(kBytes <= 232448, "dynamic shared memory");
 };
-// workspace, per CTA: every warp's first piece, then the CTA's two partial items
+// workspace, per CTA: its two partial items
 template <int D, int NT>
 constexpr size_t part_floats() {
-  return (size_t)(Geo<D, NT>::kWarps + 2) * Geo<D, NT>::kPieceFloats;
+  return (size_t)2 * Geo<D, NT>::kPieceFloats;
 }
 
 
@@ -509,6 +510,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   const uint32_t bar0 = smem_u32(smem + G::kBarOff) + warp * S * 8;
   if (lane < S) mbar_init(bar0 + 8 * lane, 1);
   fence_mbar_init();
+  if (threadIdx.x == 0) misc[126] = 0;
+  __syncthreads();
   pdl_wait_prerequisites();
   pdl_launch_dependents();
 
@@ -520,6 +523,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     const long long n = (long long)p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS) * s.pages;
     if (n > (1 << 30)) bad = true;
     pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
+    if (s.pages > 0) atomicAdd(&misc[126], p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS));
     if (n == 0 && blockIdx.x == 0) {   // rows that see nothing
       for (int i = 0; i < s.n; ++i)
         for (int h = 0; h < p.q_heads; ++h) {
@@ -544,8 +548,12 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     }
   }
   __syncthreads();
-  const int T = pre[batch];
-  const long long ctas = min((int)gridDim.x, T);   // every CTA of the split has a unit
+  const int T = pre[batch], items = misc[126];
+  // CTAs that share the list: every one gets a unit; where a warp would get
+  // two pages at most, no more than there are items, as a split item has to
+  // be joined through the workspace (one sequence of 300 tokens, 8 heads: 8
+  // CTAs of 5 pages, 8.6 us, against 40 of one page and 5 parts an item, 11 us)
+  const long long ctas = min((int)gridDim.x, max(min(items, T), (T + 2 * W - 1) / (2 * W)));
   if ((int)blockIdx.x >= ctas) {
     if (bad) atomicOr(p.error, kErrIndex);
     return;
@@ -654,9 +662,9 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
         }
       } else {
         // kept for the join: the last piece in the ring (all of it has
-        // landed and been read), an earlier one in the workspace
+        // landed and been read), an earlier one beside it
         const bool last = u + 1 == u1;
-        float* to = last ? reinterpret_cast<float*>(ring) : my_part + (size_t)warp * PF;
+        float* to = reinterpret_cast<float*>(last ? ring : smem + G::kFirstOff + warp * ROWS * D * 4);
         __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -732,9 +740,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const int id = list[k0 + i];
-      const float* from = id & 1 ? reinterpret_cast<const float*>(smem + (id >> 1) * G::kRingBytes)
-                                 : my_part + (size_t)(id >> 1) * PF;
-      const float4 v = reinterpret_cast<const float4*>(from)[x];
+      const float4 v = reinterpret_cast<const float4*>(
+          smem + (id & 1 ? (id >> 1) * G::kRingBytes : G::kFirstOff + (id >> 1) * ROWS * D * 4))[x];
       const float f = share(meta_m[id * ROWS + row], top);
       sum = fmaf(meta_l[id * ROWS + row], f, sum);
       o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
@@ -744,7 +751,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
       if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
     } else {
       // slot 0: the item began before this CTA's range; slot 1: it goes on behind it
-      float* to = my_part + (size_t)(W + (item0 < c0 ? 0 : 1)) * PF;
+      float* to = my_part + (size_t)(item0 < c0 ? 0 : 1) * PF;
       reinterpret_cast<float4*>(to)[x] = o;
       if (ch == 0) to[ROWS * D + row] = top, to[ROWS * (D + 1) + row] = sum;
     }
@@ -777,7 +784,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     const int n = last - first + 1;
     const Cursor& c = *item_of(slot);
     auto theirs = [&](int i) {
-      return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(W + (i == 0 ? 1 : 0)) * PF;
+      return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(i == 0 ? 1 : 0) * PF;
     };
     for (int task = warp; task < TASKS; task += W) {
       const int x = task * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
