@@ -101,9 +101,13 @@ int launch_prompt(const AttnParams& p, const host::Context& ctx, cudaStream_t s)
 template <int D>
 int launch_weights(const AttnParams& p, const host::Context& ctx, cudaStream_t s, bool many) {
   void* args[] = {const_cast<AttnParams*>(&p)};
-  if (!many) return host::launch((const void*)weights_kernel<D>, dim3(ctx.sms * 4), dim3(256), 0, s, args);
-  static std::once_flag once[64];
-  static cudaError_t err[64];
+  static std::once_flag once[64], few_once[64];
+  static cudaError_t err[64], few_err[64];
+  if (!many) {
+    using G = WeightsGeo<D>;
+    if (!raise_smem(weights_kernel<D>, G::kBytes, ctx.dev, few_once, few_err)) return BUSFILL_ERR_LAUNCH;
+    return host::launch((const void*)weights_kernel<D>, dim3(ctx.sms), dim3(G::kWarps * 32), G::kBytes, s, args);
+  }
   constexpr int bytes = wsum::Geo<D>::kAlloc;
   if (!raise_smem(weights_prompt_kernel<D>, bytes, ctx.dev, once, err)) return BUSFILL_ERR_LAUNCH;
   return host::launch((const void*)weights_prompt_kernel<D>, dim3(ctx.sms), dim3(wsum::kThreads), bytes, s, args);

@@ -115,6 +115,22 @@ __device__ __forceinline__ void sees(const AttnParams& p, const Span& s, int i, 
   lo = p.window > 0 ? max(0, s.len - s.n + i + 1 - p.window) : 0;
 }
 
+// pre[1 .. n] to its running sum, pre[0] = 0 (one warp)
+__device__ __forceinline__ void running_sum(int* pre, int n, int lane) {
+  int total = 0;
+  if (lane == 0) pre[0] = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    int x = i0 + lane < n ? pre[i0 + lane + 1] : 0;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, m);
+      if (lane >= m) x += y;
+    }
+    if (i0 + lane < n) pre[i0 + lane + 1] = total + x;
+    total += __shfl_sync(0xffffffffu, x, 31);
+  }
+}
+
 // Query operand of one row group of 8 rows, and per column pair (2j, 2j + 1)
 // of the score fragments: -8 sum(q) of every block, the factor to log2
 // scores, the slots seen.
@@ -492,6 +508,43 @@ __device__ __forceinline__ void seek(const AttnParams& p, const int* pre, int u,
   c.page = c.s.page0 + r - c.rg * c.s.pages;
 }
 
+// The pages of a range of units one after another, for the copies that run
+// ahead: a cursor of its own; the warp's lanes hold the next 32 page numbers.
+template <int D, int ROWS>
+struct PageFeed {
+  Cursor in;
+  int held = -64, number = 0;   // lane i holds the number of page held + i
+
+  __device__ explicit PageFeed(const Cursor& c) : in(c) {}
+  __device__ __forceinline__ const uint8_t* next(const AttnParams& p, const int* pre, int lane, bool& bad) {
+    if (in.page < held || in.page >= held + 32) {
+      held = in.page;
+      number = 0;
+      if (held + lane < in.s.page0 + in.s.pages)
+        number = page_of(p.c, p.c.table, p.c.table_cols, in.b, held + lane, bad);
+    }
+    const int pg = __shfl_sync(0xffffffffu, number, in.page - held);
+    const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + in.head) * Fmt<D>::kPageBytes;
+    if (++in.page == in.s.page0 + in.s.pages) {
+      if (++in.rg == in.rgs) {
+        in.rg = 0;
+        if (++in.head == p.c.heads) {
+          in.head = 0;
+          do ++in.b;
+          while (in.b < p.c.batch && pre[in.b + 1] == pre[in.b]);
+          if (in.b < p.c.batch) {
+            in.s = span_of(p, in.b, bad);
+            in.rgs = (in.s.n * p.group + ROWS - 1) / ROWS;
+          }
+          held = -64;
+        }
+      }
+      in.page = in.s.page0;
+    }
+    return src;
+  }
+};
+
 template <int D, int NT>
 __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const __grid_constant__ AttnParams p) {
   using F = Fmt<D>;
@@ -533,20 +586,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     }
   }
   __syncthreads();
-  if (warp == 0) {
-    int total = 0;
-    if (lane == 0) pre[0] = 0;
-    for (int b0 = 0; b0 < batch; b0 += 32) {
-      int x = b0 + lane < batch ? pre[b0 + lane + 1] : 0;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, m);
-        if (lane >= m) x += y;
-      }
-      if (b0 + lane < batch) pre[b0 + lane + 1] = total + x;
-      total += __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
+  if (warp == 0) running_sum(pre, batch, lane);
   __syncthreads();
   const int T = pre[batch], items = misc[126];
   // CTAs that share the list: every one gets a unit; where a warp would get
@@ -567,37 +607,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   if (u0 < u1) {
     Cursor c;
     seek<ROWS>(p, pre, u0, c, bad);
-    // the pages ahead: a cursor of its own; the lanes hold the next 32 page
-    // numbers of the sequence
-    Cursor in = c;
-    int held = -64, number = 0;   // lane i holds page held + i
-    auto next_source = [&]() -> const uint8_t* {
-      if (in.page < held || in.page >= held + 32) {
-        held = in.page;
-        number = 0;
-        if (held + lane < in.s.page0 + in.s.pages)
-          number = page_of(p.c, p.c.table, p.c.table_cols, in.b, held + lane, bad);
-      }
-      const int pg = __shfl_sync(0xffffffffu, number, in.page - held);
-      const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + in.head) * F::kPageBytes;
-      if (++in.page == in.s.page0 + in.s.pages) {
-        if (++in.rg == in.rgs) {
-          in.rg = 0;
-          if (++in.head == p.c.heads) {
-            in.head = 0;
-            do ++in.b;
-            while (in.b < batch && pre[in.b + 1] == pre[in.b]);
-            if (in.b < batch) {
-              in.s = span_of(p, in.b, bad);
-              in.rgs = (in.s.n * p.group + ROWS - 1) / ROWS;
-            }
-            held = -64;
-          }
-        }
-        in.page = in.s.page0;
-      }
-      return src;
-    };
+    PageFeed<D, ROWS> feed(c);
+    auto next_source = [&] { return feed.next(p, pre, lane, bad); };
     int issued = u0;
     for (int k = 0; k < S && issued < u1; ++k, ++issued) {
       const uint8_t* src = next_source();
@@ -826,79 +837,130 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
 
 // The weight that the call's rows give every cached token, added to the
 // running sums: weights[b][h][s] += sum over the rows r of the group of
-// exp(score[r,s] - lse[r]). Keys only. A warp takes whole pages and walks over
-// the rows that see them, so each sum has one owner and one order.
+// exp(score[r,s] - lse[r]). Keys only, so half the bytes of the attention. A
+// warp streams whole pages (ranges of the list of all pages, as above) and
+// walks over the rows that see each, so every sum has one owner and one order.
 template <int D>
-__global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ AttnParams p) {
-  using F = Fmt<D>;
-  __shared__ int pre[kMaxBatch + 1];
+struct WeightsGeo {
+  static constexpr int kWarps = D == 256 ? 8 : 16;
+  static constexpr int kStages = 3;
+  static constexpr int kKeyBytes = 36 * D;   // key half of a page
+  static constexpr int kRingBytes = kStages * kKeyBytes;
+  static constexpr int kPreOff = kWarps * kRingBytes;
+  static constexpr int kBarOff = kPreOff + (kMaxBatch + 2) * 4;
+  static constexpr int kBytes = kBarOff + kWarps * kStages * 8;
+  static_assert(kBytes <= 232448, "dynamic shared memory");
+};
+
+template <int D>
+__global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(const __grid_constant__ AttnParams p) {
+  using G = WeightsGeo<D>;
+  constexpr int W = G::kWarps, S = G::kStages, ROWS = 1 << 20;   // an item: all rows of a sequence and head
+  extern __shared__ __align__(128) uint8_t smem[];
+  int* pre = reinterpret_cast<int*>(smem + G::kPreOff);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = p.c.batch;
+  uint8_t* ring = smem + warp * G::kRingBytes;
+  const uint32_t ring_s = smem_u32(ring), bar0 = smem_u32(smem + G::kBarOff) + warp * S * 8;
+  if (lane < S) mbar_init(bar0 + 8 * lane, 1);
+  fence_mbar_init();
   pdl_wait_prerequisites();
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = p.c.batch;
   bool bad = false;
-  for (int b = threadIdx.x; b < batch; b += blockDim.x) {
-    const Span s = span_of(p, b, bad);
-    const long long n = (long long)p.c.heads * s.pages;
+  for (int b = threadIdx.x; b < batch; b += W * 32) {
+    const long long n = (long long)p.c.heads * span_of(p, b, bad).pages;
     pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    pre[0] = 0;
-    for (int b = 0; b < batch; ++b) pre[b + 1] += pre[b];
-  }
+  if (warp == 0) running_sum(pre, batch, lane);
   __syncthreads();
-  const int T = pre[batch];
-  for (int u = blockIdx.x * (blockDim.x >> 5) + warp; u < T; u += gridDim.x * (blockDim.x >> 5)) {
-    int lo = 0, hi = batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      (pre[mid] <= u ? lo : hi) = mid;
-    }
-    const Span s = span_of(p, lo, bad);
-    const int r = u - pre[lo], head = r / s.pages, pg = s.page0 + r - head * s.pages, base = pg * kPage;
-    const uint8_t* page =
-        p.c.pages + ((size_t)page_of(p.c, p.c.table, p.c.table_cols, lo, pg, bad) * p.c.heads + head) * F::kPageBytes;
-    float sum[4][2] = {};
-    // rows that see the page: causal rows from the page's first slot on, and
-    // with a window up to the last that still reaches it
-    const int i0 = p.causal ? max(0, base - (s.len - s.n)) : 0;
-    const int i1 = p.window > 0 ? min(s.n, base + kPage - 1 + p.window - (s.len - s.n)) : s.n;
-    for (int r0 = i0 * p.group / 8 * 8; r0 < i1 * p.group; r0 += 8) {
-      QueryTile<D> q;
-      load_queries<D>(p, s, head, r0, lane, q);
-      float norm[2];
+  const long long T = pre[batch], all = (long long)gridDim.x * W, me = (long long)blockIdx.x * W + warp;
+  const int u0 = (int)(T * me / all), u1 = (int)(T * (me + 1) / all);
+  bool ok = true;
+  if (u0 < u1) {
+    Cursor c;
+    seek<ROWS>(p, pre, u0, c, bad);
+    PageFeed<D, ROWS> feed(c);
+    int issued = u0;
+    auto issue = [&](int k) {
+      const uint8_t* src = feed.next(p, pre, lane, bad);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar0 + 8 * k, G::kKeyBytes);
+        bulk_load(ring_s + k * G::kKeyBytes, src, G::kKeyBytes, bar0 + 8 * k);
+      }
+      ++issued;
+    };
+    for (int k = 0; k < S && issued < u1; ++k) issue(k);
+    QueryTile<D> q;
+    float norm[2];
+    auto load_rows = [&](int r0) {
+      load_queries<D>(p, c.s, c.head, r0, lane, q);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int row = r0 + 2 * (lane & 3) + k, i = row / p.group;
-        norm[k] = INFINITY;   // no weight from rows that are not there or see nothing
-        if (i < s.n) {
-          const float x = p.lse[(size_t)(s.first + i) * p.q_heads + head * p.group + row - i * p.group] * kLog2e;
-          if (x != -INFINITY) norm[k] = x;
+        norm[k] = -INFINITY;   // no weight from rows that are not there or see nothing
+        if (i < c.s.n) {
+          const float x = p.lse[(size_t)(c.s.first + i) * p.q_heads + c.head * p.group + row - i * p.group] * -kLog2e;
+          if (x != INFINITY) norm[k] = x;
         }
       }
+    };
+    const bool single = p.max_q * p.group <= 8;   // one row tile: loaded once per item
+    if (single) load_rows(0);
+    int stage = 0;
+    uint32_t parity = 0;
+    for (int u = u0; u < u1; ++u) {
+      const int base = c.page * kPage, past = c.s.len - c.s.n;
+      // lane 4r's slots, read ahead
+      float* out = p.weights + ((size_t)c.b * p.c.heads + c.head) * p.weights_cols + base + tile_perm(lane >> 2);
+      float sum[4][2];
+      const bool owner = (lane & 3) == 0;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        float x[1][4];
-        scores_16<D, 1>(page, mt, lane, &q, x);
+      for (int x = 0; x < 8; ++x)
+        sum[x >> 1][x & 1] = owner && base + tile_perm(lane >> 2) + 8 * x < c.s.len ? out[8 * x] : 0.0f;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, parity));
+      if (!ok) break;
+      // rows that see the page: causal rows from the page's first slot on, and
+      // with a window up to the last that still reaches it
+      const int i0 = p.causal ? max(0, base - past) : 0;
+      const int i1 = p.window > 0 ? min(c.s.n, base + kPage - 1 + p.window - past) : c.s.n;
+      for (int r0 = i0 * p.group / 8 * 8; r0 < i1 * p.group; r0 += 8) {
+        if (!single) load_rows(r0);
+        const bool whole = __all_sync(0xffffffffu, base >= max(q.lo[0], q.lo[1]) && base + kPage <= min(q.hi[0], q.hi[1]));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int slot = base + 16 * mt + tile_perm(lane >> 2) + 8 * (e >> 1);
-          const bool seen = slot >= q.lo[e & 1] && slot < q.hi[e & 1];
-          if (seen) sum[mt][e >> 1] += exp2_approx(fmaf(x[0][e], q.factor[e & 1], -norm[e & 1]));
+        for (int mt = 0; mt < 4; ++mt) {
+          float x[1][4];
+          scores_16<D, 1>(ring + stage * G::kKeyBytes, mt, lane, &q, x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int slot = base + 16 * mt + tile_perm(lane >> 2) + 8 * (e >> 1);
+            const float w = exp2_approx(fmaf(x[0][e], q.factor[e & 1], norm[e & 1]));
+            sum[mt][e >> 1] += whole || (slot >= q.lo[e & 1] && slot < q.hi[e & 1]) ? w : 0.0f;
+          }
         }
+      }
+      __syncwarp();
+      if (issued < u1) issue(stage);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        float y = sum[x >> 1][x & 1];
+        y += __shfl_xor_sync(0xffffffffu, y, 1);
+        y += __shfl_xor_sync(0xffffffffu, y, 2);
+        if (owner && base + tile_perm(lane >> 2) + 8 * x < c.s.len) out[8 * x] = y;
+      }
+      if (++stage == S) {
+        stage = 0;
+        parity ^= 1;
+      }
+      if (u + 1 == u1) break;
+      if (++c.page == c.s.page0 + c.s.pages) {
+        seek<ROWS>(p, pre, u + 1, c, bad);
+        if (single) load_rows(0);
       }
     }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float x = sum[mt][k];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        const int slot = base + 16 * mt + tile_perm(lane >> 2) + 8 * k;
-        if ((lane & 3) == 0 && slot < s.len)
-          p.weights[((size_t)lo * p.c.heads + head) * p.weights_cols + slot] += x;
-      }
+    if (!ok && lane == 0) {   // gave up: nothing may land after the CTA is gone
+      atomicOr(p.error, 1u);
+      for (int k = 0; k < S; ++k) mbar_wait(bar0 + 8 * k, k < stage ? parity ^ 1 : parity);
+    }
   }
   if (bad) atomicOr(p.error, kErrIndex);
 }

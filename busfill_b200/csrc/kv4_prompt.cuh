@@ -219,20 +219,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) {
-    int total = 0;
-    if (lane == 0) pre[0] = 0;
-    for (int b0 = 0; b0 < batch; b0 += 32) {
-      int x = b0 + lane < batch ? pre[b0 + lane + 1] : 0;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, m);
-        if (lane >= m) x += y;
-      }
-      if (b0 + lane < batch) pre[b0 + lane + 1] = total + x;
-      total += __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
+  if (warp == 0) running_sum(pre, batch, lane);
   __syncthreads();
   const uint32_t tmem = misc[0];
   const int T = pre[batch];
