@@ -259,8 +259,10 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.weights_cols = a->weights_cols;
   p.scale_log2 = a->scale * kLog2e;
   p.tokens = a->tokens, p.q_heads = a->q_heads, p.group = a->q_heads / cache->heads;
+  p.by_group = divide_by((unsigned)p.group);
   p.max_q = a->q_start ? a->max_q : 1;
   p.causal = a->causal != 0, p.window = a->window, p.bf16 = a->dtype == BUSFILL_TYPE_BF16;
+  p.wide_out = aligned(a->out, 32) && (a->out_token | a->out_head) % 16 == 0;
   p.counters = static_cast<unsigned*>(work);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
   p.error = ctx.error;

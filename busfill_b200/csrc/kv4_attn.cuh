@@ -54,7 +54,9 @@ struct AttnParams {
   long long q_token, q_head, o_token, o_head, weights_cols;
   float scale_log2;  // scale * log2(e)
   int tokens, q_heads, group, max_q;
+  Divisor by_group;  // division by group
   int causal, window, bf16;
+  int wide_out;      // output rows start on 32 bytes
   unsigned* counters;   // one per CTA, zero between calls
   float* part;          // partial results (layout of the kernel)
   unsigned* error;
@@ -147,7 +149,7 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s,
                                              QueryTile<D>& t) {
   constexpr int NB = Fmt<D>::kBlocks;
   const int n = lane >> 2, j = lane & 3;
-  const int row = r0 + n, i = row / p.group;
+  const int row = r0 + n, i = p.by_group(row);
   const bool live = i < s.n;
   float x[NB][8];
   float top = 0.0f;
@@ -202,7 +204,7 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s,
       asm("" : "+f"(t.corr[b][k + 2]));   // four registers, ready to be an accumulator
     }
     t.factor[k] = __shfl_sync(0xffffffffu, factor, from);
-    const int ri = (r0 + 2 * j + k) / p.group;
+    const int ri = p.by_group(r0 + 2 * j + k);
     t.lo[k] = 0;   // columns without a row see everything, so that they hold up no page
     t.hi[k] = s.len;
     if (ri < s.n) sees(p, s, ri, t.lo[k], t.hi[k]);
@@ -423,7 +425,7 @@ __device__ __forceinline__ int channel_of(int lane, int b, int u, int e) {
 
 template <int D>
 __device__ __forceinline__ void store_out(const AttnParams& p, const Span& s, int head, int row, int ch, float x) {
-  const int i = row / p.group;
+  const int i = p.by_group(row);
   if (i >= s.n) return;
   const size_t at = (size_t)(s.first + i) * p.o_token + (size_t)(head * p.group + row - i * p.group) * p.o_head + ch;
   if (p.bf16)
@@ -434,7 +436,7 @@ __device__ __forceinline__ void store_out(const AttnParams& p, const Span& s, in
 // four channels, ch a multiple of 4
 __device__ __forceinline__ void store_out4(const AttnParams& p, const Span& s, int head, int row, int ch,
                                            const float4& o, float f) {
-  const int i = row / p.group;
+  const int i = p.by_group(row);
   if (i >= s.n) return;
   const size_t at = (size_t)(s.first + i) * p.o_token + (size_t)(head * p.group + row - i * p.group) * p.o_head + ch;
   uint2 v;
@@ -447,7 +449,7 @@ __device__ __forceinline__ void store_out4(const AttnParams& p, const Span& s, i
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = v;
 }
 __device__ __forceinline__ void store_lse(const AttnParams& p, const Span& s, int head, int row, float m, float l) {
-  const int i = row / p.group;
+  const int i = p.by_group(row);
   if (!p.lse || i >= s.n) return;
   p.lse[(size_t)(s.first + i) * p.q_heads + head * p.group + row - i * p.group] =
       l > 0.0f ? (m + log2f(l)) * kLn2 : l == 0.0f ? -INFINITY : l;
@@ -580,8 +582,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     if (n == 0 && blockIdx.x == 0) {   // rows that see nothing
       for (int i = 0; i < s.n; ++i)
         for (int h = 0; h < p.q_heads; ++h) {
-          for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, h / p.group, i * p.group + h % p.group, ch, 0.0f);
-          store_lse(p, s, h / p.group, i * p.group + h % p.group, 0.0f, 0.0f);
+          for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, p.by_group(h), i * p.group + h % p.group, ch, 0.0f);
+          store_lse(p, s, p.by_group(h), i * p.group + h % p.group, 0.0f, 0.0f);
         }
     }
   }
@@ -896,7 +898,7 @@ __global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(
       load_queries<D>(p, c.s, c.head, r0, lane, q);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int row = r0 + 2 * (lane & 3) + k, i = row / p.group;
+        const int row = r0 + 2 * (lane & 3) + k, i = p.by_group(row);
         norm[k] = -INFINITY;   // no weight from rows that are not there or see nothing
         if (i < c.s.n) {
           const float x = p.lse[(size_t)(c.s.first + i) * p.q_heads + c.head * p.group + row - i * p.group] * -kLog2e;

@@ -39,6 +39,19 @@ __host__ __device__ __forceinline__ int value_swizzle(int t) {
 // token's value scale sits in this column: 0,1,3,2,4,5,7,6.
 __host__ __device__ __forceinline__ int tile_perm(int t) { return t ^ ((t >> 1) & 1); }
 
+// n / d for 0 <= n < 2^31 by a multiplication (set up on the host by divide_by)
+struct Divisor {
+  unsigned mul, shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    return (int)((__umulhi((unsigned)n, mul) + (unsigned)n) >> shift);
+  }
+};
+inline Divisor divide_by(unsigned d) {
+  unsigned shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return {(unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
+
 struct View {
   uint8_t* pages;
   const int* table;

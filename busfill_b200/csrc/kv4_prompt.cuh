@@ -18,13 +18,16 @@
 // than 2^8 since the last time (p stays below 2^8, far inside fp16).
 //
 // Warps: 0 copies raw pages into a ring (bulk copies); 1 issues the MMAs and
-// owns TMEM; 4-7 and 8-11 softmax of row tile 0 and 1, thread = row; 12-15
+// owns TMEM; 2 hands out the work; 4-7 and 8-11 softmax of row tile 0 and 1, thread = row; 12-15
 // dequantize. Registers move from the other warps to the softmax.
 //
-// Work split: the list of all items' tiles is cut into equal ranges, one per
+// Work split: the list of all items is cut into ranges of equal cost, one per
 // CTA of a persistent grid, so ragged and causal shapes balance by themselves;
-// an item that is cut leaves fp32 partial sums in the workspace, which the
-// CTA that finishes last joins in the order of the ranges (repeatable).
+// an item costs its tiles and kItemCost more. An item that is cut leaves fp32
+// partial sums in the workspace, which the CTA that finishes last joins in the
+// order of the ranges (repeatable). Warp 2 walks the list and hands out what
+// comes next as descriptors in shared memory: the index arithmetic stays off
+// the other warps.
 //
 // Every wait is bounded (ptx.cuh: kWaitTimeoutNs).
 #pragma once
@@ -103,6 +106,32 @@ __device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign,
   }
 }
 
+// packed fp32 pairs (sm_100): half the issue slots
+__device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float t) {   // (a, b) * s + t
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %2};\n\t"
+      "mov.b64 z, {%3, %3};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(s), "f"(t));
+}
+__device__ __forceinline__ void add_f32x2(float& a, float& b, float x, float y) {   // (a, b) += (x, y)
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 namespace prompt {
 
 constexpr int kThreads = 512;
@@ -129,11 +158,14 @@ struct Geo {
   static constexpr int kRawOff = kQOff + kRowTiles * kQTileBytes;
   static constexpr int kFacOff = kRawOff + kRawStages * kRawBytes;      // factor of every row
   static constexpr int kBarOff = kFacOff + kRows * 4;
+  static constexpr int kDescs = 4;                         // descriptors in flight
   static constexpr int bRawFull = 0, bRawEmpty = bRawFull + kRawStages, bKvFull = bRawEmpty + kRawStages,
-                       bKvEmpty = bKvFull + kSlots, bS = bKvEmpty + kSlots, bP = bS + 2, bO = bP + 2, bQ = bO + 2,
-                       bFinal = bQ + 2, kBars = bFinal + 1;
+                       bKvEmpty = bKvFull + kSlots, bS = bKvEmpty + kSlots, bP = bS + 2, bO = bP + 4, bQ = bO + 2,
+                       bDescFull = bQ + 2, bDescEmpty = bDescFull + kDescs, bParts = bDescEmpty + kDescs,
+                       bLast = bParts + 1, bFinal = bLast + 1, kBars = bFinal + 1;
   static constexpr int kMiscOff = kBarOff + kBars * 8;
-  static constexpr int kPreOff = kMiscOff + 16;            // tiles before each sequence
+  static constexpr int kDescOff = (kMiscOff + 16 + 15) / 16 * 16;
+  static constexpr int kPreOff = kDescOff + kDescs * 64;   // cost before each sequence
   static constexpr int kBytes = kPreOff + (kMaxBatch + 1) * 4;
   static constexpr int kAlloc = kBytes + 1024;
   static_assert(kAlloc <= 232448, "dynamic shared memory");
@@ -144,13 +176,24 @@ struct Geo {
   static constexpr int kPartFloats = kRows * (D + 2);
 };
 
-// An item: rows [row0, row0 + kRows) of (sequence, head); tiles [tile0, tile0 + tiles).
+// An item: group t of kRows rows of (sequence, head); tiles [tile0, tile0 + tiles).
 struct Item {
-  int b, head, t;      // t: row tile pair of the sequence
+  int b, head, t;
   int groups;          // of the sequence
   int tile0, tiles;
   Span s;
 };
+// What a CTA does of an item.
+struct Work {
+  int b, head, first, n;         // first row and rows of the sequence
+  int len, row0, tile0, tiles;   // tiles 0: the end
+  int kind, c_first, c_last, row_tiles;
+};
+enum { kWhole = 0, kTail = 1, kHead = 2 };   // kTail: began in an earlier CTA; kHead: goes on in the next
+static_assert(sizeof(Work) <= 64, "descriptor slots");
+// Tiles that the start and the end of an item are worth (queries, epilogue,
+// refilling the pipeline).
+constexpr int kItemCost = 2;
 
 template <int D>
 __device__ __forceinline__ int groups_of(const AttnParams& p, const Span& s) {
@@ -160,7 +203,7 @@ __device__ __forceinline__ int groups_of(const AttnParams& p, const Span& s) {
 template <int D>
 __device__ __forceinline__ int tiles_of(const AttnParams& p, const Span& s, int t, int& tile0) {
   constexpr int R = Geo<D>::kRows, K = Geo<D>::kTile;
-  const int i0 = t * R / p.group, i1 = min(s.n - 1, (t * R + R - 1) / p.group);
+  const int i0 = p.by_group(t * R), i1 = min(s.n - 1, p.by_group(t * R + R - 1));
   int lo, hi, x;
   sees(p, s, i0, lo, x);
   sees(p, s, i1, x, hi);
@@ -188,9 +231,12 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
 
   if (warp == 0) {
     for (int i = lane; i < G::kBars; i += 32) {
-      const bool warps4 = (i >= G::bRawEmpty && i < G::bKvEmpty) || (i >= G::bP && i < G::bP + 2) ||
-                          (i >= G::bQ && i < G::bQ + 2);
-      mbar_init(BAR(i), warps4 ? 4 : 1);
+      int n = 1;
+      if ((i >= G::bRawEmpty && i < G::bKvEmpty) || (i >= G::bP && i < G::bP + 4) || (i >= G::bQ && i < G::bQ + 2))
+        n = 4;
+      if (i >= G::bDescEmpty && i < G::bDescEmpty + G::kDescs) n = 14;   // all warps but 2 and 3
+      if (i == G::bParts) n = 8;
+      mbar_init(BAR(i), n);
     }
     fence_mbar_init();
   } else if (warp == 1) {
@@ -199,20 +245,20 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   }
   pdl_wait_prerequisites();
   pdl_launch_dependents();
-  // tiles of every sequence (a warp each), then their running sum
+  // cost of every sequence (a warp each), then the running sum
   bool bad = false;
   for (int b = warp; b < batch; b += kThreads / 32) {
     const Span s = span_of(p, b, bad);
     const int groups = groups_of<D>(p, s);
     int n = 0, x;
-    for (int t = lane; t < groups; t += 32) n += tiles_of<D>(p, s, t, x);
+    for (int t = lane; t < groups; t += 32) n += tiles_of<D>(p, s, t, x) + kItemCost;
     n = __reduce_add_sync(0xffffffffu, n) * p.c.heads;
     if (lane == 0) pre[b + 1] = n;
     if (s.len == 0 && blockIdx.x == 0) {   // nothing cached: rows are 0
       for (int r = lane; r < s.n * p.q_heads; r += 32) {
         const int i = r / p.q_heads, h = r - i * p.q_heads;
-        for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, h / p.group, i * p.group + h % p.group, ch, 0.0f);
-        store_lse(p, s, h / p.group, i * p.group + h % p.group, 0.0f, 0.0f);
+        for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, p.by_group(h), i * p.group + h % p.group, ch, 0.0f);
+        store_lse(p, s, p.by_group(h), i * p.group + h % p.group, 0.0f, 0.0f);
       }
     }
   }
@@ -222,76 +268,6 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   if (warp == 0) running_sum(pre, batch, lane);
   __syncthreads();
   const uint32_t tmem = misc[0];
-  const int T = pre[batch];
-  const long long ctas = min((int)gridDim.x, T);
-  const bool idle = (int)blockIdx.x >= ctas;
-  const int u0 = idle ? 0 : (int)((long long)T * blockIdx.x / ctas);
-  const int u1 = idle ? 0 : (int)((long long)T * (blockIdx.x + 1) / ctas);
-
-  // the item of tile u0 and where in it u0 lies (all warps alike)
-  Item first{};
-  int skip = 0;   // tiles of the first item that belong to CTAs before
-  if (u0 < u1) {
-    int lo = 0, hi = batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      (pre[mid] <= u0 ? lo : hi) = mid;
-    }
-    first.b = lo;
-    first.s = span_of(p, lo, bad);
-    first.groups = groups_of<D>(p, first.s);
-    const int per_head = (pre[lo + 1] - pre[lo]) / p.c.heads;
-    int r = u0 - pre[lo];
-    first.head = r / per_head;
-    r -= first.head * per_head;
-    for (int t0 = 0;; t0 += 32) {
-      int x0;
-      const int n = t0 + lane < first.groups ? tiles_of<D>(p, first.s, t0 + lane, x0) : 0;
-      int x = n;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, m);
-        if (lane >= m) x += y;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, x > r);
-      if (over) {
-        const int k = __ffs(over) - 1;
-        first.t = t0 + k;
-        skip = r - __shfl_sync(0xffffffffu, x - n, k);
-        break;
-      }
-      r -= __shfl_sync(0xffffffffu, x, 31);
-    }
-    first.tiles = tiles_of<D>(p, first.s, first.t, first.tile0);
-  }
-  // step to the item behind `it`
-  auto next_item = [&](Item& it) {
-    if (++it.t == it.groups) {
-      it.t = 0;
-      if (++it.head == p.c.heads) {
-        it.head = 0;
-        do ++it.b;
-        while (it.b < batch && pre[it.b + 1] == pre[it.b]);
-        if (it.b >= batch) return;
-        it.s = span_of(p, it.b, bad);
-        it.groups = groups_of<D>(p, it.s);
-      }
-    }
-    it.tiles = tiles_of<D>(p, it.s, it.t, it.tile0);
-  };
-  // for every piece (part of an item) of this CTA: f(item, first tile, tiles, whole)
-  auto for_pieces = [&](auto f) {
-    Item it = first;
-    int from = skip;
-    for (int u = u0; u < u1;) {
-      const int n = min(it.tiles - from, u1 - u);
-      if (!f(it, from, n, u)) return;
-      u += n;
-      from = 0;
-      if (u < u1) next_item(it);
-    }
-  };
-  auto row_tiles = [&](const Item& it) { return RT == 2 && it.s.n * p.group - it.t * G::kRows > 128 ? 2 : 1; };
 
   bool ok = true;
   auto wait = [&](int bar, uint32_t phase) -> bool {   // the warp waits for completion number `phase` of the barrier
@@ -301,26 +277,134 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   auto failed = [&](unsigned bit) {
     if (lane == 0) atomicOr(p.error, bit);
   };
+  uint32_t taken = 0;   // descriptors this warp has seen
+  auto next_piece = [&]() -> Work {
+    Work x;
+    const int st = taken % G::kDescs;
+    if (!wait(G::bDescFull + st, taken / G::kDescs)) {
+      x.tiles = 0;
+      return x;
+    }
+    x = *reinterpret_cast<const Work*>(smem + G::kDescOff + 64 * st);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(BAR(G::bDescEmpty + st));
+    ++taken;
+    return x;
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 0) {
+    if (warp == 2) {
+      // ---------------- work list ----------------
+      const int T = pre[batch];
+      const long long ctas = min((int)gridDim.x, T);
+      const bool idle = (int)blockIdx.x >= ctas;
+      const int u0 = idle ? 0 : (int)((long long)T * blockIdx.x / ctas);
+      const int u1 = idle ? 0 : (int)((long long)T * (blockIdx.x + 1) / ctas);
+      uint32_t n = 0;
+      auto push = [&](const Work& x) -> bool {
+        const int st = n % G::kDescs;
+        if (!wait(G::bDescEmpty + st, n / G::kDescs + 1)) return false;
+        if (lane == 0) {
+          *reinterpret_cast<Work*>(smem + G::kDescOff + 64 * st) = x;
+          mbar_arrive(BAR(G::bDescFull + st));
+        }
+        __syncwarp();
+        ++n;
+        return true;
+      };
+      if (u0 < u1) {
+        // the item at cost u0
+        Item it;
+        int lo = 0, hi = batch;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          (pre[mid] <= u0 ? lo : hi) = mid;
+        }
+        it.b = lo;
+        it.s = span_of(p, lo, bad);
+        it.groups = groups_of<D>(p, it.s);
+        const int per_head = (pre[lo + 1] - pre[lo]) / p.c.heads;
+        int r = u0 - pre[lo];
+        it.head = r / per_head;
+        r -= it.head * per_head;
+        for (int t0 = 0;; t0 += 32) {
+          int x0;
+          const int c = t0 + lane < it.groups ? tiles_of<D>(p, it.s, t0 + lane, x0) + kItemCost : 0;
+          int x = c;
+#pragma unroll
+          for (int m = 1; m < 32; m <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, m);
+            if (lane >= m) x += y;
+          }
+          const unsigned over = __ballot_sync(0xffffffffu, x > r);
+          if (over) {
+            const int k = __ffs(over) - 1;
+            it.t = t0 + k;
+            r -= __shfl_sync(0xffffffffu, x - c, k);
+            break;
+          }
+          r -= __shfl_sync(0xffffffffu, x, 31);
+        }
+        // tile k of an item that begins at cost x lies at cost x + kItemCost + k
+        auto cta_of = [&](int y) { return (int)((((long long)y + 1) * ctas - 1) / T); };
+        for (int x = u0 - r;;) {
+          it.tiles = tiles_of<D>(p, it.s, it.t, it.tile0);
+          const int from = min(max(u0 - x - kItemCost, 0), it.tiles), to = min(max(u1 - x - kItemCost, 0), it.tiles);
+          if (to > from) {
+            Work y;
+            y.b = it.b, y.head = it.head, y.first = it.s.first, y.n = it.s.n, y.len = it.s.len;
+            y.row0 = it.t * G::kRows, y.tile0 = it.tile0 + from, y.tiles = to - from;
+            y.kind = from > 0 ? kTail : to < it.tiles ? kHead : kWhole;
+            y.c_first = cta_of(x + kItemCost), y.c_last = cta_of(x + kItemCost + it.tiles - 1);
+            y.row_tiles = RT == 2 && it.s.n * p.group - y.row0 > 128 ? 2 : 1;
+            if (!push(y)) break;
+            // its queries on their way to L2
+            for (int k = lane; k < G::kRows; k += 32) {
+              const int row = y.row0 + k, tok = p.by_group(row);
+              if (tok < y.n) {
+                const uint16_t* q = static_cast<const uint16_t*>(p.q) + (size_t)(y.first + tok) * p.q_token +
+                                    (size_t)(y.head * p.group + row - tok * p.group) * p.q_head;
+#pragma unroll
+                for (int c = 0; c < D; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + c));
+              }
+            }
+          }
+          x += it.tiles + kItemCost;
+          if (x >= u1) break;
+          if (++it.t == it.groups) {
+            it.t = 0;
+            if (++it.head == p.c.heads) {
+              it.head = 0;
+              do ++it.b;
+              while (it.b < batch && pre[it.b + 1] == pre[it.b]);
+              if (it.b >= batch) break;
+              it.s = span_of(p, it.b, bad);
+              it.groups = groups_of<D>(p, it.s);
+            }
+          }
+        }
+      }
+      Work end{};
+      push(end);
+      if (!ok) failed(1u);
+    } else if (warp == 0) {
       // ---------------- raw pages ----------------
       uint32_t n = 0;
-      for_pieces([&](const Item& it, int from, int tiles, int) {
-        const int pages = (it.s.len + kPage - 1) / kPage;
-        for (int j = 0; j < tiles; ++j) {
-          const int page0 = (it.tile0 + from + j) * G::kTilePages;
+      for (Work x = next_piece(); ok && x.tiles > 0; x = next_piece()) {
+        const int pages = (x.len + kPage - 1) / kPage;
+        for (int j = 0; ok && j < x.tiles; ++j) {
+          const int page0 = (x.tile0 + j) * G::kTilePages;
           const int have = min(G::kTilePages, pages - page0);
           const uint8_t* src[G::kTilePages];
 #pragma unroll
           for (int k = 0; k < G::kTilePages; ++k)
-            src[k] = p.c.pages + ((size_t)(k < have ? page_of(p.c, p.c.table, p.c.table_cols, it.b, page0 + k, bad) : 0) *
-                                      p.c.heads + it.head) * F::kPageBytes;
+            src[k] = p.c.pages + ((size_t)(k < have ? page_of(p.c, p.c.table, p.c.table_cols, x.b, page0 + k, bad) : 0) *
+                                      p.c.heads + x.head) * F::kPageBytes;
 #pragma unroll
-          for (int half = 0; half < 2; ++half, ++n) {
+          for (int half = 0; half < 2; ++half) {
             const int st = n % G::kRawStages;
-            if (!wait(G::bRawEmpty + st, n / G::kRawStages + 1)) return false;
+            if (!wait(G::bRawEmpty + st, n / G::kRawStages + 1)) break;
             if (elect_one()) {
               mbar_arrive_expect_tx(BAR(G::bRawFull + st), have * G::kHalfPage);
 #pragma unroll
@@ -330,10 +414,10 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
                             G::kHalfPage, BAR(G::bRawFull + st));
             }
             __syncwarp();
+            ++n;
           }
         }
-        return true;
-      });
+      }
       if (!ok) failed(1u);
       // nothing may land after the CTA is gone
       ok = true;
@@ -353,8 +437,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
                      make_sdesc_sw128(b + (k / 4) * K * 128 + (k % 4) * 32), kIdescS, k > 0);
         tc_commit(BAR(G::bS + i));
       };
-      for_pieces([&](const Item& it, int, int tiles, int) {
-        const int nr = row_tiles(it);
+      auto one_piece = [&](int nr, int tiles) -> bool {
         for (int i = 0; i < nr; ++i)
           if (!wait(G::bQ + i, items[i]++)) return false;
         if (!wait(G::bKvFull + half % G::kSlots, half / G::kSlots)) return false;
@@ -371,14 +454,23 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           if (!wait(G::bKvFull + vs, half / G::kSlots)) return false;
           if (more && !wait(G::bKvFull + ks, (half + 1) / G::kSlots)) return false;
           for (int i = 0; i < nr; ++i) {
-            if (!wait(G::bP + i, done[i]++)) return false;
-            tc_fence_after();
-            if (elect_one()) {
+            auto issue_o = [&](int part) {
               const uint32_t b = sbase + G::kSlotOff + vs * G::kSlotBytes;
 #pragma unroll
-              for (int k = 0; k < K / 16; ++k)
+              for (int x = 0; x < K / 32; ++x) {
+                const int k = part * (K / 32) + x;
                 mma_f16_ts(tmem + G::kO + i * D, tmem + G::kS + i * K + 8 * k,
                            make_sdesc_mn_sw128(b + k * 16 * 128, K * 128), kIdescO, j > 0 || k > 0);
+              }
+            };
+            if (!wait(G::bP + i, done[i])) return false;
+            tc_fence_after();
+            if (elect_one()) issue_o(0);
+            __syncwarp();
+            if (!wait(G::bP + 2 + i, done[i]++)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+              issue_o(1);
               tc_commit(BAR(G::bO + i));
               if (more) issue_s(i, ks);
               if (i + 1 == nr) {
@@ -391,7 +483,9 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           half += more ? 2 : 1;
         }
         return true;
-      });
+      };
+      for (Work x = next_piece(); ok && x.tiles > 0; x = next_piece())
+        if (!one_piece(x.row_tiles, x.tiles)) break;
       if (!ok) failed(4u);
       // every MMA has completed before TMEM is freed
       ok = true;
@@ -405,134 +499,177 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int w = warp - kDequantWarp0, j = lane & 3;
     uint32_t n = 0;
-    for_pieces([&](const Item& it, int from, int tiles, int) {
-      for (int tile = 0; tile < tiles; ++tile) {
-        const int base = (it.tile0 + from + tile) * K;
+    for (Work x0 = next_piece(); ok && x0.tiles > 0; x0 = next_piece()) {
+      const int len = x0.len;
+      int base = x0.tile0 * K;
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half, ++n) {
-          const int st = n % G::kRawStages, slot = n % G::kSlots;
-          if (!wait(G::bRawFull + st, n / G::kRawStages)) return false;
-          if (!wait(G::bKvEmpty + slot, n / G::kSlots + 1)) return false;
-          const uint8_t* raw = smem + G::kRawOff + st * G::kRawBytes;
-          uint8_t* dst = smem + G::kSlotOff + slot * G::kSlotBytes;
+      for (int left = 2 * x0.tiles; left > 0; --left, ++n) {
+        const int half = left & 1;   // keys, then values
+        const int st = n % G::kRawStages, slot = n % G::kSlots;
+        if (!wait(G::bRawFull + st, n / G::kRawStages)) break;
+        if (!wait(G::bKvEmpty + slot, n / G::kSlots + 1)) break;
+        const uint8_t* raw = smem + G::kRawOff + st * G::kRawBytes;
+        uint8_t* dst = smem + G::kSlotOff + slot * G::kSlotBytes;
 #pragma unroll
-          for (int pass = 0; pass < K / 32; ++pass) {
-            // lane j of a token's four: words j of all its blocks
-            const int tok = w * (K / 4) + pass * 8 + (lane >> 2);
-            const uint8_t* pg = raw + (tok / kPage) * G::kHalfPage;
-            const int t = tok & (kPage - 1);
-            uint32_t x[NB];
-            __half2 d[NB];
-            if (half == 0) {
-              uint32_t sc[NB / 2];
-              lds_words<NB>(pg + t * F::kRow + j * 4 * NB, x);
-              lds_words<NB / 2>(pg + F::kKeyScale + t * 2 * NB, sc);
+        for (int pass = 0; pass < K / 32; ++pass) {
+          // lane j of a token's four: words j of all its blocks
+          const int tok = w * (K / 4) + pass * 8 + (lane >> 2);
+          const uint8_t* pg = raw + (tok / kPage) * G::kHalfPage;
+          const int t = tok & (kPage - 1);
+          uint32_t x[NB];
+          __half2 d[NB];
+          if (half == 0) {
+            uint32_t sc[NB / 2];
+            lds_words<NB>(pg + t * F::kRow + j * 4 * NB, x);
+            lds_words<NB / 2>(pg + F::kKeyScale + t * 2 * NB, sc);
 #pragma unroll
-              for (int b = 0; b < NB; ++b)
-                d[b] = b & 1 ? __high2half2(u32_as_h2(sc[b / 2])) : __low2half2(u32_as_h2(sc[b / 2]));
-            } else {
-              uint32_t y[NB];   // value words 2j and 2j + 1 of all blocks
-              lds_words<NB>(pg + t * F::kRow + ((2 * j) ^ value_swizzle<D>(t)) * 2 * NB, y);
-              const bool live = base + tok < it.s.len;   // slots behind the sequence hold anything
-#pragma unroll
-              for (int b = 0; b < NB; ++b) {
-                x[b] = prmt(y[b / 2], y[NB / 2 + b / 2], b & 1 ? 0x7632u : 0x5410u);
-                const __half s = *reinterpret_cast<const __half*>(pg + 32 * D + (b * kPage + tile_perm(t)) * 2);
-                d[b] = __half2half2(live ? s : __ushort_as_half(0));
-              }
-            }
-            // odd tokens write their blocks in swapped pairs, so that the 8
-            // lanes of a store phase cover all banks
-            if (t & 1) {
-#pragma unroll
-              for (int b = 0; b < NB; b += 2) {
-                const uint32_t tx = x[b];
-                x[b] = x[b + 1], x[b + 1] = tx;
-                const __half2 td = d[b];
-                d[b] = d[b + 1], d[b + 1] = td;
-              }
-            }
+            for (int b = 0; b < NB; ++b)
+              d[b] = b & 1 ? __high2half2(u32_as_h2(sc[b / 2])) : __low2half2(u32_as_h2(sc[b / 2]));
+          } else {
+            uint32_t y[NB];   // value words 2j and 2j + 1 of all blocks
+            lds_words<NB>(pg + t * F::kRow + ((2 * j) ^ value_swizzle<D>(t)) * 2 * NB, y);
+            const bool live = base + tok < len;   // slots behind the sequence hold anything
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              const int blk = b ^ (t & 1);
-              const int piece = 4 * (blk & 1) + j;   // 16-byte piece of the 128-byte row
-              *reinterpret_cast<uint4*>(dst + (b >> 1) * K * 128 + tok * 128 + ((piece ^ (tok & 7)) << 4)) =
-                  dequant_key8(x[b], d[b], minus_72(d[b]));
+              x[b] = prmt(y[b / 2], y[NB / 2 + b / 2], b & 1 ? 0x7632u : 0x5410u);
+              const __half s = *reinterpret_cast<const __half*>(pg + 32 * D + (b * kPage + tile_perm(t)) * 2);
+              d[b] = __half2half2(live ? s : __ushort_as_half(0));
             }
           }
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(BAR(G::bRawEmpty + st));
-            mbar_arrive(BAR(G::bKvFull + slot));
+          // odd tokens write their blocks in swapped pairs, so that the 8
+          // lanes of a store phase cover all banks
+          if (t & 1) {
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+              const uint32_t tx = x[b];
+              x[b] = x[b + 1], x[b + 1] = tx;
+              const __half2 td = d[b];
+              d[b] = d[b + 1], d[b + 1] = td;
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const int blk = b ^ (t & 1);
+            const int piece = 4 * (blk & 1) + j;   // 16-byte piece of the 128-byte row
+            *reinterpret_cast<uint4*>(dst + (b >> 1) * K * 128 + tok * 128 + ((piece ^ (tok & 7)) << 4)) =
+                dequant_key8(x[b], d[b], minus_72(d[b]));
           }
         }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(BAR(G::bRawEmpty + st));
+          mbar_arrive(BAR(G::bKvFull + slot));
+        }
+        base += half * K;
       }
-      return true;
-    });
+    }
     if (!ok) failed(8u);
   } else {
     // ---------------- softmax ----------------
-    // A warp whose wait ran out goes on through its pieces without waiting or
-    // writing, so that the named barriers (no timeout) always fill.
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int i = (warp - kSoftmaxWarp0) / 4, q = warp & 3;   // row tile, lane quarter
     const int my_row = 32 * q + lane;
     const uint32_t tm = tmem + ((uint32_t)(32 * q) << 16);
     const uint32_t ts = tm + G::kS + i * K, to = tm + G::kO + i * D;
-    uint32_t done = 0;
+    uint32_t done = 0, joins = 0;
     const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    float* my_part = p.part + (size_t)blockIdx.x * 2 * G::kPartFloats;
-    for_pieces([&](const Item& it, int from, int tiles, int u) {
-      const bool active = i < row_tiles(it);
-      const int row0 = it.t * G::kRows + i * 128;
-      const int row = row0 + my_row;
-      float m = -INFINITY, l = 0.0f;
-      if (active) {
-        // queries: lanes together on a row, 16 bytes each
-        constexpr int LPR = D / 8, RPI = 32 / LPR;
-        const int c = lane % LPR;
-#pragma unroll 4
-        for (int k = 0; k < 32; k += RPI) {
-          const int r = 32 * q + k + lane / LPR;
-          const int tok = (row0 + r) / p.group;
-          const bool live = tok < it.s.n;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (live)
-            v = __ldg(reinterpret_cast<const uint4*>(
-                static_cast<const uint16_t*>(p.q) + (size_t)(it.s.first + tok) * p.q_token +
-                (size_t)(it.head * p.group + row0 + r - tok * p.group) * p.q_head + 8 * c));
+    // queries of a piece's row tile to shared memory, lanes together on a row,
+    // 16 bytes each
+    constexpr int LPR = D / 8, RPI = 32 / LPR, NQ = 32 / RPI;
+    auto load_q = [&](const Work& x) {
+      const int row0 = x.row0 + i * 128 + 32 * q, c = lane % LPR;
+      constexpr int BATCH = NQ < 16 ? NQ : 16;   // loads in flight
+#pragma unroll 1
+      for (int k0 = 0; k0 < NQ; k0 += BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int row = row0 + (k0 + k) * RPI + lane / LPR, tok = p.by_group(row);
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (tok < x.n)
+            v[k] = __ldg(reinterpret_cast<const uint4*>(
+                static_cast<const uint16_t*>(p.q) + (size_t)(x.first + tok) * p.q_token +
+                (size_t)(x.head * p.group + row - tok * p.group) * p.q_head + 8 * c));
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int r = 32 * q + (k0 + k) * RPI + lane / LPR;
           float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
-          normalize_query8<LPR>(v, p.bf16, sign, fac);
+          normalize_query8<LPR>(v[k], p.bf16, sign, fac);
           *reinterpret_cast<uint4*>(smem + G::kQOff + i * G::kQTileBytes + (c / 8) * 128 * 128 + r * 128 +
-                                    (((c & 7) ^ (r & 7)) << 4)) = v;
+                                    (((c & 7) ^ (r & 7)) << 4)) = v[k];
           if (c == 0) factors[i * 128 + r] = fac;
         }
-        fence_proxy_async_shared();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(G::bQ + i));
-        const float f = factors[i * 128 + my_row];
-        int lo = 0, hi = 0x7fffffff;
-        const int tok = row / p.group;
-        if (tok < it.s.n) sees(p, it.s, tok, lo, hi);
+      }
+      fence_proxy_async_shared();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(G::bQ + i));
+    };
+    // 32 columns of an output row
+    auto put32 = [&](size_t at, const float* x, float scale) {
+      uint32_t e[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const float a = x[2 * y] * scale, b = x[2 * y + 1] * scale;
+        if (p.bf16) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+          e[y] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          e[y] = h2_as_u32(__floats2half2_rn(a, b));
+        }
+      }
+      uint16_t* to_row = static_cast<uint16_t*>(p.out) + at;
+      if (p.wide_out) {   // whole 32-byte sectors
+#pragma unroll
+        for (int y = 0; y < 16; y += 8)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to_row + 2 * y), "r"(e[y]),
+                       "r"(e[y + 1]), "r"(e[y + 2]), "r"(e[y + 3]), "r"(e[y + 4]), "r"(e[y + 5]), "r"(e[y + 6]),
+                       "r"(e[y + 7])
+                       : "memory");
+      } else {
+#pragma unroll
+        for (int y = 0; y < 16; y += 4)
+          *reinterpret_cast<uint4*>(to_row + 2 * y) = make_uint4(e[y], e[y + 1], e[y + 2], e[y + 3]);
+      }
+    };
 
-        for (int j = 0; j < tiles; ++j, ++done) {
-          const int base = (it.tile0 + from + j) * K;
+    Work x = next_piece();
+    if (ok && x.tiles > 0 && i < x.row_tiles) load_q(x);
+    while (ok && x.tiles > 0) {
+      const bool active = i < x.row_tiles;
+      const int row = x.row0 + i * 128 + my_row, tok = p.by_group(row);
+      const bool live = active && tok < x.n;
+      float m = -INFINITY, l = 0.0f;
+      Work nx;
+      if (active) {
+        const float f = factors[i * 128 + my_row];
+        // slots seen, from the piece's first token on
+        int lo = 0, hi = 0x7fffffff;
+        if (live) {
+          hi = (p.causal ? min(x.len, x.len - x.n + tok + 1) : x.len) - x.tile0 * K;
+          lo = (p.window > 0 ? max(0, x.len - x.n + tok + 1 - p.window) : 0) - x.tile0 * K;
+        }
+        for (int j = 0; j < x.tiles; ++j, ++done, lo -= K, hi -= K) {
           if (!wait(G::bS + i, done)) break;
           tc_fence_after();
           float s[K];
 #pragma unroll
           for (int c2 = 0; c2 < K; c2 += 32) tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(s) + c2);
           tc_wait_ld();
-          if (!__all_sync(0xffffffffu, lo <= base && base + K <= hi)) {
+          if (__any_sync(0xffffffffu, hi < K)) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) s[k] = base + k >= lo && base + k < hi ? s[k] : -INFINITY;
+            for (int k = 0; k < K; ++k) s[k] = k < hi ? s[k] : -INFINITY;
+          }
+          if (__any_sync(0xffffffffu, lo > 0)) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) s[k] = k >= lo ? s[k] : -INFINITY;
           }
           float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int k = 4; k < K; ++k) top[k & 3] = fmaxf(top[k & 3], s[k]);
-          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+          for (int k = 4; k + 1 < K; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
+          const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
           if (j == 0) {
             m = mt;
           } else if (__any_sync(0xffffffffu, mt > m + prompt::kLag || (m == -INFINITY && mt > m))) {
@@ -554,51 +691,51 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           }
           const float off = m == -INFINITY ? 0.0f : -m;
           float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          // P goes out in two halves, so that the first one's MMAs run while
+          // the second one's exponentials are taken
 #pragma unroll
-          for (int c2 = 0; c2 < K; c2 += 64) {
-            uint32_t pk[32];
+          for (int half = 0; half < 2; ++half) {
+            constexpr int H = K / 2;
+            uint32_t pk[H / 2];
 #pragma unroll
-            for (int k = 0; k < 64; k += 2) {
-              const float x = exp2_approx(fmaf(s[c2 + k], f, off)), y = exp2_approx(fmaf(s[c2 + k + 1], f, off));
-              sum[k & 2] += x;
-              sum[(k & 2) + 1] += y;
-              pk[k / 2] = h2_as_u32(__floats2half2_rn(x, y));
+            for (int k = 0; k < H; k += 2) {
+              float &a = s[half * H + k], &b = s[half * H + k + 1];
+              fma_f32x2(a, b, f, off);
+              a = exp2_approx(a);
+              b = exp2_approx(b);
+              add_f32x2(sum[k & 2], sum[(k & 2) + 1], a, b);
+              pk[k / 2] = h2_as_u32(__floats2half2_rn(a, b));
             }
-            tmem_st_x32(ts + c2 / 2, pk);
+            if constexpr (H == 64)
+              tmem_st_x32(ts + half * H / 2, pk);
+            else
+              tmem_st_x16(ts + half * H / 2, pk);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(G::bP + 2 * half + i));   // a barrier per half: warps run apart
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tc_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(BAR(G::bP + i));
         }
+      }
+      // the next piece's queries go to shared memory now that this one's last
+      // scores are there, so that its first MMAs run during the epilogue
+      nx = next_piece();
+      if (ok && nx.tiles > 0 && i < nx.row_tiles) load_q(nx);
+      if (active) {
         if (ok) wait(G::bO + i, done - 1);
         tc_fence_after();
       }
-      // 32 columns of this thread's output row
-      const int my_tok = row / p.group;
-      const bool live = ok && active && my_tok < it.s.n;
-      const size_t out_at = live ? (size_t)(it.s.first + my_tok) * p.o_token +
-                                       (size_t)(it.head * p.group + row - my_tok * p.group) * p.o_head
+      if (!ok) break;
+      const size_t out_at = live ? (size_t)(x.first + tok) * p.o_token +
+                                       (size_t)(x.head * p.group + row - tok * p.group) * p.o_head
                                  : 0;
-      auto put32 = [&](int c2, const float* x, float scale) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          uint32_t e[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float a = x[k + 2 * y] * scale, b = x[k + 2 * y + 1] * scale;
-            if (p.bf16) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-              e[y] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-              e[y] = h2_as_u32(__floats2half2_rn(a, b));
-            }
-          }
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + out_at + c2 + k) = make_uint4(e[0], e[1], e[2], e[3]);
-        }
+      auto put_lse = [&](float mm, float ll) {
+        if (p.lse)
+          p.lse[(size_t)(x.first + tok) * p.q_heads + x.head * p.group + row - tok * p.group] =
+              ll > 0.0f ? (mm + log2f(ll)) * kLn2 : ll == 0.0f ? -INFINITY : ll;
       };
-      if (from == 0 && tiles == it.tiles) {
+      if (x.kind == kWhole) {
         if (active) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
@@ -606,41 +743,47 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
             float o[32];
             tmem_ld_x32(to + c2, reinterpret_cast<uint32_t*>(o));
             tc_wait_ld();
-            if (live) put32(c2, o, inv);
+            if (live) put32(out_at + c2, o, inv);
           }
-          if (live) store_lse(p, it.s, it.head, row, m, l);
+          if (live) put_lse(m, l);
         }
-        return true;
-      }
-      // a cut item: slot 0 if it began before this CTA's range, slot 1 if it goes on behind it
-      const int r = i * 128 + my_row;
-      float* to_part = my_part + (size_t)(from > 0 ? 0 : 1) * G::kPartFloats;
-      if (active) {
+      } else {
+        // a cut item: this CTA's part to its slot of the workspace
+        const int r = i * 128 + my_row;
+        if (active) {
+          float* to_part = p.part + ((size_t)blockIdx.x * 2 + (x.kind == kTail ? 0 : 1)) * G::kPartFloats;
 #pragma unroll 1
-        for (int c2 = 0; c2 < D; c2 += 32) {
-          uint32_t o[32];
-          tmem_ld_x32(to + c2, o);
-          tc_wait_ld();
+          for (int c2 = 0; c2 < D; c2 += 32) {
+            uint32_t o[32];
+            tmem_ld_x32(to + c2, o);
+            tc_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) to_part[(c2 + k) * G::kRows + r] = __uint_as_float(o[k]);
+            for (int k = 0; k < 32; ++k) to_part[(c2 + k) * G::kRows + r] = __uint_as_float(o[k]);
+          }
+          to_part[D * G::kRows + r] = m;
+          to_part[(D + 1) * G::kRows + r] = l;
         }
-        to_part[D * G::kRows + r] = m;
-        to_part[(D + 1) * G::kRows + r] = l;
-      }
-      __threadfence();
-      named_bar_sync(1, 128 * 2);
-      const int item0 = u - from, end = item0 + it.tiles;
-      const int c_first = (int)((((long long)item0 + 1) * ctas - 1) / T), c_last = (int)(((long long)end * ctas - 1) / T);
-      if (threadIdx.x == 32 * kSoftmaxWarp0)
-        misc[1] = atom_add_acq_rel_gpu(p.counters + c_first, 1u) == (unsigned)(c_last - c_first) ? 1u : 0u;
-      named_bar_sync(1, 128 * 2);
-      if (misc[1]) {
         __threadfence();
-        const int n = c_last - c_first + 1;
-        auto theirs = [&](int k) {
-          return p.part + ((size_t)(c_first + k) * 2 + (k == 0 ? 1 : 0)) * G::kPartFloats;
-        };
-        if (live) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(G::bParts));
+        if (warp == kSoftmaxWarp0) {
+          if (!wait(G::bParts, joins)) break;
+          if (lane == 0) {
+            __threadfence();
+            const bool last = atom_add_acq_rel_gpu(p.counters + x.c_first, 1u) == (unsigned)(x.c_last - x.c_first);
+            if (last) p.counters[x.c_first] = 0;
+            misc[1] = last;
+            mbar_arrive(BAR(G::bLast));
+          }
+          __syncwarp();
+        }
+        if (!wait(G::bLast, joins++)) break;
+        if (misc[1] && live) {
+          __threadfence();
+          const int n = x.c_last - x.c_first + 1;
+          auto theirs = [&](int k) {
+            return p.part + ((size_t)(x.c_first + k) * 2 + (k == 0 ? 1 : 0)) * G::kPartFloats;
+          };
           float mm = -INFINITY, ll = 0.0f;
           for (int k = 0; k < n; ++k) mm = fmaxf(mm, __ldcg(theirs(k) + D * G::kRows + r));
           // a piece that saw nothing has m = -inf, l = 0 and o = 0
@@ -652,23 +795,21 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll 1
           for (int c2 = 0; c2 < D; c2 += 32) {
-            float x[32];
+            float o[32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = 0.0f;
+            for (int k = 0; k < 32; ++k) o[k] = 0.0f;
             for (int y = 0; y < n; ++y) {
               const float a = share(y);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = fmaf(__ldcg(theirs(y) + (c2 + k) * G::kRows + r), a, x[k]);
+              for (int k = 0; k < 32; ++k) o[k] = fmaf(__ldcg(theirs(y) + (c2 + k) * G::kRows + r), a, o[k]);
             }
-            put32(c2, x, inv);
+            put32(out_at + c2, o, inv);
           }
-          store_lse(p, it.s, it.head, row, mm, ll);
+          put_lse(mm, ll);
         }
-        if (threadIdx.x == 32 * kSoftmaxWarp0) p.counters[c_first] = 0;
       }
-      named_bar_sync(1, 128 * 2);
-      return true;
-    });
+      x = nx;
+    }
     if (!ok) failed(16u);
   }
   if (bad) atomicOr(p.error, kErrIndex);

@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
         uint4 v[NI];
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-          const int row = row0 + k * RPI + lane / LPR, tok = row / p.group;
+          const int row = row0 + k * RPI + lane / LPR, tok = p.by_group(row);
           v[k] = make_uint4(0, 0, 0, 0);
           if (tok < it.s.n)
             v[k] = __ldg(reinterpret_cast<const uint4*>(
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
         float4* consts = reinterpret_cast<float4*>(smem + G::kConstOff) + st * 128 + w * 16;
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-          const int r = k * RPI + lane / LPR, row = row0 + r, tok = row / p.group;
+          const int r = k * RPI + lane / LPR, row = row0 + r, tok = p.by_group(row);
           float fac = fabsf(p.scale_log2);
           normalize_query8<LPR>(v[k], p.bf16, sign, fac);
           const int rr = w * 16 + r;
