@@ -654,21 +654,28 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
         for (int j = 0; j < x.tiles; ++j, ++done, lo -= K, hi -= K) {
           if (!wait(G::bS + i, done)) break;
           tc_fence_after();
-          float s[K];
+          // the row's scores in two halves, the second one first: the first
+          // one stays in registers for its exponentials, the second one is
+          // read again (a whole row of 128 would not fit the registers)
+          constexpr int H = K / 2;
+          float s[H];
+          const bool edge = __any_sync(0xffffffffu, hi < K || lo > 0);
+          auto load_half = [&](int half) {
 #pragma unroll
-          for (int c2 = 0; c2 < K; c2 += 32) tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(s) + c2);
-          tc_wait_ld();
-          if (__any_sync(0xffffffffu, hi < K)) {
+            for (int c2 = 0; c2 < H; c2 += 32) tmem_ld_x32(ts + half * H + c2, reinterpret_cast<uint32_t*>(s) + c2);
+            tc_wait_ld();
+            if (edge) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) s[k] = k < hi ? s[k] : -INFINITY;
+              for (int k = 0; k < H; ++k) s[k] = half * H + k < hi && half * H + k >= lo ? s[k] : -INFINITY;
+            }
+          };
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int half = 1; half >= 0; --half) {
+            load_half(half);
+#pragma unroll
+            for (int k = 0; k < H; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
           }
-          if (__any_sync(0xffffffffu, lo > 0)) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) s[k] = k >= lo ? s[k] : -INFINITY;
-          }
-          float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int k = 4; k + 1 < K; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
           const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
           if (j == 0) {
             m = mt;
@@ -695,11 +702,11 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           // the second one's exponentials are taken
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            constexpr int H = K / 2;
+            if (half == 1) load_half(1);
             uint32_t pk[H / 2];
 #pragma unroll
             for (int k = 0; k < H; k += 2) {
-              float &a = s[half * H + k], &b = s[half * H + k + 1];
+              float &a = s[k], &b = s[k + 1];
               fma_f32x2(a, b, f, off);
               a = exp2_approx(a);
               b = exp2_approx(b);
