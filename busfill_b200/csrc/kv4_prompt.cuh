@@ -429,12 +429,17 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
       uint32_t half = 0;             // half tiles consumed
       uint32_t done[2] = {0, 0};     // tiles of row tile i whose P was waited for
       uint32_t items[2] = {0, 0};
+      // descriptors are made once and stepped by their address field (16-byte
+      // units): built anew for every MMA, their arithmetic kept the issuing
+      // thread at 115 cycles an MMA of 65
+      const uint64_t q_desc = make_sdesc_sw128(sbase + G::kQOff), k_desc = make_sdesc_sw128(sbase + G::kSlotOff),
+                     v_desc = make_sdesc_mn_sw128(sbase + G::kSlotOff, K * 128);
       auto issue_s = [&](int i, uint32_t slot) {
-        const uint32_t a = sbase + G::kQOff + i * G::kQTileBytes, b = sbase + G::kSlotOff + slot * G::kSlotBytes;
+        const uint64_t a = q_desc + (uint32_t)(i * G::kQTileBytes / 16), b = k_desc + slot * (G::kSlotBytes / 16);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem + G::kS + i * K, make_sdesc_sw128(a + (k / 4) * 128 * 128 + (k % 4) * 32),
-                     make_sdesc_sw128(b + (k / 4) * K * 128 + (k % 4) * 32), kIdescS, k > 0);
+          mma_f16_ss(tmem + G::kS + i * K, a + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16,
+                     b + ((k / 4) * K * 128 + (k % 4) * 32) / 16, kIdescS, k > 0);
         tc_commit(BAR(G::bS + i));
       };
       auto one_piece = [&](int nr, int tiles) -> bool {
@@ -455,12 +460,12 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           if (more && !wait(G::bKvFull + ks, (half + 1) / G::kSlots)) return false;
           for (int i = 0; i < nr; ++i) {
             auto issue_o = [&](int part) {
-              const uint32_t b = sbase + G::kSlotOff + vs * G::kSlotBytes;
+              const uint64_t b = v_desc + vs * (G::kSlotBytes / 16);
 #pragma unroll
               for (int x = 0; x < K / 32; ++x) {
                 const int k = part * (K / 32) + x;
                 mma_f16_ts(tmem + G::kO + i * D, tmem + G::kS + i * K + 8 * k,
-                           make_sdesc_mn_sw128(b + k * 16 * 128, K * 128), kIdescO, j > 0 || k > 0);
+                           b + k * 16 * 128 / 16, kIdescO, j > 0 || k > 0);
               }
             };
             if (!wait(G::bP + i, done[i])) return false;
