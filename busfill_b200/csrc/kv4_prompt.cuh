@@ -659,27 +659,25 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
         for (int j = 0; j < x.tiles; ++j, ++done, lo -= K, hi -= K) {
           if (!wait(G::bS + i, done)) break;
           tc_fence_after();
-          // the row's scores in two halves, the second one first: the first
-          // one stays in registers for its exponentials, the second one is
-          // read again (a whole row of 128 would not fit the registers)
-          constexpr int H = K / 2;
-          float s[H];
+          // 32 scores at a time, once for the maximum and again for the
+          // exponentials: TMEM is quick to read (~50 cycles), the registers
+          // do not hold the row, and short loops stay in the instruction cache
           const bool edge = __any_sync(0xffffffffu, hi < K || lo > 0);
-          auto load_half = [&](int half) {
-#pragma unroll
-            for (int c2 = 0; c2 < H; c2 += 32) tmem_ld_x32(ts + half * H + c2, reinterpret_cast<uint32_t*>(s) + c2);
+          float s[32];
+          auto load_scores = [&](int c2) {
+            tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(s));
             tc_wait_ld();
             if (edge) {
 #pragma unroll
-              for (int k = 0; k < H; ++k) s[k] = half * H + k < hi && half * H + k >= lo ? s[k] : -INFINITY;
+              for (int k = 0; k < 32; ++k) s[k] = c2 + k < hi && c2 + k >= lo ? s[k] : -INFINITY;
             }
           };
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c2 = 0; c2 < K; c2 += 32) {
+            load_scores(c2);
 #pragma unroll
-          for (int half = 1; half >= 0; --half) {
-            load_half(half);
-#pragma unroll
-            for (int k = 0; k < H; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
+            for (int k = 0; k < 32; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
           }
           const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
           if (j == 0) {
@@ -705,12 +703,12 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           // P goes out in two halves, so that the first one's MMAs run while
           // the second one's exponentials are taken
+#pragma unroll 1
+          for (int c2 = 0; c2 < K; c2 += 32) {
+            load_scores(c2);
+            uint32_t pk[16];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (half == 1) load_half(1);
-            uint32_t pk[H / 2];
-#pragma unroll
-            for (int k = 0; k < H; k += 2) {
+            for (int k = 0; k < 32; k += 2) {
               float &a = s[k], &b = s[k + 1];
               fma_f32x2(a, b, f, off);
               a = exp2_approx(a);
@@ -718,14 +716,14 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
               add_f32x2(sum[k & 2], sum[(k & 2) + 1], a, b);
               pk[k / 2] = h2_as_u32(__floats2half2_rn(a, b));
             }
-            if constexpr (H == 64)
-              tmem_st_x32(ts + half * H / 2, pk);
-            else
-              tmem_st_x16(ts + half * H / 2, pk);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(BAR(G::bP + 2 * half + i));   // a barrier per half: warps run apart
+            tmem_st_x16(ts + c2 / 2, pk);
+            if ((c2 + 32) % (K / 2) == 0) {
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              // a barrier per half: warps run apart
+              if (lane == 0) mbar_arrive(BAR(G::bP + (c2 < K / 2 ? 0 : 2) + i));
+            }
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
