@@ -659,25 +659,29 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
         for (int j = 0; j < x.tiles; ++j, ++done, lo -= K, hi -= K) {
           if (!wait(G::bS + i, done)) break;
           tc_fence_after();
-          // 32 scores at a time, once for the maximum and again for the
+          // Scores 32 at a time, once for the maximum and again for the
           // exponentials: TMEM is quick to read (~50 cycles), the registers
-          // do not hold the row, and short loops stay in the instruction cache
+          // do not hold the row, and short loops stay in the instruction
+          // cache. The next 32 are on their way while 32 are worked on.
           const bool edge = __any_sync(0xffffffffu, hi < K || lo > 0);
-          float s[32];
-          auto load_scores = [&](int c2) {
-            tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(s));
-            tc_wait_ld();
-            if (edge) {
+          float s[2][32];
+          auto load_scores = [&](int c2, float* x) { tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(x)); };
+          auto mask_scores = [&](int c2, float* x) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) s[k] = c2 + k < hi && c2 + k >= lo ? s[k] : -INFINITY;
-            }
+            for (int k = 0; k < 32; ++k) x[k] = c2 + k < hi && c2 + k >= lo ? x[k] : -INFINITY;
           };
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-          for (int c2 = 0; c2 < K; c2 += 32) {
-            load_scores(c2);
+          for (int c2 = 0; c2 < K; c2 += 64) {
+            load_scores(c2, s[0]);
+            load_scores(c2 + 32, s[1]);
+            tc_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
+            for (int x = 0; x < 2; ++x) {
+              if (edge) mask_scores(c2 + 32 * x, s[x]);
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[x][k], s[x][k + 1]);
+            }
           }
           const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
           if (j == 0) {
@@ -699,30 +703,37 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
               tmem_st_x32(to + c2, o);
             }
           }
+          load_scores(0, s[0]);
           const float off = m == -INFINITY ? 0.0f : -m;
           float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           // P goes out in two halves, so that the first one's MMAs run while
           // the second one's exponentials are taken
 #pragma unroll 1
-          for (int c2 = 0; c2 < K; c2 += 32) {
-            load_scores(c2);
-            uint32_t pk[16];
+          for (int c0 = 0; c0 < K; c0 += 64) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float &a = s[k], &b = s[k + 1];
-              fma_f32x2(a, b, f, off);
-              a = exp2_approx(a);
-              b = exp2_approx(b);
-              add_f32x2(sum[k & 2], sum[(k & 2) + 1], a, b);
-              pk[k / 2] = h2_as_u32(__floats2half2_rn(a, b));
-            }
-            tmem_st_x16(ts + c2 / 2, pk);
-            if ((c2 + 32) % (K / 2) == 0) {
-              tc_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              // a barrier per half: warps run apart
-              if (lane == 0) mbar_arrive(BAR(G::bP + (c2 < K / 2 ? 0 : 2) + i));
+            for (int x = 0; x < 2; ++x) {
+              const int c2 = c0 + 32 * x;
+              tc_wait_ld();
+              if (c2 + 32 < K) load_scores(c2 + 32, s[x ^ 1]);
+              if (edge) mask_scores(c2, s[x]);
+              uint32_t pk[16];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                float &a = s[x][k], &b = s[x][k + 1];
+                fma_f32x2(a, b, f, off);
+                a = exp2_approx(a);
+                b = exp2_approx(b);
+                add_f32x2(sum[k & 2], sum[(k & 2) + 1], a, b);
+                pk[k / 2] = h2_as_u32(__floats2half2_rn(a, b));
+              }
+              tmem_st_x16(ts + c2 / 2, pk);
+              if ((c2 + 32) % (K / 2) == 0) {
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                // a barrier per half: warps run apart
+                if (lane == 0) mbar_arrive(BAR(G::bP + (c2 < K / 2 ? 0 : 2) + i));
+              }
             }
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
