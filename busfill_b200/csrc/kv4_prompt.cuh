@@ -14,8 +14,9 @@
 // The two row tiles i = 0, 1 take turns: while one's S is in the softmax
 // threads, the tensor pipe works on the other. Codes are dequantized once per
 // tile and CTA into a ring of fp16 operands, exactly ((c - 8) d has at most 11
-// significant bits). O is rescaled only when a row's maximum has grown by more
-// than 2^8 since the last time (p stays below 2^8, far inside fp16).
+// significant bits). Exponentials are taken against a reference that is a
+// maximum of earlier scores; O is rescaled only when a score lies more than
+// 2^14 above it.
 //
 // Warps: 0 copies raw pages into a ring (bulk copies); 1 issues the MMAs and
 // owns TMEM; 2 hands out the work; 4-7 and 8-11 softmax of row tile 0 and 1, thread = row; 12-15
@@ -136,7 +137,7 @@ namespace prompt {
 
 constexpr int kThreads = 512;
 constexpr int kSoftmaxWarp0 = 4, kDequantWarp0 = 12;
-constexpr float kLag = 8.0f;   // log2 growth of a row's maximum that O is not rescaled for (p < 2^8)
+constexpr float kOver = 14.0f;   // how far, in log2, a score may lie above the row's reference (p < 2^14 in fp16)
 
 template <int D>
 struct Geo {
@@ -160,7 +161,7 @@ struct Geo {
   static constexpr int kBarOff = kFacOff + kRows * 4;
   static constexpr int kDescs = 4;                         // descriptors in flight
   static constexpr int bRawFull = 0, bRawEmpty = bRawFull + kRawStages, bKvFull = bRawEmpty + kRawStages,
-                       bKvEmpty = bKvFull + kSlots, bS = bKvEmpty + kSlots, bP = bS + 2, bO = bP + 4, bQ = bO + 2,
+                       bKvEmpty = bKvFull + kSlots, bS = bKvEmpty + kSlots, bP = bS + 2, bO = bP + 4, bQ = bO + 4,
                        bDescFull = bQ + 2, bDescEmpty = bDescFull + kDescs, bParts = bDescEmpty + kDescs,
                        bLast = bParts + 1, bFinal = bLast + 1, kBars = bFinal + 1;
   static constexpr int kMiscOff = kBarOff + kBars * 8;
@@ -470,13 +471,16 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
             };
             if (!wait(G::bP + i, done[i])) return false;
             tc_fence_after();
-            if (elect_one()) issue_o(0);
+            if (elect_one()) {
+              issue_o(0);
+              tc_commit(BAR(G::bO + i));
+            }
             __syncwarp();
             if (!wait(G::bP + 2 + i, done[i]++)) return false;
             tc_fence_after();
             if (elect_one()) {
               issue_o(1);
-              tc_commit(BAR(G::bO + i));
+              tc_commit(BAR(G::bO + 2 + i));
               if (more) issue_s(i, ks);
               if (i + 1 == nr) {
                 tc_commit(BAR(G::bKvEmpty + vs));
@@ -659,84 +663,76 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
         for (int j = 0; j < x.tiles; ++j, ++done, lo -= K, hi -= K) {
           if (!wait(G::bS + i, done)) break;
           tc_fence_after();
-          // Scores 32 at a time, once for the maximum and again for the
-          // exponentials: TMEM is quick to read (~50 cycles), the registers
-          // do not hold the row, and short loops stay in the instruction
-          // cache. The next 32 are on their way while 32 are worked on.
           const bool edge = __any_sync(0xffffffffu, hi < K || lo > 0);
-          float s[2][32];
-          auto load_scores = [&](int c2, float* x) { tmem_ld_x32(ts + c2, reinterpret_cast<uint32_t*>(x)); };
-          auto mask_scores = [&](int c2, float* x) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = c2 + k < hi && c2 + k >= lo ? x[k] : -INFINITY;
-          };
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          // Half a row at a time: P goes out in two halves, so that the first
+          // one's MMAs run while the second one's exponentials are taken. The
+          // exponentials are taken against the maximum known so far, while
+          // the half's own is found beside them: only where that is more than
+          // 2^kOver above (at the start, and then rarely) are they taken
+          // again. Short loops stay in the instruction cache.
 #pragma unroll 1
-          for (int c2 = 0; c2 < K; c2 += 64) {
-            load_scores(c2, s[0]);
-            load_scores(c2 + 32, s[1]);
-            tc_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (edge) mask_scores(c2 + 32 * x, s[x]);
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[x][k], s[x][k + 1]);
-            }
-          }
-          const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
-          if (j == 0) {
-            m = mt;
-          } else if (__any_sync(0xffffffffu, mt > m + prompt::kLag || (m == -INFINITY && mt > m))) {
-            const float m2 = fmaxf(m, mt);
-            const float a = m == m2 ? 1.0f : exp2_approx(m - m2);
-            m = m2;
-            l *= a;
-            if (!wait(G::bO + i, done - 1)) break;
-            tc_fence_after();
-#pragma unroll
-            for (int c2 = 0; c2 < D; c2 += 32) {
-              uint32_t o[32];
-              tmem_ld_x32(to + c2, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
-              tmem_st_x32(to + c2, o);
-            }
-          }
-          load_scores(0, s[0]);
-          const float off = m == -INFINITY ? 0.0f : -m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          // P goes out in two halves, so that the first one's MMAs run while
-          // the second one's exponentials are taken
+          for (int h = 0; ok && h < 2; ++h) {
+            constexpr int H = K / 2;
+            uint32_t pk[H / 2];
+            float sum[4];
 #pragma unroll 1
-          for (int c0 = 0; c0 < K; c0 += 64) {
+            for (bool again = false;; again = true) {
+              float x[H];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int c2 = c0 + 32 * x;
+              for (int c2 = 0; c2 < H; c2 += 32)
+                tmem_ld_x32(ts + h * H + c2, reinterpret_cast<uint32_t*>(x) + c2);
               tc_wait_ld();
-              if (c2 + 32 < K) load_scores(c2 + 32, s[x ^ 1]);
-              if (edge) mask_scores(c2, s[x]);
-              uint32_t pk[16];
+              if (edge) {
+                const int first = lo - h * H, last = hi - h * H;
 #pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                float &a = s[x][k], &b = s[x][k + 1];
+                for (int k = 0; k < H; ++k) x[k] = k < last && k >= first ? x[k] : -INFINITY;
+              }
+              const float off = m == -INFINITY ? 0.0f : -m;
+              float top[4] = {x[0], x[1], x[2], x[3]};
+              sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+#pragma unroll
+              for (int k = 0; k < H; k += 2) {
+                float a = x[k], b = x[k + 1];
+                if (k >= 4) top[k / 2 & 3] = max3(top[k / 2 & 3], a, b);
                 fma_f32x2(a, b, f, off);
                 a = exp2_approx(a);
                 b = exp2_approx(b);
                 add_f32x2(sum[k & 2], sum[(k & 2) + 1], a, b);
                 pk[k / 2] = h2_as_u32(__floats2half2_rn(a, b));
               }
-              tmem_st_x16(ts + c2 / 2, pk);
-              if ((c2 + 32) % (K / 2) == 0) {
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                // a barrier per half: warps run apart
-                if (lane == 0) mbar_arrive(BAR(G::bP + (c2 < K / 2 ? 0 : 2) + i));
+              const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
+              if (again || !__any_sync(0xffffffffu, mt > m + kOver || (m == -INFINITY && mt > m))) break;
+              const float m2 = fmaxf(m, mt);
+              const float a = m == m2 ? 1.0f : exp2_approx(m - m2);
+              m = m2;
+              l *= a;
+              if (j == 0 && h == 0) continue;
+              // O so far: the MMAs of the half before this one. (Barriers per
+              // half: the one before that is done, and its completion is not
+              // mistaken for this one's.)
+              if (!wait(G::bO + 2 * (h ^ 1) + i, h ? done : done - 1)) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c2 = 0; c2 < D; c2 += 32) {
+                uint32_t o[32];
+                tmem_ld_x32(to + c2, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
+                tmem_st_x32(to + c2, o);
               }
             }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if constexpr (H == 64)
+              tmem_st_x32(ts + h * H / 2, pk);
+            else
+              tmem_st_x16(ts + h * H / 2, pk);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            // a barrier per half: warps run apart
+            if (lane == 0) mbar_arrive(BAR(G::bP + 2 * h + i));
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
       }
       // the next piece's queries go to shared memory now that this one's last
@@ -744,7 +740,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
       nx = next_piece();
       if (ok && nx.tiles > 0 && i < nx.row_tiles) load_q(nx);
       if (active) {
-        if (ok) wait(G::bO + i, done - 1);
+        if (ok) wait(G::bO + 2 + i, done - 1);
         tc_fence_after();
       }
       if (!ok) break;
