@@ -221,7 +221,7 @@ int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_start, int token
   host::Context ctx;
   st = host::context(s, &ctx);
   if (st != BUSFILL_OK || tokens == 0) return st;
-  ReadParams p{view_of(cache), q_start, tokens, (2 * cache->heads * (cache->head_dim / 8) + 31) / 32,
+  ReadParams p{view_of(cache), q_start, tokens, (2 * cache->heads + 7) / 8,
                reinterpret_cast<__half*>(k), reinterpret_cast<__half*>(v), ctx.error};
   const long long blocks = ((long long)tokens * p.chunks + 7) / 8;
   if (blocks > kMaxGrid / 8) return BUSFILL_ERR_SHAPE;

@@ -211,23 +211,6 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s,
   }
 }
 
-// A vector of a lane's 32-bit words of one row: NB words (keys), NB / 2 (values).
-template <int N>
-__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t* w) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
-      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-    }
-  }
-}
-
 // Scores of 16 tokens (tokens 16 mt .. of the page) for NT row tiles, times
 // nothing: s[nt][0..3] are rows (token tile_perm(lane / 4), and + 8) x column
 // pair. To log2 scores: * factor.
@@ -237,10 +220,10 @@ __device__ __forceinline__ void scores_16(const uint8_t* page, int mt, int lane,
   constexpr int NB = F::kBlocks;
   const int j = lane & 3, t = 16 * mt + tile_perm(lane >> 2);
   uint32_t w0[NB], w1[NB], sc0[NB / 2], sc1[NB / 2];
-  lds_words<NB>(page + t * F::kRow + j * 4 * NB, w0);
-  lds_words<NB>(page + (t + 8) * F::kRow + j * 4 * NB, w1);
-  lds_words<NB / 2>(page + F::kKeyScale + t * 2 * NB, sc0);
-  lds_words<NB / 2>(page + F::kKeyScale + (t + 8) * 2 * NB, sc1);
+  load_words<NB>(page + t * F::kRow + j * 4 * NB, w0);
+  load_words<NB>(page + (t + 8) * F::kRow + j * 4 * NB, w1);
+  load_words<NB / 2>(page + F::kKeyScale + t * 2 * NB, sc0);
+  load_words<NB / 2>(page + F::kKeyScale + (t + 8) * 2 * NB, sc1);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
@@ -366,10 +349,10 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
     }
     const int ta = 16 * mt + tile_perm(2 * j), tb = 16 * mt + tile_perm(2 * j + 1);
     uint32_t w[4][NB / 2];
-    lds_words<NB / 2>(vals + ta * F::kRow + (c ^ value_swizzle<D>(ta)) * 2 * NB, w[0]);
-    lds_words<NB / 2>(vals + tb * F::kRow + (c ^ value_swizzle<D>(tb)) * 2 * NB, w[1]);
-    lds_words<NB / 2>(vals + (ta + 8) * F::kRow + (c ^ value_swizzle<D>(ta + 8)) * 2 * NB, w[2]);
-    lds_words<NB / 2>(vals + (tb + 8) * F::kRow + (c ^ value_swizzle<D>(tb + 8)) * 2 * NB, w[3]);
+    load_words<NB / 2>(vals + ta * F::kRow + (c ^ value_swizzle<D>(ta)) * 2 * NB, w[0]);
+    load_words<NB / 2>(vals + tb * F::kRow + (c ^ value_swizzle<D>(tb)) * 2 * NB, w[1]);
+    load_words<NB / 2>(vals + (ta + 8) * F::kRow + (c ^ value_swizzle<D>(ta + 8)) * 2 * NB, w[2]);
+    load_words<NB / 2>(vals + (tb + 8) * F::kRow + (c ^ value_swizzle<D>(tb + 8)) * 2 * NB, w[3]);
     // slots behind the sequence hold anything, non-finite scales too
     const int left = len - base - 16 * mt;
 #pragma unroll

@@ -137,6 +137,23 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float* x) {
   for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
 }
 
+// N consecutive 32-bit words, aligned to their size (16 bytes at most), by the widest loads.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  }
+}
+
 // Two fp16 values (c - 8) d of the codes that `bits` holds at bits 4-7 of its
 // halves: 0x5400 | code << 4 is the fp16 number 64 + c, and with 72 d exact
 // (d has 7 significant bits) one fused multiply-add gives the exact product.

@@ -529,14 +529,14 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           __half2 d[NB];
           if (half == 0) {
             uint32_t sc[NB / 2];
-            lds_words<NB>(pg + t * F::kRow + j * 4 * NB, x);
-            lds_words<NB / 2>(pg + F::kKeyScale + t * 2 * NB, sc);
+            load_words<NB>(pg + t * F::kRow + j * 4 * NB, x);
+            load_words<NB / 2>(pg + F::kKeyScale + t * 2 * NB, sc);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
               d[b] = b & 1 ? __high2half2(u32_as_h2(sc[b / 2])) : __low2half2(u32_as_h2(sc[b / 2]));
           } else {
             uint32_t y[NB];   // value words 2j and 2j + 1 of all blocks
-            lds_words<NB>(pg + t * F::kRow + ((2 * j) ^ value_swizzle<D>(t)) * 2 * NB, y);
+            load_words<NB>(pg + t * F::kRow + ((2 * j) ^ value_swizzle<D>(t)) * 2 * NB, y);
             const bool live = base + tok < len;   // slots behind the sequence hold anything
 #pragma unroll
             for (int b = 0; b < NB; ++b) {

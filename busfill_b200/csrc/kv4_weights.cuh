@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
         if (base + tok < it.s.len) {
           const int pg = page_of(p.c, p.c.table, p.c.table_cols, it.b, (base + tok) / kPage, bad);
           const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + it.head) * F::kPageBytes;
-          lds_words<NB>(src + t * F::kRow + j * 4 * NB, x);
-          lds_words<NB / 2>(src + F::kKeyScale + t * 2 * NB, sc);
+          load_words<NB>(src + t * F::kRow + j * 4 * NB, x);
+          load_words<NB / 2>(src + F::kKeyScale + t * 2 * NB, sc);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
