@@ -199,13 +199,18 @@ int busfill_kv4_append(const busfill_kv4* cache, const busfill_kv4_rows* r, void
   p.tokens = r->tokens;
   p.vec = aligned(r->k, 16) && aligned(r->v, 16) && (r->k_token | r->k_head | r->v_token | r->v_head) % 8 == 0;
   p.error = ctx.error;
-  p.chunks = (2 * cache->heads * (cache->head_dim / 8) + 31) / 32;
+  // four groups a lane where that leaves every scheduler two warps
+  const int groups = (2 * cache->heads * (cache->head_dim / 8) + 31) / 32;
+  const bool four = (long long)p.tokens * groups >= (long long)ctx.sms * 32;
+  p.chunks = four ? (groups + 3) / 4 : groups;
   const long long blocks = ((long long)p.tokens * p.chunks + 7) / 8;
   if (blocks > kMaxGrid / 8) return BUSFILL_ERR_SHAPE;   // the kernel counts warps in an int
   void* args[] = {&p};
   return by_dim(cache->head_dim, [&](auto d) {
-    const void* kern = r->dtype == BUSFILL_TYPE_F16 ? (const void*)append_kernel<d(), __half>
-                                                    : (const void*)append_kernel<d(), __nv_bfloat16>;
+    const void* kern = r->dtype == BUSFILL_TYPE_F16
+                           ? (four ? (const void*)append_kernel<d(), __half, 4> : (const void*)append_kernel<d(), __half, 1>)
+                           : (four ? (const void*)append_kernel<d(), __nv_bfloat16, 4>
+                                   : (const void*)append_kernel<d(), __nv_bfloat16, 1>);
     return host::launch(kern, dim3((unsigned)blocks), dim3(256), 0, s, args);
   });
 }
@@ -301,17 +306,22 @@ int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, v
                 e->out_table,   e->out_cols, e->keep,       e->recent,       in_place, ctx.error};
   const int rows = cache->batch * cache->heads;
   void* args[] = {&p};
-  st = host::launch((const void*)evict_select_kernel, dim3(rows), dim3(kSelectThreads), 0, s, args);
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  if (!raise_smem(evict_select_kernel, kSelectBytes, ctx.dev, once, err)) return BUSFILL_ERR_LAUNCH;
+  st = host::launch((const void*)evict_select_kernel, dim3(rows), dim3(kSelectThreads), kSelectBytes, s, args);
   if (st != BUSFILL_OK) return st;
-  // CTAs of a row: in place one; else enough to fill the device, as far as there are tokens
-  int per = 1;
-  if (!in_place)
-    per = std::max(1, std::min((e->keep + kMoveThreads / 8 * kMoveRows - 1) / (kMoveThreads / 8 * kMoveRows),
-                               (ctx.sms * 4 + rows - 1) / rows));
-  void* margs[] = {&p, &per};
   return by_dim(cache->head_dim, [&](auto d) {
-    return host::launch((const void*)evict_move_kernel<d()>, dim3((unsigned)(rows * per)), dim3(kMoveThreads), 0, s,
-                        margs);
+    int per = 1;
+    void* margs[] = {&p, &per};
+    if (in_place)
+      return host::launch((const void*)evict_move_kernel<d(), true>, dim3((unsigned)rows),
+                          dim3(MoveGeo<d(), true>::kThreads), 0, s, margs);
+    // enough CTAs to fill the device, as far as there are tokens
+    using G = MoveGeo<d(), false>;
+    per = std::max(1, std::min((e->keep + G::kTokens - 1) / G::kTokens, (ctx.sms * 8 + rows - 1) / rows));
+    return host::launch((const void*)evict_move_kernel<d(), false>, dim3((unsigned)(rows * per)), dim3(G::kThreads), 0,
+                        s, margs);
   });
 }
 

@@ -126,7 +126,7 @@ struct AppendParams {
   const int* q_start;
   long long k_token, k_head, v_token, v_head;
   int tokens;
-  int chunks;      // warps of a token: ceil(2 * heads * D / 8 / 32)
+  int chunks;      // warps of a token
   int vec;         // 16-byte loads
   unsigned* error;
 };
@@ -163,8 +163,7 @@ __device__ __forceinline__ uint32_t quantize8(float* x, int j, __half& scale) {
   // floor(x / d + 8.5), exactly: x has at most 11 significant bits and d 7, so
   // x / d + 8.5 is a whole number or at least 2^-14 away from one. The product
   // with the reciprocal is off by less than 2^-19; 2^-16 more lifts the ties
-  // over their boundary and nothing else. (The IEEE division instead: 39 us
-  // for 16000 tokens x 8 heads of 128, against 15.)
+  // over their boundary and nothing else.
   const float inv = copysignf(__frcp_rn(fabsf(d)), d);
   uint32_t w = 0;
 #pragma unroll
@@ -176,16 +175,39 @@ __device__ __forceinline__ uint32_t quantize8(float* x, int j, __half& scale) {
   return w;
 }
 
-// One lane takes 8 channels of one key or value row: word j of block b.
-template <int D, typename T>
+// One lane takes 8 channels of a key or value row (word j of block b), GROUPS
+// times. Its elements are on their way before the token's place in the cache
+// is looked up, a chain of four small loads that would otherwise set the time
+// (16000 tokens x 8 heads of 128: 33 us, 13 with both).
+template <int D, typename T, int GROUPS>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   using F = Fmt<D>;
+  constexpr int kItems = D / 8;
   pdl_wait_prerequisites();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int warp = (int)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int token = warp / p.chunks;
   if (token >= p.tokens) return;
+  const int item0 = (warp - token * p.chunks) * (32 * GROUPS) + lane;
+  alignas(16) T e[GROUPS][8];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int item = item0 + 32 * g, row = item / kItems, piece = item - row * kItems;   // row: 2 * head + (value)
+    const int head = row >> 1;
+    if (head < p.c.heads) {
+      const T* src = row & 1 ? static_cast<const T*>(p.v) + token * p.v_token + head * p.v_head
+                             : static_cast<const T*>(p.k) + token * p.k_token + head * p.k_head;
+      if (p.vec) {
+        *reinterpret_cast<uint4*>(e[g]) = __ldg(reinterpret_cast<const uint4*>(src + piece * 8));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[g][i] = src[piece * 8 + i];
+      }
+    } else {
+      *reinterpret_cast<uint4*>(e[g]) = make_uint4(0, 0, 0, 0);
+    }
+  }
   const int b = sequence_of(p.q_start, p.c.batch, token, lane);
   if (b < 0) return;
   bool bad = false;
@@ -203,35 +225,28 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
     return;
   }
   if (!inside) return;
-  constexpr int kItems = D / 8;
-  const int item = (warp - token * p.chunks) * 32 + lane;
-  const int row = item / kItems, piece = item - row * kItems;   // row: 2 * head + (value)
-  const int head = row >> 1, isv = row & 1;
-  const bool live = head < p.c.heads;
-  const int blk = piece >> 2, j = piece & 3;
-  float x[8];
+  const int t = slot & (kPage - 1), sw = value_swizzle<D>(t);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  if (live) {
-    const T* src = isv ? static_cast<const T*>(p.v) + token * p.v_token + head * p.v_head
-                       : static_cast<const T*>(p.k) + token * p.k_token + head * p.k_head;
-    load8(src + piece * 8, p.vec, x);
-  }
-  __half d;
-  const uint32_t w = quantize8(x, j, d);
-  if (!live) return;
-  const int t = slot & (kPage - 1);
-  uint8_t* pg = p.c.pages + ((size_t)page * p.c.heads + head) * F::kPageBytes;
-  if (!isv) {
-    *reinterpret_cast<uint32_t*>(pg + t * F::kRow + (j * F::kBlocks + blk) * 4) = w;
-    if (j == 0) *reinterpret_cast<__half*>(pg + F::kKeyScale + (t * F::kBlocks + blk) * 2) = d;
-  } else {
-    // the low half of the key-order word is the value word 2j, the high half 2j + 1
-    const int sw = value_swizzle<D>(t);
-    uint8_t* r = pg + F::kValue + t * F::kRow;
-    *reinterpret_cast<uint16_t*>(r + (((2 * j) ^ sw) * F::kBlocks + blk) * 2) = (uint16_t)w;
-    *reinterpret_cast<uint16_t*>(r + (((2 * j + 1) ^ sw) * F::kBlocks + blk) * 2) = (uint16_t)(w >> 16);
-    if (j == 0) *reinterpret_cast<__half*>(pg + F::kValueScale + (blk * kPage + tile_perm(t)) * 2) = d;
+  for (int g = 0; g < GROUPS; ++g) {
+    const int item = item0 + 32 * g, row = item / kItems, piece = item - row * kItems;
+    const int head = row >> 1, blk = piece >> 2, j = piece & 3;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = to_float(e[g][k]);
+    __half d;
+    const uint32_t w = quantize8(x, j, d);
+    if (head >= p.c.heads) continue;
+    uint8_t* pg = p.c.pages + ((size_t)page * p.c.heads + head) * F::kPageBytes;
+    if (!(row & 1)) {
+      *reinterpret_cast<uint32_t*>(pg + t * F::kRow + (j * F::kBlocks + blk) * 4) = w;
+      if (j == 0) *reinterpret_cast<__half*>(pg + F::kKeyScale + (t * F::kBlocks + blk) * 2) = d;
+    } else {
+      // the low half of the key-order word is the value word 2j, the high half 2j + 1
+      uint8_t* r = pg + F::kValue + t * F::kRow;
+      *reinterpret_cast<uint16_t*>(r + (((2 * j) ^ sw) * F::kBlocks + blk) * 2) = (uint16_t)w;
+      *reinterpret_cast<uint16_t*>(r + (((2 * j + 1) ^ sw) * F::kBlocks + blk) * 2) = (uint16_t)(w >> 16);
+      if (j == 0) *reinterpret_cast<__half*>(pg + F::kValueScale + (blk * kPage + tile_perm(t)) * 2) = d;
+    }
   }
 }
 
@@ -331,19 +346,49 @@ __device__ __forceinline__ unsigned weight_key(float w) {
 }
 
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectKeys = 40960;   // weights that are held in shared memory at a time
+constexpr int kSelectBytes = kSelectKeys * 4 + 2048 * 4;
+
+// Exclusive sum of x over the CTA's threads; total of all in `total`.
+__device__ __forceinline__ unsigned block_sum(unsigned x, unsigned* sums, unsigned& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned run = x;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, run, m);
+    if (lane >= m) run += y;
+  }
+  __syncthreads();   // `sums` may still be read from the last time
+  if (lane == 31) sums[warp] = run;
+  __syncthreads();
+  unsigned before = 0;
+  total = 0;
+#pragma unroll 8
+  for (int w = 0; w < kSelectThreads / 32; ++w) {
+    const unsigned y = sums[w];
+    before += w < warp ? y : 0;
+    total += y;
+  }
+  return before + run - x;
+}
 
 // Which tokens stay: one CTA per sequence and head. The (keep - recent)-th
-// largest key is found digit by digit (8 bits a pass over the weights, a
-// shared histogram), then one more pass writes the kept slots in order; among
-// the tokens with exactly that key the lower slots win.
+// largest key is found digit by digit (11, 11 and 10 bits, a shared histogram
+// each: wide digits spread weights of like size over many counters); then one
+// ordered pass writes the kept slots, every thread a run of them. Among the
+// tokens with exactly that key the lower slots win. The weights sit in shared
+// memory; of longer sequences the histograms read them from global memory and
+// the ordered pass goes part by part.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned sums[32], totals[2];
+  extern __shared__ unsigned select_smem[];
+  float* held = reinterpret_cast<float*>(select_smem);
+  unsigned* hist = select_smem + kSelectKeys;
+  __shared__ unsigned sums[32];
   __shared__ unsigned pick[2];   // digit, keys still to find
   pdl_wait_prerequisites();
   pdl_launch_dependents();
   const int b = blockIdx.x / p.c.heads, h = blockIdx.x - b * p.c.heads;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   bool bad = false;
   const int len = cached(p.c, b, bad);
   if (bad && tid == 0) atomicOr(p.error, kErrIndex);
@@ -353,106 +398,85 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   const float* w = p.weights + row * p.weights_cols;
   float* wo = p.weights_out + row * p.weights_cols;
   int* index = p.index + row * p.keep;
+  const bool fits = len <= kSelectKeys;
+  if (fits) {
+#pragma unroll 4
+    for (int i = tid; i < len; i += kSelectThreads) held[i] = w[i];
+  }
+  const float* keys = fits ? held : w;
 
   unsigned edge = 0, mask = 0, left = (unsigned)need;
   if (need > 0 && need < old) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    for (int shift = 21;; shift = shift > 10 ? 10 : 0) {
+      const int bins = shift ? 2048 : 1024;
+      hist[tid] = hist[tid + 1024] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int i = tid; i < old; i += kSelectThreads) {
-        const unsigned key = weight_key(w[i]);
-        if ((key & mask) == edge) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+        const unsigned key = weight_key(keys[i]);
+        if ((key & mask) == edge) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
       }
       __syncthreads();
-      if (warp == 0) {   // the digit where the count from above reaches `left`
-        unsigned mine = 0;
-        for (int k = 0; k < 8; ++k) mine += hist[255 - (8 * lane + k)];
-        unsigned run = mine;
-        for (int m = 1; m < 32; m <<= 1) {
-          const unsigned y = __shfl_up_sync(0xffffffffu, run, m);
-          if (lane >= m) run += y;
-        }
-        unsigned above = run - mine;
-        if (above < left && run >= left) {
-          for (int k = 0; k < 8; ++k) {
-            const unsigned n = hist[255 - (8 * lane + k)];
-            if (above + n >= left) {
-              pick[0] = 255u - (8 * lane + k);
-              pick[1] = left - above;
-              break;
-            }
-            above += n;
-          }
-        }
+      // the digit where the count from above reaches `left`: two digits a thread
+      const int top = bins - 1 - 2 * tid;
+      const unsigned n0 = top > 0 ? hist[top] : 0, n1 = top > 0 ? hist[top - 1] : 0;
+      unsigned total;
+      const unsigned above = block_sum(n0 + n1, sums, total);
+      if (above < left && above + n0 + n1 >= left) {
+        const bool second = above + n0 < left;
+        pick[0] = (unsigned)(second ? top - 1 : top);
+        pick[1] = left - above - (second ? n0 : 0);
       }
       __syncthreads();
       edge |= pick[0] << shift;
-      mask |= 255u << shift;
+      mask |= (unsigned)(bins - 1) << shift;
       left = pick[1];
-      __syncthreads();
+      if (shift == 0) break;
     }
   }
-  // ordered pass: `left` tokens of key == edge and all of key > edge stay
-  // (need == old: everything stays; need == 0: nothing)
-  unsigned at = 0, ties = 0;
+  // `left` tokens of key == edge and all of key > edge stay (need == old:
+  // everything stays; need == 0: nothing); what is written has been read
   const bool all = need >= old;
-  for (int i0 = 0; i0 < len; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    float x = 0.0f;
-    bool above = false, tie = false;
-    if (i < len) {
-      x = w[i];
-      if (i >= old || all) {
-        above = true;
-      } else if (need > 0) {
-        const unsigned key = weight_key(x);
-        above = key > edge;
-        tie = key == edge;
+  unsigned at = 0, ties = 0;   // kept, and ties met, in earlier parts
+  for (int base = 0; base < len; base += kSelectKeys) {
+    const int n = min(kSelectKeys, len - base);
+    __syncthreads();
+    if (!fits)
+      for (int i = tid; i < n; i += kSelectThreads) held[i] = w[base + i];
+    __syncthreads();
+    // an odd run of slots per thread: the threads of a warp read different banks
+    const int run = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
+    const int i0 = min(n, tid * run), i1 = min(n, i0 + run);
+    auto kind = [&](int i) -> int {   // 0 goes, 1 stays, 2 tie
+      if (base + i >= old || all) return 1;
+      if (need == 0) return 0;
+      const unsigned key = weight_key(held[i]);
+      return key > edge ? 1 : key == edge ? 2 : 0;
+    };
+    unsigned mine = 0, stays = 0;   // ties, kept above them
+    for (int i = i0; i < i1; ++i) {
+      const int k = kind(i);
+      mine += k == 2;
+      stays += k == 1;
+    }
+    unsigned all_ties, all_kept;
+    unsigned rank = ties + block_sum(mine, sums, all_ties);
+    // ties of rank < left stay
+    const unsigned tied = rank < left ? min(mine, left - rank) : 0;
+    unsigned to = at + block_sum(stays + tied, sums, all_kept);
+    for (int i = i0; i < i1; ++i) {
+      const int k = kind(i);
+      if (k == 1 || (k == 2 && rank++ < left)) {
+        index[to] = base + i;
+        wo[to] = held[i];
+        ++to;
       }
     }
-    // rank of the ties first, then of the kept
-    unsigned bal = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) sums[warp] = __popc(bal);
-    __syncthreads();
-    if (warp == 0) {
-      const unsigned mine = sums[lane];
-      unsigned run = mine;
-      for (int m = 1; m < 32; m <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, run, m);
-        if (lane >= m) run += y;
-      }
-      sums[lane] = run - mine;
-      if (lane == 31) totals[0] = run;
-    }
-    __syncthreads();
-    const unsigned rank = ties + sums[warp] + __popc(bal & ((1u << lane) - 1));
-    const bool stay = above || (tie && rank < left);
-    ties += totals[0];
-    __syncthreads();
-    bal = __ballot_sync(0xffffffffu, stay);
-    if (lane == 0) sums[warp] = __popc(bal);
-    __syncthreads();
-    if (warp == 0) {
-      const unsigned mine = sums[lane];
-      unsigned run = mine;
-      for (int m = 1; m < 32; m <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, run, m);
-        if (lane >= m) run += y;
-      }
-      sums[lane] = run - mine;
-      if (lane == 31) totals[1] = run;
-    }
-    __syncthreads();
-    // kept tokens move down: what is written here has been read by now
-    if (stay) {
-      const unsigned to = at + sums[warp] + __popc(bal & ((1u << lane) - 1));
-      index[to] = i;
-      wo[to] = x;
-    }
-    at += totals[1];
-    __syncthreads();
+    ties += all_ties;
+    at += all_kept;
   }
   for (int i = keep + tid; i < p.keep; i += kSelectThreads) index[i] = -1;
+  __syncthreads();
   for (long long i = keep + tid; i < p.weights_cols; i += kSelectThreads) wo[i] = 0.0f;
   if (h == 0 && tid == 0) p.kv_len_out[b] = keep;
 }
@@ -489,17 +513,24 @@ __device__ __forceinline__ void write_token(uint8_t* pg, int t, int c, const Mov
   if (c < F::kBlocks) reinterpret_cast<__half*>(pg + F::kValueScale)[c * kPage + tile_perm(t)] = m.vs;
 }
 
-// Moves the kept tokens. To other pages: every group of 8 lanes takes kept
-// tokens of its own. In place: one CTA per sequence and head goes through
-// them in order, kMoveRows groups at a time: token i comes from a slot >= i,
-// so once a round has been read, nothing that is still to be read lies below
-// what the round writes.
-constexpr int kMoveThreads = 512;
-constexpr int kMoveRows = 4;   // tokens a lane holds in one round
+// Moves the kept tokens, a group of 8 lanes to a token and ROWS tokens a lane
+// at a time. To other pages: many small CTAs. In place: one large CTA per
+// sequence and head goes through them in order: token i comes from a slot
+// >= i, so once a round has been read, nothing that is still to be read lies
+// below what the round writes.
+template <int D, bool IN_PLACE>
+struct MoveGeo {
+  static constexpr int kThreads = IN_PLACE ? 1024 : 256;
+  static constexpr int kRows = IN_PLACE ? 4 : 2;
+  static constexpr int kTokens = kThreads / 8 * kRows;   // of a CTA in a round
+};
 
-template <int D>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p, int ctas_per_row) {
+template <int D, bool IN_PLACE>
+__global__ void __launch_bounds__(MoveGeo<D, IN_PLACE>::kThreads)
+    evict_move_kernel(const EvictParams p, int ctas_per_row) {
   using F = Fmt<D>;
+  using G = MoveGeo<D, IN_PLACE>;
+  constexpr int R = G::kRows, kGroups = G::kThreads / 8;
   pdl_wait_prerequisites();
   pdl_launch_dependents();
   const int row = blockIdx.x / ctas_per_row, part = blockIdx.x - row * ctas_per_row;
@@ -507,36 +538,38 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
   bool bad = false;
   const int len = cached(p.c, b, bad);
   const int keep = min(len, p.keep);
-  if (p.in_place && keep == len) return;
+  if (IN_PLACE && keep == len) return;
   const int* index = p.index + (size_t)row * p.keep;
   const int c = threadIdx.x & 7, g = threadIdx.x >> 3;
-  constexpr int kGroups = kMoveThreads / 8;
   const size_t page_stride = (size_t)p.c.heads * F::kPageBytes;
   uint8_t* base = p.c.pages + (size_t)h * F::kPageBytes;
-  for (int i0 = part * kGroups * kMoveRows; i0 < keep; i0 += ctas_per_row * kGroups * kMoveRows) {
-    MovedToken<D> m[kMoveRows];
+  for (int i0 = part * G::kTokens; i0 < keep; i0 += ctas_per_row * G::kTokens) {
+    MovedToken<D> m[R];
+    int from[R], to[R];
 #pragma unroll
-    for (int r = 0; r < kMoveRows; ++r) {
+    for (int r = 0; r < R; ++r) {
       const int i = i0 + r * kGroups + g;
-      if (i < keep) {
-        const int from = index[i];
-        const int pg = page_of(p.c, p.c.table, p.c.table_cols, b, from / kPage, bad);
-        read_token<D>(base + pg * page_stride, from & (kPage - 1), c, m[r]);
-      }
+      from[r] = i < keep ? index[i] : 0;
+      to[r] = i < keep ? p.out_table[(size_t)b * p.out_cols + i / kPage] : 0;
     }
-    if (p.in_place) __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kMoveRows; ++r) {
+    for (int r = 0; r < R; ++r)
+      if (i0 + r * kGroups + g < keep) {
+        const int pg = page_of(p.c, p.c.table, p.c.table_cols, b, from[r] / kPage, bad);
+        read_token<D>(base + pg * page_stride, from[r] & (kPage - 1), c, m[r]);
+      }
+    if (IN_PLACE) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       const int i = i0 + r * kGroups + g;
       if (i < keep) {
-        const int to = p.out_table[(size_t)b * p.out_cols + i / kPage];
-        if ((unsigned)to < (unsigned)p.c.num_pages)
-          write_token<D>(base + to * page_stride, i & (kPage - 1), c, m[r]);
+        if ((unsigned)to[r] < (unsigned)p.c.num_pages)
+          write_token<D>(base + to[r] * page_stride, i & (kPage - 1), c, m[r]);
         else
           bad = true;
       }
     }
-    if (p.in_place) __syncthreads();
+    if (IN_PLACE) __syncthreads();
   }
   if (bad) atomicOr(p.error, kErrIndex);
 }

@@ -483,6 +483,33 @@ def test_evict(dim, in_place, lens, keep, recent, kind):
         assert torch.equal(before[used], b.pages[used])
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_of_sequences_beyond_shared_memory(in_place):
+    torch = _torch()
+    lens, keep, recent, heads, dim = [90000, 41000], 30001, 77, 1, 64
+    need = sum(-(-min(n, keep) // 64) for n in lens)
+    b = Batch(lens, heads, dim, seed=5, spare=need)
+    gen = torch.Generator().manual_seed(5)
+    weights = (torch.rand((2, heads, 64 * b.cols), generator=gen) * 1000).round().to(DEV)    # many equals
+    w = weights.cpu().numpy().copy()
+    table = b.table
+    if not in_place:
+        t = np.zeros((2, -(-keep // 64)), np.int32)
+        t[:] = b.free[:t.size].reshape(t.shape)
+        table = torch.from_numpy(t).to(DEV)
+    index, wout, kv_len = bf.kv4_evict(b.pages, b.table, b.kv_len, weights, keep, recent,
+                                       out_table=None if in_place else table, weights_out=weights if in_place else None)
+    k, v = bf.kv4_read(b.pages, table, kv_len, b.starts([keep, keep]), 2 * keep)
+    assert bf.stream_status() == 0 and kv_len.tolist() == [keep, keep]
+    for i, n in enumerate(lens):
+        stay = orc.kept(w[i, 0], n, keep, recent)
+        assert np.array_equal(index[i, 0].cpu().numpy(), stay)
+        assert np.array_equal(wout[i, 0, :keep].cpu().numpy(), w[i, 0][stay])
+        kk, vv = b.seq(i, 0)
+        assert np.array_equal(_np(k)[i * keep:(i + 1) * keep, 0], kk[stay])
+        assert np.array_equal(_np(v)[i * keep:(i + 1) * keep, 0], vv[stay])
+
+
 def test_weights_then_evict_then_attend_runs_a_sequence_under_budget():
     """Steps of append, attention with weights and eviction in place, against the oracle's own run."""
     torch = _torch()
