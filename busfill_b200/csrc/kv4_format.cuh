@@ -137,6 +137,27 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float* x) {
   for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
 }
 
+// (a, b) = (a, b) * s + t and (a, b) += t as packed fp32 pairs (sm_100)
+__device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float t) {
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %2};\n\t"
+      "mov.b64 z, {%3, %3};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(s), "f"(t));
+}
+__device__ __forceinline__ void add_f32x2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+
 // N consecutive 32-bit words, aligned to their size (16 bytes at most), by the widest loads.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {

@@ -107,26 +107,6 @@ __device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign,
   }
 }
 
-// packed fp32 pairs (sm_100): half the issue slots
-__device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float t) {   // (a, b) * s + t
-  asm("{\n\t.reg .b64 x, y, z;\n\t"
-      "mov.b64 x, {%0, %1};\n\t"
-      "mov.b64 y, {%2, %2};\n\t"
-      "mov.b64 z, {%3, %3};\n\t"
-      "fma.rn.f32x2 x, x, y, z;\n\t"
-      "mov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(a), "+f"(b)
-      : "f"(s), "f"(t));
-}
-__device__ __forceinline__ void add_f32x2(float& a, float& b, float x, float y) {   // (a, b) += (x, y)
-  asm("{\n\t.reg .b64 x, y;\n\t"
-      "mov.b64 x, {%0, %1};\n\t"
-      "mov.b64 y, {%2, %3};\n\t"
-      "add.rn.f32x2 x, x, y;\n\t"
-      "mov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(a), "+f"(b)
-      : "f"(x), "f"(y));
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
