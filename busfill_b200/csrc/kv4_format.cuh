@@ -158,6 +158,17 @@ __device__ __forceinline__ void add_f32x2(float& a, float& b, float x, float y) 
       : "f"(x), "f"(y));
 }
 
+__device__ __forceinline__ void fma_f32x2(float& a, float& b, float s0, float s1, float t0, float t1) {   // pairwise
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "mov.b64 z, {%4, %5};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(s0), "f"(s1), "f"(t0), "f"(t1));
+}
+
 // N consecutive 32-bit words, aligned to their size (16 bytes at most), by the widest loads.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {

@@ -83,25 +83,22 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
 template <int LANES>
 __device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign, float& fac) {
   if (bf16) {
-    float x[8], up = sign, top = 0.0f;
-    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+    auto pair = [](uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); };
+    auto bits = [](__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); };
+    __nv_bfloat162 top = __hmax2(__hmax2(__habs2(pair(v.x)), __habs2(pair(v.y))),
+                                 __hmax2(__habs2(pair(v.z)), __habs2(pair(v.w))));
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      x[2 * y] = __uint_as_float(e[y] << 16);
-      x[2 * y + 1] = __uint_as_float(e[y] & 0xffff0000u);
-      top = fmaxf(top, fmaxf(fabsf(x[2 * y]), fabsf(x[2 * y + 1])));
-    }
-#pragma unroll
-    for (int y = 1; y < LANES; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
-    int ex = 136 - (int)(__float_as_uint(top) >> 23);
-    if (top == 0.0f || !(top <= 3.4e38f)) ex = 0;
-    ex = max(-126, min(126, ex));
-    up *= __uint_as_float((unsigned)(127 + ex) << 23);
+    for (int y = 1; y < LANES; y <<= 1) top = __hmax2(top, pair(__shfl_xor_sync(0xffffffffu, bits(top), y)));
+    const unsigned e = __bfloat16_as_ushort(__hmax(top.x, top.y)) >> 7;   // biased exponent; 255: not finite
+    const int ex = e == 0 || e == 255 ? 0 : max(-126, min(126, 136 - (int)e));
+    const __nv_bfloat162 up = __bfloat162bfloat162(
+        __ushort_as_bfloat16((unsigned short)((127 + ex) << 7 | (sign < 0.0f ? 0x8000 : 0))));
     fac *= __uint_as_float((unsigned)(127 - ex) << 23);
-    v.x = h2_as_u32(__floats2half2_rn(x[0] * up, x[1] * up));
-    v.y = h2_as_u32(__floats2half2_rn(x[2] * up, x[3] * up));
-    v.z = h2_as_u32(__floats2half2_rn(x[4] * up, x[5] * up));
-    v.w = h2_as_u32(__floats2half2_rn(x[6] * up, x[7] * up));
+    auto half = [&](uint32_t u) {
+      const uint32_t x = bits(__hmul2(pair(u), up));   // exact
+      return h2_as_u32(__floats2half2_rn(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)));
+    };
+    v = make_uint4(half(v.x), half(v.y), half(v.z), half(v.w));
   } else if (sign < 0.0f) {
     v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
   }

@@ -37,7 +37,7 @@ struct Geo {
   static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kStages = 2;                        // query blocks, each with its S^T in TMEM
   static constexpr int kKeyOff = 0, kQOff = kKeyBufs * kKeyBytes;
-  static constexpr int kConstOff = kQOff + kStages * kQBytes;   // per row: factor, -lse2, first and last slot
+  static constexpr int kConstOff = kQOff + kStages * kQBytes;   // [factor, -lse2, first slot, slot behind the last][row]
   static constexpr int kBarOff = kConstOff + kStages * 128 * 16;
   static constexpr int bKFull = 0, bKEmpty = bKFull + kKeyBufs, bQFull = bKEmpty + kKeyBufs,
                        bQEmpty = bQFull + kStages, bS = bQEmpty + kStages, bFinal = bS + kStages, kBars = bFinal + 1;
@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
   if (warp == 0) {
     // ---------------- MMA ----------------
     constexpr uint32_t kIdesc = make_idesc_f16_f32(128, 128);
+    // descriptors are made once and stepped by their address field
+    const uint64_t k_desc = make_sdesc_sw128(sbase + G::kKeyOff), q_desc = make_sdesc_sw128(sbase + G::kQOff);
     uint32_t item = 0, n = 0;
     for_pieces([&](const Item&, int, int blocks, int) {
       const int kb = item % G::kKeyBufs;
@@ -204,14 +206,14 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
         if (!wait(G::bQFull + st, n / G::kStages)) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t b = sbase + G::kQOff + st * G::kQBytes;
+          const uint64_t b = q_desc + (uint32_t)(st * G::kQBytes / 16);
 #pragma unroll
           for (int i = 0; i < TT; ++i) {
-            const uint32_t a = sbase + G::kKeyOff + kb * G::kKeyBytes + i * G::kKeyTile;
+            const uint64_t a = k_desc + (uint32_t)((kb * G::kKeyBytes + i * G::kKeyTile) / 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              mma_f16_ss(tmem + (st * TT + i) * 128, make_sdesc_sw128(a + (k / 4) * 128 * 128 + (k % 4) * 32),
-                         make_sdesc_sw128(b + (k / 4) * 128 * 128 + (k % 4) * 32), kIdesc, k > 0);
+              mma_f16_ss(tmem + (st * TT + i) * 128, a + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16,
+                         b + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, kIdesc, k > 0);
           }
           tc_commit(BAR(G::bS + st));
           tc_commit(BAR(G::bQEmpty + st));
@@ -265,44 +267,53 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(G::bKFull + kb));
       ++item;
-      for (int blk = 0; blk < blocks; ++blk, ++n) {
-        const int st = n % G::kStages;
-        if (!wait(G::bQEmpty + st, n / G::kStages + 1)) return false;
-        constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;   // a warp's 16 rows
-        const int c = lane % LPR, row0 = (it.block0 + from + blk) * 128 + w * 16;
-        uint4 v[NI];
+      // a block's rows are on their way while its stage is still in use
+      constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;   // a warp's 16 rows
+      const int c = lane % LPR;
+      uint4 v[NI];
+      float lse[NI];
+      auto fetch = [&](int blk) {
+        const int row0 = (it.block0 + from + blk) * 128 + w * 16;
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
           const int row = row0 + k * RPI + lane / LPR, tok = p.by_group(row);
           v[k] = make_uint4(0, 0, 0, 0);
-          if (tok < it.s.n)
-            v[k] = __ldg(reinterpret_cast<const uint4*>(
-                static_cast<const uint16_t*>(p.q) + (size_t)(it.s.first + tok) * p.q_token +
-                (size_t)(it.head * p.group + row - tok * p.group) * p.q_head + 8 * c));
+          lse[k] = -INFINITY;
+          if (tok < it.s.n) {
+            const int r = it.s.first + tok, h = it.head * p.group + row - tok * p.group;
+            v[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (size_t)r * p.q_token +
+                                                        (size_t)h * p.q_head + 8 * c));
+            if (c == 0) lse[k] = p.lse[(size_t)r * p.q_heads + h];
+          }
         }
-        float4* consts = reinterpret_cast<float4*>(smem + G::kConstOff) + st * 128 + w * 16;
+      };
+      fetch(0);
+      for (int blk = 0; blk < blocks; ++blk, ++n) {
+        const int st = n % G::kStages;
+        if (!wait(G::bQEmpty + st, n / G::kStages + 1)) return false;
+        const int row0 = (it.block0 + from + blk) * 128 + w * 16;
+        float* consts = reinterpret_cast<float*>(smem + G::kConstOff) + st * 512 + w * 16;
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-          const int r = k * RPI + lane / LPR, row = row0 + r, tok = p.by_group(row);
-          float fac = fabsf(p.scale_log2);
+          const int r = k * RPI + lane / LPR;
+          float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
           normalize_query8<LPR>(v[k], p.bf16, sign, fac);
           const int rr = w * 16 + r;
           *reinterpret_cast<uint4*>(smem + G::kQOff + st * G::kQBytes + (c / 8) * 128 * 128 + rr * 128 +
                                     (((c & 7) ^ (rr & 7)) << 4)) = v[k];
           if (c == 0) {
-            float lse2 = INFINITY;   // rows that are not there or see nothing give no weight
+            const int tok = p.by_group(row0 + r);
             int lo = 0, hi = 0;
-            if (tok < it.s.n) {
-              const float x = p.lse[(size_t)(it.s.first + tok) * p.q_heads + it.head * p.group + row - tok * p.group];
-              if (x != -INFINITY) lse2 = x * kLog2e;
-              sees(p, it.s, tok, lo, hi);
-            }
-            consts[r] = make_float4(fac, -lse2, __int_as_float(lo), __int_as_float(hi));
+            if (tok < it.s.n) sees(p, it.s, tok, lo, hi);
+            // rows that are not there or see nothing give no weight
+            consts[r] = fac, consts[128 + r] = lse[k] == -INFINITY ? -INFINITY : -lse[k] * kLog2e;
+            consts[256 + r] = __int_as_float(lo), consts[384 + r] = __int_as_float(hi);
           }
         }
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(G::bQFull + st));
+        if (blk + 1 < blocks) fetch(blk + 1);
       }
       return true;
     });
@@ -324,28 +335,34 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
         const int st = n % G::kStages;
         if (!wait(G::bS + st, n / G::kStages)) break;
         tc_fence_after();
-        const float4* consts = reinterpret_cast<const float4*>(smem + G::kConstOff) + st * 128;
+        const float* consts = reinterpret_cast<const float*>(smem + G::kConstOff) + st * 512;
         // the block's first row ends first, its last row begins last
         const int r1 = min((it.block0 + from + blk) * 128 + 127, it.s.n * p.group - 1) - (it.block0 + from + blk) * 128;
-        const bool whole = base + 32 <= __float_as_int(consts[0].w) && base >= __float_as_int(consts[r1].z);
+        const bool whole = base + 32 <= __float_as_int(consts[384]) && base >= __float_as_int(consts[256 + r1]);
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           float s[32];
           tmem_ld_x32(tm + (st * TT + i) * 128 + c, reinterpret_cast<uint32_t*>(s));
           tc_wait_ld();
-          if (whole) {
+          if (!whole) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float2 x = *reinterpret_cast<const float2*>(consts + c + k);
-              sum[k & 3] += exp2_approx(fmaf(s[k], x.x, x.y));
+            for (int k = 0; k < 32; k += 4) {
+              const float4 lo = *reinterpret_cast<const float4*>(consts + 256 + c + k),
+                           hi = *reinterpret_cast<const float4*>(consts + 384 + c + k);
+              s[k] = slot >= __float_as_int(lo.x) && slot < __float_as_int(hi.x) ? s[k] : -INFINITY;
+              s[k + 1] = slot >= __float_as_int(lo.y) && slot < __float_as_int(hi.y) ? s[k + 1] : -INFINITY;
+              s[k + 2] = slot >= __float_as_int(lo.z) && slot < __float_as_int(hi.z) ? s[k + 2] : -INFINITY;
+              s[k + 3] = slot >= __float_as_int(lo.w) && slot < __float_as_int(hi.w) ? s[k + 3] : -INFINITY;
             }
-          } else {
+          }
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float4 x = consts[c + k];
-              const float e = exp2_approx(fmaf(s[k], x.x, x.y));
-              sum[k & 3] += slot >= __float_as_int(x.z) && slot < __float_as_int(x.w) ? e : 0.0f;
-            }
+          for (int k = 0; k < 32; k += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(consts + c + k),
+                         t = *reinterpret_cast<const float4*>(consts + 128 + c + k);
+            fma_f32x2(s[k], s[k + 1], f.x, f.y, t.x, t.y);
+            fma_f32x2(s[k + 2], s[k + 3], f.z, f.w, t.z, t.w);
+            add_f32x2(sum[0], sum[1], exp2_approx(s[k]), exp2_approx(s[k + 1]));
+            add_f32x2(sum[2], sum[3], exp2_approx(s[k + 2]), exp2_approx(s[k + 3]));
           }
         }
         tc_fence_before();
