@@ -67,53 +67,63 @@ def _packer(cls):
 
 
 _pack_cache, _pack_rope, _pack_rows, _pack_attn, _pack_eviction = map(_packer, (Cache, Rope, Rows, Attn, Eviction))
-_TYPE = {}   # torch dtype -> BUSFILL_TYPE_*
+_TYPE = {}   # torch dtype -> BUSFILL_TYPE_*; filled with torch's dtypes at the first call
+_U8 = _I32 = _F32 = _F16 = _raw_stream = None
 
 
-def _dtype(t, name):
-    if not _TYPE:
-        torch = _torch()
-        _TYPE.update({torch.float16: 1, torch.bfloat16: 30})
-    code = _TYPE.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name} must be fp16 or bf16, got {t.dtype}")
-    return code
+def _init():
+    global _U8, _I32, _F32, _F16, _raw_stream
+    torch = _torch()
+    _U8, _I32, _F32, _F16 = torch.uint8, torch.int32, torch.float32, torch.float16
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+    _TYPE.update({torch.float16: 1, torch.bfloat16: 30})
 
 
-def _need_cuda(t, name):
-    if not isinstance(t, _torch().Tensor) or not t.is_cuda:
+def _refuse_heads(t, name, like):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _TYPE or (like is not None and t.dtype != like.dtype):
+        raise TypeError(f"{name} must be {'fp16 or bf16' if like is None else like.dtype}, got {t.dtype}")
+    raise ValueError(f"{name} must be [tokens, heads, D] with contiguous channels, got {tuple(t.shape)} with strides "
+                     f"{t.stride()}")
 
 
-def _need_heads(t, name, like=None):
-    """A step's tensor [tokens, heads, D], fp16 or bf16, channels contiguous; (token, head) strides."""
-    _need_cuda(t, name)
-    if like is None:
-        _dtype(t, name)
-    elif t.dtype != like.dtype:
-        raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, D], got {tuple(t.shape)}")
-    token, head, channel = t.stride()
-    if channel != 1 and t.shape[2] > 1:
-        raise ValueError(f"{name} must have contiguous channels")
-    return token, head
+def _heads(t, name, like=None):
+    """(token, head) strides of a step's tensor [tokens, heads, D]: fp16 or bf16, channels contiguous."""
+    if not _TYPE:
+        _init()
+    try:
+        if t.is_cuda and (t.dtype in _TYPE if like is None else t.dtype is like.dtype):
+            token, head, channel = t.stride()
+            if channel == 1 or t.shape[2] == 1:
+                return token, head
+    except (AttributeError, ValueError):
+        pass
+    _refuse_heads(t, name, like)
 
 
-def _need_array(t, dtype, name, ndim):
-    _need_cuda(t, name)
+def _array(t, dtype, name, ndim):
+    """The address of a contiguous CUDA tensor of that type and rank."""
+    try:
+        if t.is_cuda and t.dtype is dtype and t.dim() == ndim and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != ndim or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {ndim}-D tensor")
+    raise ValueError(f"{name} must be a contiguous {ndim}-D tensor")
 
 
 def _cache(pages, table, kv_len):
     """(busfill_kv4 as bytes, batch, heads, head_dim, table columns)"""
-    torch = _torch()
-    _need_array(pages, torch.uint8, "pages", 3)
-    _need_array(table, torch.int32, "table", 2)
-    _need_array(kv_len, torch.int32, "kv_len", 1)
+    if not _TYPE:
+        _init()
+    pages_ptr, table_ptr, len_ptr = (_array(pages, _U8, "pages", 3), _array(table, _I32, "table", 2),
+                                     _array(kv_len, _I32, "kv_len", 1))
     num_pages, heads, width = pages.shape
     batch, cols = table.shape
     dim, rest = divmod(width, 72)
@@ -121,8 +131,7 @@ def _cache(pages, table, kv_len):
         raise ValueError(f"pages must be [num_pages, kv_heads, 72 * D] with D 64, 128 or 256, got {tuple(pages.shape)}")
     if batch != kv_len.shape[0]:
         raise ValueError(f"table {tuple(table.shape)} and kv_len {tuple(kv_len.shape)} differ in batch")
-    return (_pack_cache(pages.data_ptr(), table.data_ptr(), kv_len.data_ptr(), num_pages, cols, batch, heads, dim),
-            batch, heads, dim, cols)
+    return _pack_cache(pages_ptr, table_ptr, len_ptr, num_pages, cols, batch, heads, dim), batch, heads, dim, cols
 
 
 def _need_start(q_start, batch, tokens):
@@ -130,34 +139,34 @@ def _need_start(q_start, batch, tokens):
         if tokens != batch:
             raise ValueError(f"{tokens} rows for {batch} sequences: give q_start")
         return 0
-    _need_array(q_start, _torch().int32, "q_start", 1)
+    ptr = _array(q_start, _I32, "q_start", 1)
     if q_start.shape[0] != batch + 1:
         raise ValueError(f"q_start must have {batch + 1} entries, got {q_start.shape[0]}")
-    return q_start.data_ptr()
+    return ptr
 
 
-def _need_weights(weights, name, batch, heads, cols):
-    _need_array(weights, _torch().float32, name, 3)
+def _weights(weights, name, batch, heads, cols):
+    """(address, columns)"""
+    ptr = _array(weights, _F32, name, 3)
     b, h, n = weights.shape
     if b != batch or h != heads or n < KV4_PAGE * cols:
         raise ValueError(f"{name} must be [{batch}, {heads}, >= {KV4_PAGE * cols}], got {tuple(weights.shape)}")
-    return n
+    return ptr, n
 
 
 def _raw(stream, like):
     """The cudaStream_t of the call."""
     if stream is None:
-        return _torch()._C._cuda_getCurrentRawStream(like.get_device())
+        return _raw_stream(like.get_device())
     return stream.cuda_stream
 
 
-def _empty(stream, shape, dtype, device):
-    """A tensor that belongs to the call's stream."""
-    torch = _torch()
+def _empty(stream, like, shape, dtype):
+    """A tensor on like's device that belongs to the call's stream."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def kv4_page_bytes(head_dim: int) -> int:
@@ -192,45 +201,46 @@ def rope_axes(q, k, positions, cos, sin, axis=None, adjacent=False, inverse=Fals
     it (default: axis 0). Frequency i turns channels (i, i + rot/2), or (2i, 2i + 1) with
     ``adjacent``; channels from rot on are copied. ``inverse`` turns back, which is also the gradient.
     q_out, k_out may be q, k. Returns (q_out, k_out)."""
-    torch = _torch()
-    q_token, q_head = _need_heads(q, "q")
-    _need_cuda(positions, "positions")
-    if positions.dim() == 1:
+    q_token, q_head = _heads(q, "q")
+    if getattr(positions, "ndim", 0) == 1:
         positions = positions[None]
-    _need_array(positions, torch.int32, "positions", 2)
-    _need_array(cos, torch.float32, "cos", 2)
-    _need_array(sin, torch.float32, "sin", 2)
-    tokens, heads, dim = q.shape
+    pos_ptr, cos_ptr, sin_ptr = (_array(positions, _I32, "positions", 2), _array(cos, _F32, "cos", 2),
+                                 _array(sin, _F32, "sin", 2))
+    shape = q.shape
+    tokens, heads, dim = shape
     max_pos, half = cos.shape
-    axes = positions.shape[0]
+    axes, n = positions.shape
     axis = bytes(half) if axis is None else bytes(axis)
-    if cos.shape != sin.shape or len(axis) != half or positions.shape[1] != tokens:
+    if sin.shape != cos.shape or len(axis) != half or n != tokens:
         raise ValueError(f"shape mismatch: cos {tuple(cos.shape)}, sin {tuple(sin.shape)}, axis {len(axis)}, "
-                         f"positions {tuple(positions.shape)}, q {tuple(q.shape)}")
-    if max(axis, default=0) >= axes:
+                         f"positions {tuple(positions.shape)}, q {tuple(shape)}")
+    if half and max(axis) >= axes:
         raise ValueError(f"axis entries must be in 0..{axes - 1}")
     if q_out is None:
-        q_out = _empty(stream, q.shape, q.dtype, q.device)
-    elif q_out.shape != q.shape:
-        raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-    qo_token, qo_head = _need_heads(q_out, "q_out", like=q)
+        q_out = _empty(stream, q, shape, q.dtype)
+        qo_token, qo_head = heads * dim, dim
+    else:
+        qo_token, qo_head = _heads(q_out, "q_out", like=q)
+        if q_out.shape != shape:
+            raise ValueError(f"q_out must be {tuple(shape)}, got {tuple(q_out.shape)}")
     k_ptr = ko_ptr = k_heads = k_token = k_head = ko_token = ko_head = 0
     if k is not None:
-        k_token, k_head = _need_heads(k, "k", like=q)
-        k_heads = k.shape[1]
-        if k.shape[0] != tokens or k.shape[2] != dim:
-            raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        k_token, k_head = _heads(k, "k", like=q)
+        n, k_heads, k_dim = k.shape
+        if n != tokens or k_dim != dim:
+            raise ValueError(f"shape mismatch: q {tuple(shape)}, k {tuple(k.shape)}")
         if k_out is None:
-            k_out = _empty(stream, k.shape, k.dtype, k.device)
-        elif k_out.shape != k.shape:
-            raise ValueError(f"k_out must be {tuple(k.shape)}, got {tuple(k_out.shape)}")
-        ko_token, ko_head = _need_heads(k_out, "k_out", like=q)
+            k_out = _empty(stream, k, k.shape, k.dtype)
+            ko_token, ko_head = k_heads * dim, dim
+        else:
+            ko_token, ko_head = _heads(k_out, "k_out", like=q)
+            if k_out.shape != k.shape:
+                raise ValueError(f"k_out must be {tuple(k.shape)}, got {tuple(k_out.shape)}")
         k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     table = ctypes.create_string_buffer(axis, half)
-    r = _pack_rope(q.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, positions.data_ptr(), cos.data_ptr(),
-                   sin.data_ptr(), ctypes.addressof(table), q_token, q_head, k_token, k_head, qo_token, qo_head,
-                   ko_token, ko_head, tokens, heads, k_heads, dim, 2 * half, axes, max_pos, bool(adjacent),
-                   bool(inverse), _dtype(q, "q"))
+    r = _pack_rope(q.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, pos_ptr, cos_ptr, sin_ptr, ctypes.addressof(table),
+                   q_token, q_head, k_token, k_head, qo_token, qo_head, ko_token, ko_head, tokens, heads, k_heads, dim,
+                   2 * half, axes, max_pos, bool(adjacent), bool(inverse), _TYPE[q.dtype])
     _check(_lib().busfill_rope_axes(r, _raw(stream, q)), "busfill_rope_axes")
     return q_out, k_out
 
@@ -239,13 +249,13 @@ def kv4_append(pages, table, kv_len, k, v, q_start=None, stream=None):
     """Quantize the step's keys and values [tokens, kv_heads, D] into the slots of their sequences'
     newest tokens (row r of a sequence's n rows goes to slot kv_len - n + r)."""
     c, batch, heads, dim, _ = _cache(pages, table, kv_len)
-    k_token, k_head = _need_heads(k, "k")
-    v_token, v_head = _need_heads(v, "v", like=k)
-    tokens = k.shape[0]
-    if k.shape != v.shape or k.shape[1] != heads or k.shape[2] != dim:
+    k_token, k_head = _heads(k, "k")
+    v_token, v_head = _heads(v, "v", like=k)
+    tokens, k_heads, k_dim = k.shape
+    if k.shape != v.shape or k_heads != heads or k_dim != dim:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {heads}, {dim}]")
     r = _pack_rows(k.data_ptr(), v.data_ptr(), _need_start(q_start, batch, tokens), k_token, k_head, v_token, v_head,
-                   tokens, _dtype(k, "k"))
+                   tokens, _TYPE[k.dtype])
     _check(_lib().busfill_kv4_append(c, r, _raw(stream, pages)), "busfill_kv4_append")
 
 
@@ -255,7 +265,7 @@ def kv4_read(pages, table, kv_len, q_start=None, tokens=None, stream=None):
     c, batch, heads, dim, _ = _cache(pages, table, kv_len)
     tokens = batch if tokens is None else int(tokens)
     start = _need_start(q_start, batch, tokens)
-    k, v = _empty(stream, (2, tokens, heads, dim), _torch().float16, pages.device).unbind()
+    k, v = _empty(stream, pages, (2, tokens, heads, dim), _F16).unbind()
     _check(_lib().busfill_kv4_read(c, start, tokens, k.data_ptr(), v.data_ptr(), _raw(stream, pages)),
            "busfill_kv4_read")
     return k, v
@@ -272,31 +282,32 @@ def attn_kv4(q, pages, table, kv_len, q_start=None, max_q=None, scale=None, caus
     To ``weights`` fp32 [batch, kv_heads, cols >= 64 * table columns] the attention weight of every
     cached token, summed over the call's rows and the group's heads, is added."""
     c, batch, kv_heads, head_dim, cols = _cache(pages, table, kv_len)
-    q_token, q_head = _need_heads(q, "q")
-    tokens, heads, dim = q.shape
+    q_token, q_head = _heads(q, "q")
+    shape = q.shape
+    tokens, heads, dim = shape
     if dim != head_dim or heads % kv_heads:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {kv_heads} heads of {head_dim}")
     start = _need_start(q_start, batch, tokens)
     w_ptr = w_cols = lse_ptr = 0
     if weights is not None:
-        w_cols = _need_weights(weights, "weights", batch, kv_heads, cols)
-        w_ptr = weights.data_ptr()
+        w_ptr, w_cols = _weights(weights, "weights", batch, kv_heads, cols)
         if lse is None:
-            lse = _empty(stream, (tokens, heads), weights.dtype, q.device)
+            lse = _empty(stream, q, (tokens, heads), _F32)
     if lse is not None:
-        _need_array(lse, _torch().float32, "lse", 2)
+        lse_ptr = _array(lse, _F32, "lse", 2)
         if lse.shape != (tokens, heads):
             raise ValueError(f"lse must be [{tokens}, {heads}], got {tuple(lse.shape)}")
-        lse_ptr = lse.data_ptr()
     if out is None:
-        out = _empty(stream, q.shape, q.dtype, q.device)
-    elif out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    o_token, o_head = _need_heads(out, "out", like=q)
+        out = _empty(stream, q, shape, q.dtype)
+        o_token, o_head = heads * dim, dim
+    else:
+        o_token, o_head = _heads(out, "out", like=q)
+        if out.shape != shape:
+            raise ValueError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     a = _pack_attn(q.data_ptr(), out.data_ptr(), lse_ptr, w_ptr, start, q_token, q_head, o_token, o_head, w_cols,
                    dim ** -0.5 if scale is None else scale, tokens, heads,
                    max(1, tokens if max_q is None else int(max_q)) if start else 1, bool(causal), int(window),
-                   _dtype(q, "q"))
+                   _TYPE[q.dtype])
     _check(_lib().busfill_attn_kv4(c, a, _raw(stream, q)), "busfill_attn_kv4")
     return out
 
@@ -307,25 +318,25 @@ def kv4_evict(pages, table, kv_len, weights, keep, recent, out_table=None, weigh
     equals), in their order. ``out_table`` int32 [batch, cols] names the pages they move to (default:
     the same table, in place). Returns (index, weights_out, new kv_len): index int32 [batch,
     kv_heads, keep] holds the slots they came from (-1 behind a shorter sequence's)."""
-    torch = _torch()
     c, batch, heads, _, cols = _cache(pages, table, kv_len)
-    w_cols = _need_weights(weights, "weights", batch, heads, cols)
+    w_ptr, w_cols = _weights(weights, "weights", batch, heads, cols)
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"need 1 <= keep and 0 <= recent <= keep, got keep {keep}, recent {recent}")
     out_table = table if out_table is None else out_table
-    _need_array(out_table, torch.int32, "out_table", 2)
-    if out_table.shape[0] != batch or out_table.shape[1] * KV4_PAGE < keep:
+    out_ptr = _array(out_table, _I32, "out_table", 2)
+    rows, out_cols = out_table.shape
+    if rows != batch or out_cols * KV4_PAGE < keep:
         raise ValueError(f"out_table must be [{batch}, >= {-(-keep // KV4_PAGE)}], got {tuple(out_table.shape)}")
-    index = _empty(stream, (batch, heads, keep), torch.int32, pages.device)
-    kv_len_out = _empty(stream, (batch,), torch.int32, pages.device)
+    index = _empty(stream, kv_len, (batch, heads, keep), _I32)
+    kv_len_out = _empty(stream, kv_len, (batch,), _I32)
     if weights_out is None:
-        weights_out = _empty(stream, weights.shape, torch.float32, pages.device)
+        weights_out = _empty(stream, weights, weights.shape, _F32)
+        wo_ptr = weights_out.data_ptr()
     else:
-        _need_array(weights_out, torch.float32, "weights_out", 3)
+        wo_ptr = _array(weights_out, _F32, "weights_out", 3)
         if weights_out.shape != weights.shape:
             raise ValueError(f"weights_out must be {tuple(weights.shape)}, got {tuple(weights_out.shape)}")
-    e = _pack_eviction(weights.data_ptr(), weights_out.data_ptr(), w_cols, index.data_ptr(), kv_len_out.data_ptr(),
-                       out_table.data_ptr(), out_table.shape[1], keep, recent)
+    e = _pack_eviction(w_ptr, wo_ptr, w_cols, index.data_ptr(), kv_len_out.data_ptr(), out_ptr, out_cols, keep, recent)
     _check(_lib().busfill_kv4_evict(c, e, _raw(stream, pages)), "busfill_kv4_evict")
     return index, weights_out, kv_len_out
