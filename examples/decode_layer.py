@@ -25,7 +25,7 @@ HIDDEN, HEADS, KV_HEADS, DIM = 5120, 64, 8, 128
 def random_q4k(rows, k, gen, dev):
     """Random block_q4_K rows [rows, k / 256 * 144] with small scales."""
     blocks = torch.randint(0, 256, (rows, k // 256, 144), dtype=torch.uint8, generator=gen).to(dev)
-    blocks[..., 0:4] = torch.tensor([6e-5, 4e-4], dtype=torch.float16).view(torch.uint8).to(dev)
+    blocks[..., 0:4] = torch.tensor([4e-5, 3e-4], dtype=torch.float16).view(torch.uint8).to(dev)
     return blocks.view(rows, -1)
 
 
