@@ -104,6 +104,12 @@ __device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign,
   }
 }
 
+// 16 bytes to shared memory; zeros unless `have`
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -172,6 +178,13 @@ static_assert(sizeof(Work) <= 64, "descriptor slots");
 // Tiles that the start and the end of an item are worth (queries, epilogue,
 // refilling the pipeline).
 constexpr int kItemCost = 2;
+// A range is worth at least kMinCost tiles, and its end moves to an item's edge
+// where that is at most kSnap tiles away.
+constexpr int kMinCost = 4;
+constexpr int kSnap = 3;
+static_assert(kSnap >= kItemCost, "a cut leaves tiles on both sides");
+// how far behind its start an item of cost c is not cut
+__device__ __forceinline__ int near_start(int c) { return min(kSnap, c / 2); }
 
 template <int D>
 __device__ __forceinline__ int groups_of(const AttnParams& p, const Span& s) {
@@ -275,7 +288,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
     if (warp == 2) {
       // ---------------- work list ----------------
       const int T = pre[batch];
-      const long long ctas = min((int)gridDim.x, T);
+      const long long ctas = max(1, min((int)gridDim.x, T / kMinCost));
       const bool idle = (int)blockIdx.x >= ctas;
       const int u0 = idle ? 0 : (int)((long long)T * blockIdx.x / ctas);
       const int u1 = idle ? 0 : (int)((long long)T * (blockIdx.x + 1) / ctas);
@@ -324,17 +337,23 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           }
           r -= __shfl_sync(0xffffffffu, x, 31);
         }
-        // tile k of an item that begins at cost x lies at cost x + kItemCost + k
+        // A range ends at cost u: between tiles of the item that begins at x and
+        // costs c, unless that is near an edge of the item.
+        auto cut = [&](int u, int x, int c) {
+          const int o = u - x;
+          return o <= near_start(c) ? 0 : o + kSnap >= c ? c - kItemCost : o - kItemCost;
+        };
+        // the CTA whose range holds cost y
         auto cta_of = [&](int y) { return (int)((((long long)y + 1) * ctas - 1) / T); };
         for (int x = u0 - r;;) {
           it.tiles = tiles_of<D>(p, it.s, it.t, it.tile0);
-          const int from = min(max(u0 - x - kItemCost, 0), it.tiles), to = min(max(u1 - x - kItemCost, 0), it.tiles);
+          const int c = it.tiles + kItemCost, from = cut(u0, x, c), to = cut(u1, x, c);
           if (to > from) {
             Work y;
             y.b = it.b, y.head = it.head, y.first = it.s.first, y.n = it.s.n, y.len = it.s.len;
             y.row0 = it.t * G::kRows, y.tile0 = it.tile0 + from, y.tiles = to - from;
             y.kind = from > 0 ? kTail : to < it.tiles ? kHead : kWhole;
-            y.c_first = cta_of(x + kItemCost), y.c_last = cta_of(x + kItemCost + it.tiles - 1);
+            y.c_first = cta_of(x + near_start(c)), y.c_last = cta_of(x + c - kSnap - 1);
             y.row_tiles = RT == 2 && it.s.n * p.group - y.row0 > 128 ? 2 : 1;
             if (!push(y)) break;
             // its queries on their way to L2
@@ -348,7 +367,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
               }
             }
           }
-          x += it.tiles + kItemCost;
+          x += c;
           if (x >= u1) break;
           if (++it.t == it.groups) {
             it.t = 0;
@@ -560,34 +579,52 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
     const uint32_t ts = tm + G::kS + i * K, to = tm + G::kO + i * D;
     uint32_t done = 0, joins = 0;
     const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    // queries of a piece's row tile to shared memory, lanes together on a row,
-    // 16 bytes each
+    // Queries of a piece's row tile to shared memory, lanes together on a row,
+    // 16 bytes each: copied asynchronously, then brought to fp16's range where
+    // they lie. Short loops: 16 rows' loads and normalizations unrolled were
+    // fetched from beyond the instruction cache for every item (7 us).
     constexpr int LPR = D / 8, RPI = 32 / LPR, NQ = 32 / RPI;
     auto load_q = [&](const Work& x) {
-      const int row0 = x.row0 + i * 128 + 32 * q, c = lane % LPR;
-      constexpr int BATCH = NQ < 16 ? NQ : 16;   // loads in flight
-#pragma unroll 1
-      for (int k0 = 0; k0 < NQ; k0 += BATCH) {
-        uint4 v[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const int row = row0 + (k0 + k) * RPI + lane / LPR, tok = p.by_group(row);
-          v[k] = make_uint4(0, 0, 0, 0);
-          if (tok < x.n)
-            v[k] = __ldg(reinterpret_cast<const uint4*>(
-                static_cast<const uint16_t*>(p.q) + (size_t)(x.first + tok) * p.q_token +
-                (size_t)(x.head * p.group + row - tok * p.group) * p.q_head + 8 * c));
-        }
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const int r = 32 * q + (k0 + k) * RPI + lane / LPR;
-          float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
-          normalize_query8<LPR>(v[k], p.bf16, sign, fac);
-          *reinterpret_cast<uint4*>(smem + G::kQOff + i * G::kQTileBytes + (c / 8) * 128 * 128 + r * 128 +
-                                    (((c & 7) ^ (r & 7)) << 4)) = v[k];
-          if (c == 0) factors[i * 128 + r] = fac;
-        }
+      const int c = lane % LPR, r0 = 32 * q + lane / LPR;
+      const uint32_t q_tile = (uint32_t)(G::kQOff + i * G::kQTileBytes + (c / 8) * 128 * 128);
+      auto at = [&](int r) { return q_tile + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (size_t)x.first * p.q_token +
+                            (size_t)(x.head * p.group) * p.q_head + 8 * c;
+#pragma unroll 2
+      for (int k = 0; k < NQ; ++k) {
+        const int r = r0 + k * RPI, row = x.row0 + i * 128 + r, tok = p.by_group(row);
+        const bool have = tok < x.n;
+        cp_async16(sbase + at(r), have ? src + (size_t)tok * p.q_token + (size_t)(row - tok * p.group) * p.q_head : src,
+                   have);
       }
+      cp_async_wait_all();
+      const float fac0 = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
+      auto in_place = [&](auto bf16) {
+        constexpr int BATCH = 4;
+#pragma unroll 1
+        for (int k0 = 0; k0 < NQ; k0 += BATCH) {
+          uint4 v[BATCH];
+          float fac[BATCH];
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) v[k] = *reinterpret_cast<const uint4*>(smem + at(r0 + (k0 + k) * RPI));
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            fac[k] = fac0;
+            normalize_query8<LPR>(v[k], bf16(), sign, fac[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            *reinterpret_cast<uint4*>(smem + at(r0 + (k0 + k) * RPI)) = v[k];
+            if (c == 0) factors[i * 128 + r0 + (k0 + k) * RPI] = fac[k];
+          }
+        }
+      };
+      if (p.bf16)
+        in_place(std::true_type());
+      else if (sign < 0.0f)
+        in_place(std::false_type());
+      else
+        factors[i * 128 + my_row] = fac0;
       fence_proxy_async_shared();
       tc_fence_before();
       __syncwarp();
@@ -792,7 +829,19 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
             float o[32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = 0.0f;
-            for (int y = 0; y < n; ++y) {
+            int y = 0;
+#pragma unroll 1
+            for (; y + 1 < n; y += 2) {   // two parts' loads in flight
+              const float a = share(y), b = share(y + 1);
+              float u[32], v[32];
+#pragma unroll
+              for (int k = 0; k < 32; ++k) u[k] = __ldcg(theirs(y) + (c2 + k) * G::kRows + r);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = __ldcg(theirs(y + 1) + (c2 + k) * G::kRows + r);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = fmaf(v[k], b, fmaf(u[k], a, o[k]));
+            }
+            if (y < n) {
               const float a = share(y);
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] = fmaf(__ldcg(theirs(y) + (c2 + k) * G::kRows + r), a, o[k]);

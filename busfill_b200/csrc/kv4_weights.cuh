@@ -267,48 +267,67 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(G::bKFull + kb));
       ++item;
-      // a block's rows are on their way while its stage is still in use
-      constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;   // a warp's 16 rows
+      // A block's rows are on their way while its stage is still in use (the
+      // first PRE of a lane's); lane r holds the constants of the warp's row r.
+      constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI, PRE = NI < 8 ? NI : 8;
       const int c = lane % LPR;
-      uint4 v[NI];
-      float lse[NI];
+      uint4 v[PRE];
+      float lse;
+      int lo, hi;
+      auto load = [&](int row0, int k0) {
+#pragma unroll
+        for (int k = 0; k < PRE; ++k) {
+          const int row = row0 + (k0 + k) * RPI + lane / LPR, tok = p.by_group(row);
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (tok < it.s.n)
+            v[k] = __ldg(reinterpret_cast<const uint4*>(
+                static_cast<const uint16_t*>(p.q) + (size_t)(it.s.first + tok) * p.q_token +
+                (size_t)(it.head * p.group + row - tok * p.group) * p.q_head + 8 * c));
+        }
+      };
       auto fetch = [&](int blk) {
         const int row0 = (it.block0 + from + blk) * 128 + w * 16;
-#pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          const int row = row0 + k * RPI + lane / LPR, tok = p.by_group(row);
-          v[k] = make_uint4(0, 0, 0, 0);
-          lse[k] = -INFINITY;
-          if (tok < it.s.n) {
-            const int r = it.s.first + tok, h = it.head * p.group + row - tok * p.group;
-            v[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (size_t)r * p.q_token +
-                                                        (size_t)h * p.q_head + 8 * c));
-            if (c == 0) lse[k] = p.lse[(size_t)r * p.q_heads + h];
-          }
+        load(row0, 0);
+        const int row = row0 + (lane & 15), tok = p.by_group(row);
+        lse = -INFINITY, lo = 0, hi = 0;   // rows that are not there or see nothing give no weight
+        if (tok < it.s.n) {
+          lse = p.lse[(size_t)(it.s.first + tok) * p.q_heads + it.head * p.group + row - tok * p.group];
+          sees(p, it.s, tok, lo, hi);
         }
       };
       fetch(0);
       for (int blk = 0; blk < blocks; ++blk, ++n) {
         const int st = n % G::kStages;
         if (!wait(G::bQEmpty + st, n / G::kStages + 1)) return false;
-        const int row0 = (it.block0 + from + blk) * 128 + w * 16;
         float* consts = reinterpret_cast<float*>(smem + G::kConstOff) + st * 512 + w * 16;
+        uint8_t* q_block = smem + G::kQOff + st * G::kQBytes + (c / 8) * 128 * 128;
+        const float fac0 = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
+        auto store = [&](auto bf16) {
+#pragma unroll 1
+          for (int k0 = 0;;) {
+            float fac[PRE];
 #pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          const int r = k * RPI + lane / LPR;
-          float fac = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
-          normalize_query8<LPR>(v[k], p.bf16, sign, fac);
-          const int rr = w * 16 + r;
-          *reinterpret_cast<uint4*>(smem + G::kQOff + st * G::kQBytes + (c / 8) * 128 * 128 + rr * 128 +
-                                    (((c & 7) ^ (rr & 7)) << 4)) = v[k];
-          if (c == 0) {
-            const int tok = p.by_group(row0 + r);
-            int lo = 0, hi = 0;
-            if (tok < it.s.n) sees(p, it.s, tok, lo, hi);
-            // rows that are not there or see nothing give no weight
-            consts[r] = fac, consts[128 + r] = lse[k] == -INFINITY ? -INFINITY : -lse[k] * kLog2e;
-            consts[256 + r] = __int_as_float(lo), consts[384 + r] = __int_as_float(hi);
+            for (int k = 0; k < PRE; ++k) {
+              fac[k] = fac0;
+              normalize_query8<LPR>(v[k], bf16(), sign, fac[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < PRE; ++k) {
+              const int r = (k0 + k) * RPI + lane / LPR, rr = w * 16 + r;
+              *reinterpret_cast<uint4*>(q_block + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[k];
+              if (c == 0) consts[r] = fac[k];
+            }
+            if ((k0 += PRE) >= NI) break;
+            load((it.block0 + from + blk) * 128 + w * 16, k0);
           }
+        };
+        if (p.bf16)
+          store(std::true_type());
+        else
+          store(std::false_type());
+        if (lane < 16) {
+          consts[128 + lane] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+          consts[256 + lane] = __int_as_float(lo), consts[384 + lane] = __int_as_float(hi);
         }
         fence_proxy_async_shared();
         __syncwarp();
