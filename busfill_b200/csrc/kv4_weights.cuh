@@ -349,17 +349,18 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
     for_pieces([&](const Item& it, int from, int blocks, int u) {
       const int base = (it.tile0 + it.t) * G::kTokens + i * 128 + 32 * q, slot = base + lane;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      // rows of a block that every token of the warp is seen by, and rows at the edge
       for (int blk = 0; blk < blocks && ok; ++blk, ++n) {
         const int st = n % G::kStages;
         if (!wait(G::bS + st, n / G::kStages)) break;
         tc_fence_after();
         const float* consts = reinterpret_cast<const float*>(smem + G::kConstOff) + st * 512;
-        // the block's first row ends first, its last row begins last
+        // all rows of the block see the warp's tokens: its first row ends first, its last row begins last
         const int r1 = min((it.block0 + from + blk) * 128 + 127, it.s.n * p.group - 1) - (it.block0 + from + blk) * 128;
         const bool whole = base + 32 <= __float_as_int(consts[384]) && base >= __float_as_int(consts[256 + r1]);
+        // none does: its last row ends last, its first row begins first
+        const bool none = base >= __float_as_int(consts[384 + r1]) || base + 32 <= __float_as_int(consts[256]);
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
+        for (int c = none ? 128 : 0; c < 128; c += 32) {
           float s[32];
           tmem_ld_x32(tm + (st * TT + i) * 128 + c, reinterpret_cast<uint32_t*>(s));
           tc_wait_ld();
