@@ -15,7 +15,7 @@
 // the ranges.
 //
 // Warps: 0 issues the MMAs and owns TMEM; 4-7 and 8-11 add up, thread = token;
-// 12-19 bring keys and queries as fp16 operands.
+// 12-27 bring keys and queries as fp16 operands.
 #pragma once
 
 #include "kv4_prompt.cuh"
@@ -24,8 +24,8 @@ namespace busfill {
 namespace kv4 {
 namespace wsum {
 
-constexpr int kThreads = 640;
-constexpr int kLoadWarps = 8, kLoadWarp0 = 12;
+constexpr int kThreads = 896;
+constexpr int kLoadWarps = 16, kLoadWarp0 = 12;
 
 template <int D>
 struct Geo {
@@ -37,8 +37,8 @@ struct Geo {
   static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kStages = 2;                        // query blocks, each with its S^T in TMEM
   static constexpr int kKeyOff = 0, kQOff = kKeyBufs * kKeyBytes;
-  static constexpr int kConstOff = kQOff + kStages * kQBytes;   // [factor, -lse2, first slot, slot behind the last][row]
-  static constexpr int kBarOff = kConstOff + kStages * 128 * 16;
+  static constexpr int kConstOff = kQOff + kStages * kQBytes;   // [factor, -lse2][row]
+  static constexpr int kBarOff = kConstOff + kStages * 128 * 8;
   static constexpr int bKFull = 0, bKEmpty = bKFull + kKeyBufs, bQFull = bKEmpty + kKeyBufs,
                        bQEmpty = bQFull + kStages, bS = bQEmpty + kStages, bFinal = bS + kStages, kBars = bFinal + 1;
   static constexpr int kMiscOff = kBarOff + kBars * 8;
@@ -240,9 +240,9 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
       if (!wait(G::bKEmpty + kb, item / G::kKeyBufs + 1)) return false;
       uint8_t* dst = smem + G::kKeyOff + kb * G::kKeyBytes;
       const int base = (it.tile0 + it.t) * G::kTokens;
-#pragma unroll 2
-      for (int pass = 0; pass < G::kTokens / 64; ++pass) {
-        const int tok = pass * 64 + w * 8 + (lane >> 2);   // a pass is a page
+#pragma unroll
+      for (int pass = 0; pass < G::kTokens / (8 * wsum::kLoadWarps); ++pass) {
+        const int tok = (pass * wsum::kLoadWarps + w) * 8 + (lane >> 2);
         uint32_t x[NB], sc[NB / 2];
 #pragma unroll
         for (int b = 0; b < NB; ++b) x[b] = 0;
@@ -267,68 +267,54 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(G::bKFull + kb));
       ++item;
-      // A block's rows are on their way while its stage is still in use (the
-      // first PRE of a lane's); lane r holds the constants of the warp's row r.
-      constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI, PRE = NI < 8 ? NI : 8;
+      // A block's rows are on their way while its stage is still in use; lane r
+      // holds the constants of the warp's row r.
+      constexpr int LPR = D / 8, RPI = 32 / LPR, NR = 128 / wsum::kLoadWarps, NI = NR / RPI;
       const int c = lane % LPR;
-      uint4 v[PRE];
+      uint4 v[NI];
       float lse;
-      int lo, hi;
-      auto load = [&](int row0, int k0) {
+      auto fetch = [&](int blk) {
+        const int row0 = (it.block0 + from + blk) * 128 + w * NR;
 #pragma unroll
-        for (int k = 0; k < PRE; ++k) {
-          const int row = row0 + (k0 + k) * RPI + lane / LPR, tok = p.by_group(row);
+        for (int k = 0; k < NI; ++k) {
+          const int row = row0 + k * RPI + lane / LPR, tok = p.by_group(row);
           v[k] = make_uint4(0, 0, 0, 0);
           if (tok < it.s.n)
             v[k] = __ldg(reinterpret_cast<const uint4*>(
                 static_cast<const uint16_t*>(p.q) + (size_t)(it.s.first + tok) * p.q_token +
                 (size_t)(it.head * p.group + row - tok * p.group) * p.q_head + 8 * c));
         }
-      };
-      auto fetch = [&](int blk) {
-        const int row0 = (it.block0 + from + blk) * 128 + w * 16;
-        load(row0, 0);
-        const int row = row0 + (lane & 15), tok = p.by_group(row);
-        lse = -INFINITY, lo = 0, hi = 0;   // rows that are not there or see nothing give no weight
-        if (tok < it.s.n) {
+        const int row = row0 + lane % NR, tok = p.by_group(row);
+        lse = -INFINITY;   // rows that are not there or see nothing give no weight
+        if (tok < it.s.n)
           lse = p.lse[(size_t)(it.s.first + tok) * p.q_heads + it.head * p.group + row - tok * p.group];
-          sees(p, it.s, tok, lo, hi);
-        }
       };
       fetch(0);
       for (int blk = 0; blk < blocks; ++blk, ++n) {
         const int st = n % G::kStages;
         if (!wait(G::bQEmpty + st, n / G::kStages + 1)) return false;
-        float* consts = reinterpret_cast<float*>(smem + G::kConstOff) + st * 512 + w * 16;
+        float* consts = reinterpret_cast<float*>(smem + G::kConstOff) + st * 256 + w * NR;
         uint8_t* q_block = smem + G::kQOff + st * G::kQBytes + (c / 8) * 128 * 128;
         const float fac0 = fmaxf(fabsf(p.scale_log2), 1e-30f);   // -inf * fac stays -inf
         auto store = [&](auto bf16) {
-#pragma unroll 1
-          for (int k0 = 0;;) {
-            float fac[PRE];
+          float fac[NI];
 #pragma unroll
-            for (int k = 0; k < PRE; ++k) {
-              fac[k] = fac0;
-              normalize_query8<LPR>(v[k], bf16(), sign, fac[k]);
-            }
+          for (int k = 0; k < NI; ++k) {
+            fac[k] = fac0;
+            normalize_query8<LPR>(v[k], bf16(), sign, fac[k]);
+          }
 #pragma unroll
-            for (int k = 0; k < PRE; ++k) {
-              const int r = (k0 + k) * RPI + lane / LPR, rr = w * 16 + r;
-              *reinterpret_cast<uint4*>(q_block + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[k];
-              if (c == 0) consts[r] = fac[k];
-            }
-            if ((k0 += PRE) >= NI) break;
-            load((it.block0 + from + blk) * 128 + w * 16, k0);
+          for (int k = 0; k < NI; ++k) {
+            const int r = k * RPI + lane / LPR, rr = w * NR + r;
+            *reinterpret_cast<uint4*>(q_block + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[k];
+            if (c == 0) consts[r] = fac[k];
           }
         };
         if (p.bf16)
           store(std::true_type());
         else
           store(std::false_type());
-        if (lane < 16) {
-          consts[128 + lane] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
-          consts[256 + lane] = __int_as_float(lo), consts[384 + lane] = __int_as_float(hi);
-        }
+        if (lane < NR) consts[128 + lane] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(G::bQFull + st));
@@ -347,18 +333,22 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
     float* my_part = p.part + (size_t)blockIdx.x * 2 * G::kTokens;
     uint32_t n = 0;
     for_pieces([&](const Item& it, int from, int blocks, int u) {
-      const int base = (it.tile0 + it.t) * G::kTokens + i * 128 + 32 * q, slot = base + lane;
+      const int slot = (it.tile0 + it.t) * G::kTokens + mine;
+      // the rows that see the thread's token: [row_a, row_z)
+      const long long at = slot - (it.s.len - it.s.n);   // the row that stands at it
+      const int row_a = p.causal ? (int)max(0ll, min(at, (long long)it.s.n)) * p.group : 0;
+      const int row_z = slot >= it.s.len ? 0
+                        : p.window > 0   ? (int)max(0ll, min(at + p.window, (long long)it.s.n)) * p.group
+                                         : it.s.n * p.group;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int blk = 0; blk < blocks && ok; ++blk, ++n) {
         const int st = n % G::kStages;
         if (!wait(G::bS + st, n / G::kStages)) break;
         tc_fence_after();
-        const float* consts = reinterpret_cast<const float*>(smem + G::kConstOff) + st * 512;
-        // all rows of the block see the warp's tokens: its first row ends first, its last row begins last
-        const int r1 = min((it.block0 + from + blk) * 128 + 127, it.s.n * p.group - 1) - (it.block0 + from + blk) * 128;
-        const bool whole = base + 32 <= __float_as_int(consts[384]) && base >= __float_as_int(consts[256 + r1]);
-        // none does: its last row ends last, its first row begins first
-        const bool none = base >= __float_as_int(consts[384 + r1]) || base + 32 <= __float_as_int(consts[256]);
+        const float* consts = reinterpret_cast<const float*>(smem + G::kConstOff) + st * 256;
+        const int row0 = (it.block0 + from + blk) * 128, a = row_a - row0, z = row_z - row0;
+        const bool whole = __all_sync(0xffffffffu, a <= 0 && z >= min(128, it.s.n * p.group - row0));
+        const bool none = __all_sync(0xffffffffu, z <= 0 || a >= 128);
 #pragma unroll 1
         for (int c = none ? 128 : 0; c < 128; c += 32) {
           float s[32];
@@ -366,14 +356,7 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
           tc_wait_ld();
           if (!whole) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 lo = *reinterpret_cast<const float4*>(consts + 256 + c + k),
-                           hi = *reinterpret_cast<const float4*>(consts + 384 + c + k);
-              s[k] = slot >= __float_as_int(lo.x) && slot < __float_as_int(hi.x) ? s[k] : -INFINITY;
-              s[k + 1] = slot >= __float_as_int(lo.y) && slot < __float_as_int(hi.y) ? s[k + 1] : -INFINITY;
-              s[k + 2] = slot >= __float_as_int(lo.z) && slot < __float_as_int(hi.z) ? s[k + 2] : -INFINITY;
-              s[k + 3] = slot >= __float_as_int(lo.w) && slot < __float_as_int(hi.w) ? s[k + 3] : -INFINITY;
-            }
+            for (int k = 0; k < 32; ++k) s[k] = c + k >= a && c + k < z ? s[k] : -INFINITY;
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
