@@ -52,15 +52,31 @@ bool raise_smem(Kernel kernel, int bytes, int dev, std::once_flag (&once)[64], c
   return err[dev & 63] == cudaSuccess;
 }
 
-// Query rows of the widest sequence and head from which the tcgen05 kernel
-// takes the call.
-constexpr int kPromptRows = 33;
+// The tcgen05 kernel takes a call whose widest sequence has this many query
+// rows per key/value head, if the call has kPromptTotal rows in all. Us of
+// attn_kernel / prompt_kernel, 8 sequences of 4096 tokens and 8 heads of 128:
+// 32 rows 49 / 57, 40 rows 58 / 57, 96 rows 105 / 57; heads of 64: 48 rows
+// 41 / 47, 64 rows 47 / 47, 96 rows 59 / 47; 4 heads of 256: 32 rows 64 / 67,
+// 40 rows 72 / 68. One sequence, 8 heads of 128: 48 rows (384 in all) 25 / 39
+// at 4096 tokens; 64 (512) 70 / 76 at 32000; 128 (1024) 33 / 40 and 121 / 76.
+constexpr int prompt_rows(int head_dim) { return head_dim == 64 ? 57 : 37; }
+constexpr long long kPromptTotal = 640;
+
+// Query rows from which the weights' second pass goes to tcgen05. Us of
+// weights_kernel / weights_prompt_kernel, 8 sequences of 4096 tokens, 8 heads
+// of 128: 24 rows 27 / 35, 32 rows 35 / 36, 40 rows 42 / 37, 96 rows 88 / 38;
+// heads of 64: 32 rows 24 / 33, 48 rows 31 / 32, 64 rows 43 / 34; one sequence
+// of 512: 16 rows 13 / 15, 32 rows 16 / 15, 64 rows 26 / 15.
+constexpr int kWeightsRows = 33;
 
 constexpr long long kMaxGrid = 2147483647;
 
 // Query rows of the widest sequence and head from which two row tiles share a
-// warp's pass over the pages.
-constexpr int kTwoTileRows = 9;
+// warp's pass over the pages, heads of 64 only. Us with one / two, 32 sequences
+// of 1024 tokens, 8 heads of 64: 8 rows 25 / 29, 24 rows 32 / 35, 32 rows
+// 38 / 35, 48 rows 46 / 43. Wider heads have no registers for it (8 sequences
+// of 4096, heads of 128: 32 rows 49 / 68).
+constexpr int kTwoTileRows = 25;
 
 // Workspace of the attention calls on a stream: a counter per CTA, then the
 // largest kernel's partial results.
@@ -68,7 +84,6 @@ constexpr size_t kCounterBytes = 4096;
 size_t workspace_bytes(int sms) {
   size_t f = part_floats<64, 2>();
   f = std::max(f, part_floats<128, 1>());
-  f = std::max(f, part_floats<128, 2>());
   f = std::max(f, part_floats<256, 1>());
   f = std::max(f, (size_t)2 * prompt::Geo<64>::kPartFloats);
   f = std::max(f, (size_t)2 * prompt::Geo<128>::kPartFloats);
@@ -272,16 +287,17 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
   p.error = ctx.error;
   if (ctx.sms > (int)(kCounterBytes / 4)) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
-  const bool many = p.max_q * p.group >= kPromptRows, two = p.max_q * p.group >= kTwoTileRows;
+  const int rows = p.max_q * p.group;
   st = by_dim(cache->head_dim, [&](auto d) {
-    if (many) return launch_prompt<d()>(p, ctx, s);
-    if constexpr (d() < 256) {
-      if (two) return launch_attn<d(), 2>(p, ctx, s);
+    if (rows >= prompt_rows(d()) && (long long)p.tokens * p.q_heads >= kPromptTotal)
+      return launch_prompt<d()>(p, ctx, s);
+    if constexpr (d() == 64) {
+      if (rows >= kTwoTileRows) return launch_attn<d(), 2>(p, ctx, s);
     }
     return launch_attn<d(), 1>(p, ctx, s);
   });
   if (st != BUSFILL_OK || !a->weights) return st;
-  return by_dim(cache->head_dim, [&](auto d) { return launch_weights<d()>(p, ctx, s, many); });
+  return by_dim(cache->head_dim, [&](auto d) { return launch_weights<d()>(p, ctx, s, rows >= kWeightsRows); });
 }
 
 int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, void* stream) {

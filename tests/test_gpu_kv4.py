@@ -309,6 +309,23 @@ def test_prompts(dim, group, new, length, window, dtype):
             seed=new + (dtype == "bf16"))
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 1), (True, 50), (True, 300)])
+def test_prompts_ragged_masks_and_empty_rows(dim, causal, window):
+    # the first case's masks, with rows enough for the kernel of many rows
+    lens = [0, 300, 31, 190, 65, 400]
+    new = [70, 0, 64, 190, 64, 20]
+    _attend(lens, new, 12, 2, dim, "bf16" if window else "fp16", causal, window, seed=7 * window + dim)
+
+
+@pytest.mark.parametrize("dim,new,lens,window", [
+    (128, 100, [9000], 0), (128, 40, [5000, 300, 7000], 0), (64, 70, [12000], 3000), (256, 60, [4000, 4100], 0),
+])
+def test_rows_on_a_long_cache_are_split_and_joined(dim, new, lens, window):
+    sample = [(0, 0), (len(lens) - 1, 1)]
+    _attend(lens, [new] * len(lens), 8, 2, dim, "bf16", window=window, seed=dim + new, sample=sample)
+
+
 def test_long_cache_is_split_and_joined():
     sample = [(0, 0), (0, 3), (1, 1)]
     _attend([70001, 33000], [1, 1], 32, 4, 128, "fp16", seed=4, sample=sample)
