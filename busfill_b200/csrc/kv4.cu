@@ -179,9 +179,13 @@ int busfill_rope_axes(const busfill_rope* r, void* stream) {
   const int pairs = vec ? (r->adjacent ? 4 : 8) : 1;
   const int pieces = half / pairs + (r->head_dim - r->rot) / (vec ? 8 : 1);
   const int heads = r->q_heads + r->k_heads;
-  // heads of one thread: as many as leave enough threads for the device
+  // Heads of one thread: as many as leave an SM 256 threads. Us with 1 / 2 / 4 /
+  // 8, 64 + 8 heads of 128, event times of about 8 us more than the kernel's:
+  // 32 tokens 8 / 10 / 10 / 12, 256 tokens 14 / 10 / 12 / 14, 512 tokens
+  // 21 / 16 / 12 / 14, 1024 tokens 33 / 25 / 18 / 16, 8192 tokens 217 / 145 /
+  // 94 / 80.
   int per = 8;
-  while (per > 1 && (long long)r->tokens * pieces * ((heads + per - 1) / per) < (long long)ctx.sms * 2048) per /= 2;
+  while (per > 1 && (long long)r->tokens * pieces * ((heads + per - 1) / per) < (long long)ctx.sms * 256) per /= 2;
   p.heads_per_thread = per;
   p.groups = (heads + per - 1) / per;
   const long long blocks = ((long long)r->tokens * pieces * p.groups + 255) / 256;
@@ -214,9 +218,12 @@ int busfill_kv4_append(const busfill_kv4* cache, const busfill_kv4_rows* r, void
   p.tokens = r->tokens;
   p.vec = aligned(r->k, 16) && aligned(r->v, 16) && (r->k_token | r->k_head | r->v_token | r->v_head) % 8 == 0;
   p.error = ctx.error;
-  // four groups a lane where that leaves every scheduler two warps
+  // Four groups a lane where one would make more than 128 warps an SM. Us with
+  // one / four (event times, some 8 us more than the kernel's), 8 heads of 128:
+  // 512 tokens 8 / 10, 2048 tokens 14 / 14, 4096 tokens 21 / 18, 8192 tokens
+  // 33 / 29; 4 heads of 64: 4096 tokens 10 / 12.
   const int groups = (2 * cache->heads * (cache->head_dim / 8) + 31) / 32;
-  const bool four = (long long)p.tokens * groups >= (long long)ctx.sms * 32;
+  const bool four = (long long)p.tokens * groups >= (long long)ctx.sms * 128;
   p.chunks = four ? (groups + 3) / 4 : groups;
   const long long blocks = ((long long)p.tokens * p.chunks + 7) / 8;
   if (blocks > kMaxGrid / 8) return BUSFILL_ERR_SHAPE;   // the kernel counts warps in an int
@@ -281,7 +288,8 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.tokens = a->tokens, p.q_heads = a->q_heads, p.group = a->q_heads / cache->heads;
   p.by_group = divide_by((unsigned)p.group);
   p.max_q = a->q_start ? a->max_q : 1;
-  p.causal = a->causal != 0, p.window = a->window, p.bf16 = a->dtype == BUSFILL_TYPE_BF16;
+  // a window as long as the table can hold is none (and stays clear of the end of int)
+  p.causal = a->causal != 0, p.window = a->window < (int64_t)kPage * cache->table_cols ? a->window : 0, p.bf16 = a->dtype == BUSFILL_TYPE_BF16;
   p.wide_out = aligned(a->out, 32) && (a->out_token | a->out_head) % 16 == 0;
   p.counters = static_cast<unsigned*>(work);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
@@ -333,7 +341,8 @@ int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, v
     if (in_place)
       return host::launch((const void*)evict_move_kernel<d(), true>, dim3((unsigned)rows),
                           dim3(MoveGeo<d(), true>::kThreads), 0, s, margs);
-    // enough CTAs to fill the device, as far as there are tokens
+    // Eight CTAs an SM, as far as there are tokens (select and move of 64 rows
+    // of 32000 weights, keep 8000: two an SM 102 us, four 80, eight 80, 32 80).
     using G = MoveGeo<d(), false>;
     per = std::max(1, std::min((e->keep + G::kTokens - 1) / G::kTokens, (ctx.sms * 8 + rows - 1) / rows));
     return host::launch((const void*)evict_move_kernel<d(), false>, dim3((unsigned)(rows * per)), dim3(G::kThreads), 0,

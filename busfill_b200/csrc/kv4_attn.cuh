@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   // CTAs that share the list: every one gets a unit; where a warp would get
   // two pages at most, no more than there are items, as a split item has to
   // be joined through the workspace (one sequence of 300 tokens, 8 heads: 8
-  // CTAs of 5 pages, 8.6 us, against 40 of one page and 5 parts an item, 11 us)
+  // CTAs of 5 pages, 9.6 us, against 40 of one page and 5 parts an item, 12.1 us)
   const long long ctas = min((int)gridDim.x, max(min(items, T), (T + 2 * W - 1) / (2 * W)));
   if ((int)blockIdx.x >= ctas) {
     if (bad) atomicOr(p.error, kErrIndex);

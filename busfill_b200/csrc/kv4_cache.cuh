@@ -141,8 +141,8 @@ __device__ __forceinline__ float2 to_floats(__nv_bfloat162 x) { return __bfloat1
 // Quantizes the 8 channels of one lane (16-bit pairs u), whose block's other
 // 24 are on the lanes j ^ 1, j ^ 2, j ^ 3 (j = lane % 4 is the place in the
 // block). Returns the code word in key order and the block's scale. Pairs are
-// worked on together where there are instructions for it: counted per element
-// the plain form took 40 instructions, this takes 16.
+// worked on together where there are instructions for it (an append of 7814
+// tokens, 8 heads of 128: 36 us element by element, 24 in pairs).
 template <typename T>
 __device__ __forceinline__ uint32_t quantize8(const uint32_t* u, int j, __half& scale) {
   using Pair = decltype(pair_of(T(), 0u));
@@ -209,8 +209,10 @@ __device__ __forceinline__ uint32_t quantize8(const uint32_t* u, int j, __half& 
 
 // One lane takes 8 channels of a key or value row (word j of block b), GROUPS
 // times. Its elements are on their way before the token's place in the cache
-// is looked up, a chain of four small loads that would otherwise set the time
-// (16000 tokens x 8 heads of 128: 33 us, 13 with both).
+// is looked up, a chain of four small loads that would otherwise set the time.
+// Bound: 2 D bytes read and 9/16 D written a row, 73 MB and 11 us for 7814
+// tokens and 8 heads of 128; measured 24 us, where the arithmetic of the
+// quantization is what is left (33 us before its loads came first).
 template <int D, typename T, int GROUPS>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   using F = Fmt<D>;

@@ -338,6 +338,16 @@ def test_many_short_sequences():
     _attend(lens, [1] * 300, 16, 2, 128, "fp16", seed=6, sample=[(i, i % 2) for i in range(0, 300, 13)])
 
 
+@pytest.mark.parametrize("new", [1, 70])
+def test_a_window_longer_than_the_cache_is_none(new):
+    b, q, out, lse, w = _attend([200, 90], [new] * 2, 16, 2, 128, "fp16", window=0, seed=30 + new)
+    w2, w3 = _torch().zeros_like(w), _torch().zeros_like(w)
+    y = bf.attn_kv4(q, b.pages, b.table, b.kv_len, q_start=b.starts([new] * 2), max_q=new, weights=w2)
+    z = bf.attn_kv4(q, b.pages, b.table, b.kv_len, q_start=b.starts([new] * 2), max_q=new, weights=w3, window=2**31 - 1)
+    t = _torch()
+    assert t.equal(y, out) and t.equal(z, out) and t.equal(w2, w3) and float(w3.sum()) > 0.99 * new * 32
+
+
 @pytest.mark.parametrize("qscale", [2.0 ** -12, 30.0, 3000.0])
 def test_query_magnitudes(qscale):
     # tiny (all tokens nearly alike), sharp, and one-hot rows
