@@ -378,48 +378,50 @@ __device__ __forceinline__ unsigned weight_key(float w) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectKeys = 40960;   // weights that are held in shared memory at a time
-constexpr int kSelectBytes = kSelectKeys * 4 + 2048 * 4;
+constexpr int kSelectRows = kSelectKeys / 32;   // of 32 weights; a mask of ties and one of those that stay for each
+constexpr int kSelectBytes = kSelectKeys * 4 + 2 * kSelectRows * 4;
+static_assert(2 * kSelectRows >= 2048, "the histogram lies where the masks do");
 
-// Exclusive sum of x over the CTA's threads; total of all in `total`.
-__device__ __forceinline__ unsigned block_sum(unsigned x, unsigned* sums, unsigned& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned run = x;
+// Inclusive sum over the lanes.
+__device__ __forceinline__ unsigned warp_sum(unsigned x) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const unsigned y = __shfl_up_sync(0xffffffffu, run, m);
-    if (lane >= m) run += y;
+    const unsigned y = __shfl_up_sync(0xffffffffu, x, m);
+    if (lane >= m) x += y;
   }
-  __syncthreads();   // `sums` may still be read from the last time
+  return x;
+}
+// Exclusive sum of x over the CTA's 32 warps of threads.
+__device__ __forceinline__ unsigned block_sum(unsigned x, unsigned* sums) {
+  static_assert(kSelectThreads == 1024, "a lane per warp");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned run = warp_sum(x);
   if (lane == 31) sums[warp] = run;
   __syncthreads();
-  unsigned before = 0;
-  total = 0;
-#pragma unroll 8
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    const unsigned y = sums[w];
-    before += w < warp ? y : 0;
-    total += y;
-  }
-  return before + run - x;
+  const unsigned y = sums[lane];
+  return __shfl_sync(0xffffffffu, warp_sum(y) - y, warp) + run - x;
 }
 
 // Which tokens stay: one CTA per sequence and head. The (keep - recent)-th
 // largest key is found digit by digit (11, 11 and 10 bits, a shared histogram
 // each: wide digits spread weights of like size over many counters); then one
-// ordered pass writes the kept slots, every thread a run of them. Among the
-// tokens with exactly that key the lower slots win. The weights sit in shared
-// memory; of longer sequences the histograms read them from global memory and
-// the ordered pass goes part by part.
+// ordered pass writes the kept slots, every warp a run of them, 32 at a time:
+// ballots count and place them, so neighbouring lanes write neighbouring
+// entries (a run per thread scattered its stores: 8 us of 31 for 64 rows of
+// 32000). Among the tokens with exactly that key the lower slots win. The
+// weights sit in shared memory; of longer sequences the histograms read them
+// from global memory and the ordered pass goes part by part.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
   extern __shared__ unsigned select_smem[];
   float* held = reinterpret_cast<float*>(select_smem);
   unsigned* hist = select_smem + kSelectKeys;
-  __shared__ unsigned sums[32];
+  __shared__ unsigned sums[32], part_ties[32], part_stays[32];
   __shared__ unsigned pick[2];   // digit, keys still to find
   pdl_wait_prerequisites();
   pdl_launch_dependents();
   const int b = blockIdx.x / p.c.heads, h = blockIdx.x - b * p.c.heads;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   bool bad = false;
   const int len = cached(p.c, b, bad);
   if (bad && tid == 0) atomicOr(p.error, kErrIndex);
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   int* index = p.index + row * p.keep;
   const bool fits = len <= kSelectKeys;
   if (fits) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid; i < len; i += kSelectThreads) held[i] = w[i];
   }
   const float* keys = fits ? held : w;
@@ -451,8 +453,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       // the digit where the count from above reaches `left`: two digits a thread
       const int top = bins - 1 - 2 * tid;
       const unsigned n0 = top > 0 ? hist[top] : 0, n1 = top > 0 ? hist[top - 1] : 0;
-      unsigned total;
-      const unsigned above = block_sum(n0 + n1, sums, total);
+      const unsigned above = block_sum(n0 + n1, sums);
       if (above < left && above + n0 + n1 >= left) {
         const bool second = above + n0 < left;
         pick[0] = (unsigned)(second ? top - 1 : top);
@@ -467,7 +468,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   }
   // `left` tokens of key == edge and all of key > edge stay (need == old:
   // everything stays; need == 0: nothing); what is written has been read
-  const bool all = need >= old;
+  if (need == 0) edge = 0xffffffffu;   // no key is as large
+  const int sure = need >= old ? 0 : old;   // from here on all stay
+  unsigned* masks = hist;
   unsigned at = 0, ties = 0;   // kept, and ties met, in earlier parts
   for (int base = 0; base < len; base += kSelectKeys) {
     const int n = min(kSelectKeys, len - base);
@@ -475,36 +478,42 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     if (!fits)
       for (int i = tid; i < n; i += kSelectThreads) held[i] = w[base + i];
     __syncthreads();
-    // an odd run of slots per thread: the threads of a warp read different banks
-    const int run = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
-    const int i0 = min(n, tid * run), i1 = min(n, i0 + run);
-    auto kind = [&](int i) -> int {   // 0 goes, 1 stays, 2 tie
-      if (base + i >= old || all) return 1;
-      if (need == 0) return 0;
-      const unsigned key = weight_key(held[i]);
-      return key > edge ? 1 : key == edge ? 2 : 0;
-    };
-    unsigned mine = 0, stays = 0;   // ties, kept above them
-    for (int i = i0; i < i1; ++i) {
-      const int k = kind(i);
-      mine += k == 2;
-      stays += k == 1;
+    const int run = (n + kSelectThreads - 1) / kSelectThreads * 32, i0 = min(n, warp * run), i1 = min(n, i0 + run);
+    unsigned mine = 0, stays = 0;   // of the warp's run: ties, kept above them
+#pragma unroll 4
+    for (int i = i0; i < i1; i += 32) {
+      const unsigned key = i + lane < i1 ? weight_key(held[i + lane]) : 0;
+      const bool out = i + lane >= i1, last = base + i + lane >= sure;
+      const unsigned tie = __ballot_sync(0xffffffffu, !out && !last && key == edge),
+                     stay = __ballot_sync(0xffffffffu, !out && (last || key > edge));
+      if (lane == 0) masks[i / 32] = tie, masks[kSelectRows + i / 32] = stay;
+      mine += __popc(tie);
+      stays += __popc(stay);
     }
-    unsigned all_ties, all_kept;
-    unsigned rank = ties + block_sum(mine, sums, all_ties);
-    // ties of rank < left stay
-    const unsigned tied = rank < left ? min(mine, left - rank) : 0;
-    unsigned to = at + block_sum(stays + tied, sums, all_kept);
-    for (int i = i0; i < i1; ++i) {
-      const int k = kind(i);
-      if (k == 1 || (k == 2 && rank++ < left)) {
-        index[to] = base + i;
-        wo[to] = held[i];
-        ++to;
+    if (lane == 0) part_ties[warp] = mine, part_stays[warp] = stays;
+    __syncthreads();
+    // a lane per warp: ties before its run, those that stay (rank < left), where its run goes
+    const unsigned its = part_ties[lane], ties_to = ties + warp_sum(its), ties_from = ties_to - its;
+    const unsigned kept = part_stays[lane] + (ties_from < left ? min(its, left - ties_from) : 0);
+    const unsigned kept_to = at + warp_sum(kept);
+    unsigned rank = __shfl_sync(0xffffffffu, ties_from, warp);
+    unsigned to = __shfl_sync(0xffffffffu, kept_to - kept, warp);
+    ties = __shfl_sync(0xffffffffu, ties_to, 31);
+    at = __shfl_sync(0xffffffffu, kept_to, 31);
+    const unsigned below = (1u << lane) - 1;
+#pragma unroll 4
+    for (int i = i0; i < i1; i += 32) {
+      const unsigned tied = masks[i / 32], above = masks[kSelectRows + i / 32], me = 1u << lane;
+      const bool stay = (above & me) || ((tied & me) && rank + __popc(tied & below) < left);
+      const unsigned staying = tied ? __ballot_sync(0xffffffffu, stay) : above;
+      if (stay) {
+        const unsigned x = to + __popc(staying & below);
+        index[x] = base + i + lane;
+        wo[x] = held[i + lane];
       }
+      rank += __popc(tied);
+      to += __popc(staying);
     }
-    ties += all_ties;
-    at += all_kept;
   }
   for (int i = keep + tid; i < p.keep; i += kSelectThreads) index[i] = -1;
   __syncthreads();

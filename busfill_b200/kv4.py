@@ -68,12 +68,13 @@ def _packer(cls):
 
 _pack_cache, _pack_rope, _pack_rows, _pack_attn, _pack_eviction = map(_packer, (Cache, Rope, Rows, Attn, Eviction))
 _TYPE = {}   # torch dtype -> BUSFILL_TYPE_*; filled with torch's dtypes at the first call
-_U8 = _I32 = _F32 = _F16 = _raw_stream = None
+_U8 = _I32 = _F32 = _F16 = _raw_stream = _empty_like = _contiguous = None
 
 
 def _init():
-    global _U8, _I32, _F32, _F16, _raw_stream
+    global _U8, _I32, _F32, _F16, _raw_stream, _empty_like, _contiguous
     torch = _torch()
+    _empty_like, _contiguous = torch.empty_like, torch.contiguous_format
     _U8, _I32, _F32, _F16 = torch.uint8, torch.int32, torch.float32, torch.float16
     _raw_stream = torch._C._cuda_getCurrentRawStream
     _TYPE.update({torch.float16: 1, torch.bfloat16: 30})
@@ -161,6 +162,14 @@ def _raw(stream, like):
     return stream.cuda_stream
 
 
+def _another(stream, like):
+    """A contiguous tensor of like's shape and type that belongs to the call's stream."""
+    if stream is None:
+        return _empty_like(like, memory_format=_contiguous)
+    with _torch().cuda.stream(stream):
+        return _empty_like(like, memory_format=_contiguous)
+
+
 def _empty(stream, like, shape, dtype):
     """A tensor on like's device that belongs to the call's stream."""
     if stream is None:
@@ -217,7 +226,7 @@ def rope_axes(q, k, positions, cos, sin, axis=None, adjacent=False, inverse=Fals
     if half and max(axis) >= axes:
         raise ValueError(f"axis entries must be in 0..{axes - 1}")
     if q_out is None:
-        q_out = _empty(stream, q, shape, q.dtype)
+        q_out = _another(stream, q)
         qo_token, qo_head = heads * dim, dim
     else:
         qo_token, qo_head = _heads(q_out, "q_out", like=q)
@@ -230,7 +239,7 @@ def rope_axes(q, k, positions, cos, sin, axis=None, adjacent=False, inverse=Fals
         if n != tokens or k_dim != dim:
             raise ValueError(f"shape mismatch: q {tuple(shape)}, k {tuple(k.shape)}")
         if k_out is None:
-            k_out = _empty(stream, k, k.shape, k.dtype)
+            k_out = _another(stream, k)
             ko_token, ko_head = k_heads * dim, dim
         else:
             ko_token, ko_head = _heads(k_out, "k_out", like=q)
@@ -265,7 +274,8 @@ def kv4_read(pages, table, kv_len, q_start=None, tokens=None, stream=None):
     c, batch, heads, dim, _ = _cache(pages, table, kv_len)
     tokens = batch if tokens is None else int(tokens)
     start = _need_start(q_start, batch, tokens)
-    k, v = _empty(stream, pages, (2, tokens, heads, dim), _F16).unbind()
+    k = _empty(stream, pages, (tokens, heads, dim), _F16)
+    v = _another(stream, k)
     _check(_lib().busfill_kv4_read(c, start, tokens, k.data_ptr(), v.data_ptr(), _raw(stream, pages)),
            "busfill_kv4_read")
     return k, v
@@ -298,7 +308,7 @@ def attn_kv4(q, pages, table, kv_len, q_start=None, max_q=None, scale=None, caus
         if lse.shape != (tokens, heads):
             raise ValueError(f"lse must be [{tokens}, {heads}], got {tuple(lse.shape)}")
     if out is None:
-        out = _empty(stream, q, shape, q.dtype)
+        out = _another(stream, q)
         o_token, o_head = heads * dim, dim
     else:
         o_token, o_head = _heads(out, "out", like=q)
@@ -329,9 +339,9 @@ def kv4_evict(pages, table, kv_len, weights, keep, recent, out_table=None, weigh
     if rows != batch or out_cols * KV4_PAGE < keep:
         raise ValueError(f"out_table must be [{batch}, >= {-(-keep // KV4_PAGE)}], got {tuple(out_table.shape)}")
     index = _empty(stream, kv_len, (batch, heads, keep), _I32)
-    kv_len_out = _empty(stream, kv_len, (batch,), _I32)
+    kv_len_out = _another(stream, kv_len)
     if weights_out is None:
-        weights_out = _empty(stream, weights, weights.shape, _F32)
+        weights_out = _another(stream, weights)
         wo_ptr = weights_out.data_ptr()
     else:
         wo_ptr = _array(weights_out, _F32, "weights_out", 3)
