@@ -153,21 +153,25 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, const Span& s,
   const bool live = i < s.n;
   float x[NB][8];
   float top = 0.0f;
-  const size_t at = live ? (size_t)(s.first + i) * p.q_token + (size_t)(head * p.group + row - i * p.group) * p.q_head : 0;
+  const uint16_t* src = static_cast<const uint16_t*>(p.q) + (size_t)(s.first + i) * p.q_token +
+                        (size_t)(head * p.group + row - i * p.group) * p.q_head + 8 * j;
+  uint4 raw[NB];   // all loads before the first use: one latency, not one a block
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int ch = 32 * b + 8 * j;
-    if (!live) {
+    raw[b] = make_uint4(0, 0, 0, 0);
+    if (live) raw[b] = __ldg(reinterpret_cast<const uint4*>(src + 32 * b));
+  }
+  if (p.bf16) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[b][e] = 0.0f;
-    } else if (p.bf16) {
-      load8(static_cast<const __nv_bfloat16*>(p.q) + at + ch, true, x[b]);
-    } else {
-      load8(static_cast<const __half*>(p.q) + at + ch, true, x[b]);
-    }
+    for (int b = 0; b < NB; ++b) to_floats<__nv_bfloat16>(raw[b], x[b]);
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) to_floats<__half>(raw[b], x[b]);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[b][e]));
-  }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   // power of two that brings the row's maximum to [2^9, 2^10); none for 0 and
@@ -462,7 +466,7 @@ struct Geo {
   static constexpr int kItemOff = kMetaOff + 2 * 2 * kWarps * kRows * 4;   // the item of every piece
   static constexpr int kMiscOff = kItemOff + 2 * kWarps * 64;
   static constexpr int kBytes = kMiscOff + 512;
-  static_assert(kPieceFloats * 4 <= kRingBytes, "a piece fits the warp's ring");
+  static_assert(kPieceFloats * 4 <= kRingBytes && kPieceFloats % 4 == 0, "a piece fits the warp's ring");
   static_assert(kBytes <= 232448, "dynamic shared memory");
 };
 // workspace, per CTA: its two partial items
@@ -782,39 +786,49 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     auto theirs = [&](int i) {
       return p.part + (size_t)(first + i) * part_floats<D, NT>() + (size_t)(i == 0 ? 1 : 0) * PF;
     };
-    for (int task = warp; task < TASKS; task += W) {
-      const int x = task * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
-      float top = -INFINITY, sum = 0.0f;
-      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      // 16 parts in flight at a time; the reference moves with the parts
-      for (int i0 = 0; i0 < n; i0 += 16) {
-        float4 v[16];
-        float m[16], l[16];
+    // The parts come to shared memory (the rings are free now), as many as fit
+    // at a time: asynchronous copies keep all of them in flight with a short
+    // loop. The reference moves with the parts.
+    constexpr int FIT = W * G::kRingBytes / (PF * 4), EACH = (TASKS + W - 1) / W;
+    float top[EACH], sum[EACH];
+    float4 o[EACH];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float* from = theirs(min(i0 + i, n - 1));
-          v[i] = __ldcg(reinterpret_cast<const float4*>(from) + x);
-          m[i] = __ldcg(from + ROWS * D + row);
-          l[i] = __ldcg(from + ROWS * (D + 1) + row);
+    for (int t = 0; t < EACH; ++t) top[t] = -INFINITY, sum[t] = 0.0f, o[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i0 = 0; i0 < n; i0 += FIT) {
+      const int have = min(FIT, n - i0);
+      __syncthreads();
+#pragma unroll 1
+      for (int k = threadIdx.x; k < have * (PF / 4); k += W * 32)
+        cp_async16(smem_u32(smem) + 16 * k, theirs(i0 + k / (PF / 4)) + 4 * (k % (PF / 4)), true);
+      cp_async_wait_all();
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < EACH; ++t) {
+        const int x = (warp + t * W) * 32 + lane, row = x / QUADS;
+        if (warp + t * W >= TASKS) break;
+        const float* parts = reinterpret_cast<const float*>(smem);
+        float next = top[t];
+        for (int i = 0; i < have; ++i) next = fmaxf(next, parts[i * PF + ROWS * D + row]);
+        const float old = share(top[t], next);
+        sum[t] *= old;
+        o[t].x *= old, o[t].y *= old, o[t].z *= old, o[t].w *= old;
+        top[t] = next;
+#pragma unroll 2
+        for (int i = 0; i < have; ++i) {
+          const float4 v = reinterpret_cast<const float4*>(parts + i * PF)[x];
+          const float f = share(parts[i * PF + ROWS * D + row], next);
+          sum[t] = fmaf(parts[i * PF + ROWS * (D + 1) + row], f, sum[t]);
+          o[t].x = fmaf(v.x, f, o[t].x), o[t].y = fmaf(v.y, f, o[t].y), o[t].z = fmaf(v.z, f, o[t].z),
+          o[t].w = fmaf(v.w, f, o[t].w);
         }
-        float next = top;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) next = fmaxf(next, m[i]);
-        const float old = share(top, next);
-        sum *= old;
-        o.x *= old, o.y *= old, o.z *= old, o.w *= old;
-        top = next;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (i0 + i < n) {
-            const float f = share(m[i], top);
-            sum = fmaf(l[i], f, sum);
-            o.x = fmaf(v[i].x, f, o.x), o.y = fmaf(v[i].y, f, o.y), o.z = fmaf(v[i].z, f, o.z),
-            o.w = fmaf(v[i].w, f, o.w);
-          }
       }
-      store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o, sum == 0.0f ? 0.0f : 1.0f / sum);
-      if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top, sum);
+    }
+#pragma unroll
+    for (int t = 0; t < EACH; ++t) {
+      const int x = (warp + t * W) * 32 + lane, row = x / QUADS, ch = 4 * (x - row * QUADS);
+      if (warp + t * W >= TASKS) break;
+      store_out4(p, c.s, c.head, c.rg * ROWS + row, ch, o[t], sum[t] == 0.0f ? 0.0f : 1.0f / sum[t]);
+      if (ch == 0) store_lse(p, c.s, c.head, c.rg * ROWS + row, top[t], sum[t]);
     }
   }
   if (bad) atomicOr(p.error, kErrIndex);

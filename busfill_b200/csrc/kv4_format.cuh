@@ -123,19 +123,20 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162f
 __device__ __forceinline__ void from_float(__half& y, float x) { y = __float2half_rn(x); }
 __device__ __forceinline__ void from_float(__nv_bfloat16& y, float x) { y = __float2bfloat16_rn(x); }
 
-// Eight consecutive 16-bit elements; `vec`: p is 16-byte aligned.
+// The eight 16-bit elements of a 16-byte piece.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float* x) {
+__device__ __forceinline__ void to_floats(const uint4& v, float* x) {
   alignas(16) T e[8];
-  if (vec) {
-    *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = p[i];
-  }
+  *reinterpret_cast<uint4*>(e) = v;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
 }
+
+// 16 bytes to shared memory; zeros unless `have`
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // (a, b) = (a, b) * s + t and (a, b) += t as packed fp32 pairs (sm_100)
 __device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float t) {

@@ -104,12 +104,6 @@ __device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign,
   }
 }
 
-// 16 bytes to shared memory; zeros unless `have`
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
