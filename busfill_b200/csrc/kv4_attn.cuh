@@ -497,6 +497,27 @@ __device__ __forceinline__ void seek(const AttnParams& p, const int* pre, int u,
   c.page = c.s.page0 + r - c.rg * c.s.pages;
 }
 
+// From any page of an item to the first of the next; true at a sequence's end.
+template <int ROWS>
+__device__ __forceinline__ bool next_item(const AttnParams& p, const int* pre, Cursor& c, bool& bad) {
+  bool moved = false;
+  if (++c.rg == c.rgs) {
+    c.rg = 0;
+    if (++c.head == p.c.heads) {
+      c.head = 0;
+      moved = true;
+      do ++c.b;
+      while (c.b < p.c.batch && pre[c.b + 1] == pre[c.b]);
+      if (c.b < p.c.batch) {
+        c.s = span_of(p, c.b, bad);
+        c.rgs = (c.s.n * p.group + ROWS - 1) / ROWS;
+      }
+    }
+  }
+  c.page = c.s.page0;
+  return moved;
+}
+
 // The pages of a range of units one after another, for the copies that run
 // ahead: a cursor of its own; the warp's lanes hold the next 32 page numbers.
 template <int D, int ROWS>
@@ -514,22 +535,7 @@ struct PageFeed {
     }
     const int pg = __shfl_sync(0xffffffffu, number, in.page - held);
     const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + in.head) * Fmt<D>::kPageBytes;
-    if (++in.page == in.s.page0 + in.s.pages) {
-      if (++in.rg == in.rgs) {
-        in.rg = 0;
-        if (++in.head == p.c.heads) {
-          in.head = 0;
-          do ++in.b;
-          while (in.b < p.c.batch && pre[in.b + 1] == pre[in.b]);
-          if (in.b < p.c.batch) {
-            in.s = span_of(p, in.b, bad);
-            in.rgs = (in.s.n * p.group + ROWS - 1) / ROWS;
-          }
-          held = -64;
-        }
-      }
-      in.page = in.s.page0;
-    }
+    if (++in.page == in.s.page0 + in.s.pages && next_item<ROWS>(p, pre, in, bad)) held = -64;
     return src;
   }
 };
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
         }
       }
       if (u + 1 < u1) {   // the next item
-        seek<ROWS>(p, pre, u + 1, c, bad);
+        next_item<ROWS>(p, pre, c, bad);
         item0 = begun = u + 1;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) load_queries<D>(p, c.s, c.head, c.rg * ROWS + 8 * nt, lane, q[nt]);
@@ -735,9 +741,10 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     const int k0 = group[g], n = group[g + 1] - k0, item0 = piece_item[list[k0]];
     const Cursor& c = *piece_cursor(list[k0]);
     float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
     for (int i = 0; i < n; ++i) top = fmaxf(top, meta_m[list[k0 + i] * ROWS + row]);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < n; ++i) {
       const int id = list[k0 + i];
       const float4 v = reinterpret_cast<const float4*>(
@@ -952,7 +959,7 @@ __global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(
       }
       if (u + 1 == u1) break;
       if (++c.page == c.s.page0 + c.s.pages) {
-        seek<ROWS>(p, pre, u + 1, c, bad);
+        next_item<ROWS>(p, pre, c, bad);
         if (single) load_rows(0);
       }
     }
