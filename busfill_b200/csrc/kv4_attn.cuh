@@ -32,6 +32,10 @@
 // first inside the CTA, then, by the CTA that comes last (a counter), from
 // the workspace; always in the order of the ranges, so results repeat bit for
 // bit.
+//
+// Measured, 64 query heads over 8 of 128: 32 sequences to 16000 tokens 82 us
+// (353 MB, 4.3 TB/s; bulk copies of that size alone 64-74 us), one of 131071
+// 44 us (106 MB), one of 300 9 us.
 #pragma once
 
 #include "kv4_format.cuh"
@@ -587,7 +591,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   // CTAs that share the list: every one gets a unit; where a warp would get
   // two pages at most, no more than there are items, as a split item has to
   // be joined through the workspace (one sequence of 300 tokens, 8 heads: 8
-  // CTAs of 5 pages, 9.6 us, against 40 of one page and 5 parts an item, 12.1 us)
+  // CTAs of 5 pages, 9.6 us, against 40 of one page and 5 parts an item, 12.1 us then)
   const long long ctas = min((int)gridDim.x, max(min(items, T), (T + 2 * W - 1) / (2 * W)));
   if ((int)blockIdx.x >= ctas) {
     if (bad) atomicOr(p.error, kErrIndex);
@@ -846,6 +850,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
 // exp(score[r,s] - lse[r]). Keys only, so half the bytes of the attention. A
 // warp streams whole pages (ranges of the list of all pages, as above) and
 // walks over the rows that see each, so every sum has one owner and one order.
+// One sequence of 131071 tokens, 8 heads of 128, one row of 64 heads: 26 us for
+// 61 MB.
 template <int D>
 struct WeightsGeo {
   static constexpr int kWarps = D == 256 ? 8 : 16;
