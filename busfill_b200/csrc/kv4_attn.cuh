@@ -121,12 +121,16 @@ __device__ __forceinline__ void sees(const AttnParams& p, const Span& s, int i, 
   lo = p.window > 0 ? max(0, s.len - s.n + i + 1 - p.window) : 0;
 }
 
-// pre[1 .. n] to its running sum, pre[0] = 0 (one warp)
-__device__ __forceinline__ void running_sum(int* pre, int n, int lane) {
-  int total = 0;
+// pre[1 .. n] (each at most 2^30) to its running sum, pre[0] = 0 (one warp).
+// More than about 2^30 in all is refused: no work, and reported.
+__device__ __forceinline__ void running_sum(int* pre, int n, int lane, bool& bad) {
+  int total = 0, size = 0;
+  for (int i = lane; i < n; i += 32) size += (pre[i + 1] >> 16) + 1;
+  const bool over = __reduce_add_sync(0xffffffffu, size) > (1 << 14) + n;
+  bad = bad || over;
   if (lane == 0) pre[0] = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
-    int x = i0 + lane < n ? pre[i0 + lane + 1] : 0;
+    int x = i0 + lane < n && !over ? pre[i0 + lane + 1] : 0;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, m);
@@ -585,7 +589,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     }
   }
   __syncthreads();
-  if (warp == 0) running_sum(pre, batch, lane);
+  if (warp == 0) running_sum(pre, batch, lane, bad);
   __syncthreads();
   const int T = pre[batch], items = misc[126];
   // CTAs that share the list: every one gets a unit; where a warp would get
@@ -883,7 +887,7 @@ __global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(
     pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
   }
   __syncthreads();
-  if (warp == 0) running_sum(pre, batch, lane);
+  if (warp == 0) running_sum(pre, batch, lane, bad);
   __syncthreads();
   const long long T = pre[batch], all = (long long)gridDim.x * W, me = (long long)blockIdx.x * W + warp;
   const int u0 = (int)(T * me / all), u1 = (int)(T * (me + 1) / all);

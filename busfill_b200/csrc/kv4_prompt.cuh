@@ -249,8 +249,9 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
     const int groups = groups_of<D>(p, s);
     int n = 0, x;
     for (int t = lane; t < groups; t += 32) n += tiles_of<D>(p, s, t, x) + kItemCost;
-    n = __reduce_add_sync(0xffffffffu, n) * p.c.heads;
-    if (lane == 0) pre[b + 1] = n;
+    const long long cost = (long long)__reduce_add_sync(0xffffffffu, n) * p.c.heads;
+    if (cost > (1 << 30)) bad = true;
+    if (lane == 0) pre[b + 1] = cost > (1 << 30) ? 0 : (int)cost;
     if (s.len == 0 && blockIdx.x == 0) {   // nothing cached: rows are 0
       for (int r = lane; r < s.n * p.q_heads; r += 32) {
         const int i = r / p.q_heads, h = r - i * p.q_heads;
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) running_sum(pre, batch, lane);
+  if (warp == 0) running_sum(pre, batch, lane, bad);
   __syncthreads();
   const uint32_t tmem = misc[0];
 

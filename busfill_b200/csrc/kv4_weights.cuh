@@ -110,13 +110,14 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
     const int tiles = wsum::tiles_of<D>(s, t0);
     int n = 0;
     for (int t = lane; t < tiles; t += 32) n += wsum::blocks_of<D>(p, s, t0 + t, x);
-    n = __reduce_add_sync(0xffffffffu, n) * p.c.heads;
-    if (lane == 0) pre[b + 1] = n;
+    const long long cost = (long long)__reduce_add_sync(0xffffffffu, n) * p.c.heads;
+    if (cost > (1 << 30)) bad = true;
+    if (lane == 0) pre[b + 1] = cost > (1 << 30) ? 0 : (int)cost;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) running_sum(pre, batch, lane);
+  if (warp == 0) running_sum(pre, batch, lane, bad);
   __syncthreads();
   const uint32_t tmem = misc[0];
   const int T = pre[batch];

@@ -395,7 +395,8 @@ BUSFILL_API int busfill_dequant_q6k(const uint8_t* body, const uint16_t* d, uint
  * read by the kernels: an entry out of range is not followed (a page index is
  * taken as page 0, a length is cut to the table, a row is left out or, for
  * rope, written as NaN), and busfill_stream_status reports
- * BUSFILL_ERR_DEVICE_INDEX.
+ * BUSFILL_ERR_DEVICE_INDEX; so it does for an attention call of more than
+ * about 2^30 pages times groups of 8 rows, which then does nothing.
  * `dtype` is BUSFILL_TYPE_F16 or BUSFILL_TYPE_BF16 and holds for every 16-bit
  * tensor of the call; strides count elements, channels are contiguous.
  * ------------------------------------------------------------------------- */
