@@ -14,9 +14,12 @@
 // The two row tiles i = 0, 1 take turns: while one's S is in the softmax
 // threads, the tensor pipe works on the other. Codes are dequantized once per
 // tile and CTA into a ring of fp16 operands, exactly ((c - 8) d has at most 11
-// significant bits). Exponentials are taken against a reference that is a
-// maximum of earlier scores; O is rescaled only when a score lies more than
-// 14 (in log2) above it.
+// significant bits). Exponentials are taken against a reference 2^kRaise below
+// a maximum of earlier scores; O is rescaled only when a score lies more than
+// kOver (in log2) above the reference. P is rounded to fp16 once (the tensor
+// core's operand); with the reference where it is, relatively for weights down
+// to 2^-22 of the largest (with the reference at the maximum: to 2^-14, and
+// what lay 2^-20 below a sink without a value was off by 1 to 9 %).
 //
 // Warps: 0 copies raw pages into a ring (bulk copies); 1 issues the MMAs and
 // owns TMEM; 2 hands out the work; 4-7 and 8-11 softmax of row tile 0 and 1,
@@ -122,7 +125,11 @@ namespace prompt {
 
 constexpr int kThreads = 512;
 constexpr int kSoftmaxWarp0 = 4, kDequantWarp0 = 12;
-constexpr float kOver = 14.0f;   // how far, in log2, a score may lie above the row's reference (p < 2^14 in fp16)
+constexpr float kOver = 15.0f;   // how far, in log2, a score may lie above the row's reference (p < 2^15 in fp16)
+// How far, in log2, below the maximum found the reference is set. What is left to
+// kOver is how far a row may grow unfollowed (prompt of 8000 tokens: 15, 8 and 7
+// left 1160 us, 4 left 1320, as some row of a warp's 32 outgrows it too often).
+constexpr float kRaise = 8.0f;
 
 template <int D>
 struct Geo {
@@ -689,8 +696,8 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           // one's MMAs run while the second one's exponentials are taken. The
           // exponentials are taken against the maximum known so far, while
           // the half's own is found beside them: only where that is more than
-          // 2^kOver above (at the start, and then rarely) are they taken
-          // again. Short loops stay in the instruction cache.
+          // 2^kOver above the reference (at the start, and then rarely) are
+          // they taken again. Short loops stay in the instruction cache.
 #pragma unroll 1
           for (int h = 0; ok && h < 2; ++h) {
             constexpr int H = K / 2;
@@ -723,7 +730,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
               }
               const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]) * f;
               if (again || !__any_sync(0xffffffffu, mt > m + kOver || (m == -INFINITY && mt > m))) break;
-              const float m2 = fmaxf(m, mt);
+              const float m2 = fmaxf(m, mt - kRaise);
               const float a = m == m2 ? 1.0f : exp2_approx(m - m2);
               m = m2;
               l *= a;

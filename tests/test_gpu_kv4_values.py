@@ -19,7 +19,7 @@ DEV = "cuda"
 HEADS = 8          # query heads of the one key/value head
 
 
-def _sequence(n, dim, rows, sink, vexp, seed, spikes=0):
+def _sequence(n, dim, rows, sink, vexp, seed, spikes=0, empty_sink=False):
     """One cached sequence whose token 0 scores about `sink` above the others for every row.
     Returns (q, pages, table, kv_len, k, v): k, v are the cached values in 64 bits."""
     import torch
@@ -29,6 +29,8 @@ def _sequence(n, dim, rows, sink, vexp, seed, spikes=0):
     k = torch.randn((n, 1, dim), generator=gen)
     k[0] = base[0] * (sink / dim ** 0.5)
     v = torch.randn((n, 1, dim), generator=gen) * 2.0 ** vexp
+    if empty_sink:
+        v[0] = 0
     for i in range(spikes):        # tokens of much larger values that no row looks at
         k[7 + 13 * i], v[7 + 13 * i] = -base[0], v[7 + 13 * i] * 2.0 ** 12
     k, v = k.half(), v.half()
@@ -96,3 +98,15 @@ def test_unseen_large_values_take_nothing_from_small_ones(dim, rows):
     out = bf.attn_kv4(wide, pages, table, kv_len, q_start=start, max_q=rows)
     assert bf.stream_status() == 0
     _check_wide(q, out, k, v, True, 500)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,n,causal", [(100, 6000, True), (330, 1000, False), (1, 6000, True), (4, 6000, True)])
+def test_rows_keep_what_lies_far_below_a_sink_without_value(dim, rows, n, causal):
+    """The sink takes all but e^-14 of every weight and has no value: the output is the other
+    tokens', whose weights are 2^-20 of the largest. 100 rows of 8 heads take the kernel of many rows."""
+    q, pages, table, kv_len, k, v = _sequence(n, dim, rows, 14, 8, seed=dim + rows, empty_sink=True)
+    wide, table, kv_len, start = _wide(q, table, kv_len, 100 if rows < 8 else 3)
+    out = bf.attn_kv4(wide, pages, table, kv_len, q_start=start, max_q=rows, causal=causal)
+    assert bf.stream_status() == 0
+    _check_wide(q, out, k, v, causal, 100 if rows < 8 else 3)
