@@ -180,6 +180,7 @@ struct Item {
 struct Work {
   int b, head, first, n;         // first row and rows of the sequence
   int len, row0, tile0, tiles;   // tiles 0: the end
+  int page0;                     // the first page that some row of the sequence sees
   int kind, c_first, c_last, row_tiles;
 };
 enum { kWhole = 0, kTail = 1, kHead = 2 };   // kTail: began in an earlier CTA; kHead: goes on in the next
@@ -365,6 +366,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           if (to > from) {
             Work y;
             y.b = it.b, y.head = it.head, y.first = it.s.first, y.n = it.s.n, y.len = it.s.len;
+            y.page0 = it.s.page0;
             y.row0 = it.t * G::kRows, y.tile0 = it.tile0 + from, y.tiles = to - from;
             y.kind = from > 0 ? kTail : to < it.tiles ? kHead : kWhole;
             y.c_first = cta_of(x + near_start(c)), y.c_last = cta_of(x + c - kSnap - 1);
@@ -406,21 +408,24 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
         const int pages = (x.len + kPage - 1) / kPage;
         for (int j = 0; ok && j < x.tiles; ++j) {
           const int page0 = (x.tile0 + j) * G::kTilePages;
-          const int have = min(G::kTilePages, pages - page0);
+          // pages [skip, have) of the tile: the ones before every row's window
+          // may have been given back, and are not looked up
+          const int skip = max(0, x.page0 - page0), have = min(G::kTilePages, pages - page0);
+          auto there = [&](int k) { return k >= skip && k < have; };
           const uint8_t* src[G::kTilePages];
 #pragma unroll
           for (int k = 0; k < G::kTilePages; ++k)
-            src[k] = p.c.pages + ((size_t)(k < have ? page_of(p.c, p.c.table, p.c.table_cols, x.b, page0 + k, bad) : 0) *
+            src[k] = p.c.pages + ((size_t)(there(k) ? page_of(p.c, p.c.table, p.c.table_cols, x.b, page0 + k, bad) : 0) *
                                       p.c.heads + x.head) * F::kPageBytes;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int st = n % G::kRawStages;
             if (!wait(G::bRawEmpty + st, n / G::kRawStages + 1)) break;
             if (elect_one()) {
-              mbar_arrive_expect_tx(BAR(G::bRawFull + st), have * G::kHalfPage);
+              mbar_arrive_expect_tx(BAR(G::bRawFull + st), (have - skip) * G::kHalfPage);
 #pragma unroll
               for (int k = 0; k < G::kTilePages; ++k)
-                if (k < have)
+                if (there(k))
                   bulk_load(sbase + G::kRawOff + st * G::kRawBytes + k * G::kHalfPage, src[k] + half * G::kHalfPage,
                             G::kHalfPage, BAR(G::bRawFull + st));
             }
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
     const int w = warp - kDequantWarp0, j = lane & 3;
     uint32_t n = 0;
     for (Work x0 = next_piece(); ok && x0.tiles > 0; x0 = next_piece()) {
-      const int len = x0.len;
+      const int len = x0.len, low = x0.page0 * kPage;
       int base = x0.tile0 * K;
 #pragma unroll 1
       for (int left = 2 * x0.tiles; left > 0; --left, ++n) {
@@ -547,7 +552,8 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           } else {
             uint32_t y[NB];   // value words 2j and 2j + 1 of all blocks
             load_words<NB>(pg + t * F::kRow + ((2 * j) ^ value_swizzle<D>(t)) * 2 * NB, y);
-            const bool live = base + tok < len;   // slots behind the sequence hold anything
+            // slots behind the sequence and of pages that were not brought hold anything
+            const bool live = base + tok < len && base + tok >= low;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
               x[b] = prmt(y[b / 2], y[NB / 2 + b / 2], b & 1 ? 0x7632u : 0x5410u);

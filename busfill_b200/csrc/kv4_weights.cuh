@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
 #pragma unroll
         for (int b = 0; b < NB / 2; ++b) sc[b] = 0;
         const int t = tok & (kPage - 1);
-        if (base + tok < it.s.len) {
+        if (base + tok < it.s.len && base + tok >= it.s.page0 * kPage) {   // not before every row's window
           const int pg = page_of(p.c, p.c.table, p.c.table_cols, it.b, (base + tok) / kPage, bad);
           const uint8_t* src = p.c.pages + ((size_t)pg * p.c.heads + it.head) * F::kPageBytes;
           load_words<NB>(src + t * F::kRow + j * 4 * NB, x);

@@ -461,7 +461,8 @@ BUSFILL_API int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_star
  * reads key/value head h / (q_heads / heads).
  *   out = sum_s p_s v_s,  p = softmax(scale * q k_s)
  * over the slots that a row sees: all of its sequence, with `causal` those up
- * to its own, with window > 0 (needs causal) the last `window` of these. A
+ * to its own, with window > 0 (needs causal) the last `window` of these; pages
+ * that lie before the windows of all of a sequence's rows are not looked up. A
  * row that sees nothing is 0 (its lse -inf). Scores, softmax statistics and
  * sums are fp32. lse (optional, [tokens][q_heads]) gets log(sum exp(score)).
  * weights (optional, fp32 [batch][heads][weights_cols]): the weight that the

@@ -1,0 +1,44 @@
+"""Calls that a server makes of the cache operators besides the plain ones: pages given back, padded
+batches, empty steps, captured steps, and calls that are refused on the device."""
+import numpy as np
+import pytest
+
+import busfill_b200 as bf
+from test_gpu_kv4 import DEV, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(shape, seed, dtype="float16"):
+    import torch
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(getattr(torch, dtype)).to(DEV)
+
+
+# ---------------------------------------------------------------------------
+# pages before every row's window may have been given back
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 6, 70, 200])
+def test_pages_before_the_window_are_not_looked_up(dim, new):
+    import torch
+    lens, window, heads = [64 * 9 + new, 1000, 64 * 5 + 30 + new], 50, 12
+    b = Batch(lens, 2, dim, seed=dim + new)
+    # page 0 belongs to nobody and holds NaN scales
+    pages = torch.cat([torch.full_like(b.pages[:1], 0xFF), b.pages])
+    table = torch.where(b.table < b.num_pages, b.table + 1, b.table)
+    gone = table.clone()
+    for i, n in enumerate(lens):
+        first = max(0, n - new + 1 - window) // 64
+        assert first > 0
+        gone[i, :first] = torch.tensor([-1, b.num_pages + 1], dtype=torch.int32, device=DEV).repeat(first)[:first]
+    q, start = _rand((3 * new, heads, dim), 1), b.starts([new] * 3)
+    results = []
+    for t in (table, gone):
+        lse = torch.zeros((3 * new, heads), device=DEV)
+        weights = torch.zeros((3, 2, 64 * b.cols), device=DEV)
+        out = bf.attn_kv4(q, pages, t, b.kv_len, q_start=start, max_q=new, window=window, lse=lse, weights=weights)
+        assert bf.stream_status() == 0
+        results.append((out, lse, weights))
+    assert torch.isfinite(results[0][0]).all()
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
