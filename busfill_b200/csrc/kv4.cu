@@ -137,8 +137,10 @@ int busfill_kv4_page_bytes(int head_dim) {
 }
 
 int busfill_rope_axes(const busfill_rope* r, void* stream) {
-  if (!r || !r->q || !r->q_out || !r->positions || !r->cos || !r->sin || !r->axis) return BUSFILL_ERR_INVALID_ARG;
-  if (r->k_heads > 0 && (!r->k || !r->k_out)) return BUSFILL_ERR_INVALID_ARG;
+  if (!r || !r->cos || !r->sin || !r->axis) return BUSFILL_ERR_INVALID_ARG;
+  // a step of no tokens has nothing to point at
+  if (r->tokens != 0 && (!r->q || !r->q_out || !r->positions || (r->k_heads > 0 && (!r->k || !r->k_out))))
+    return BUSFILL_ERR_INVALID_ARG;
   if (!is16bit(r->dtype)) return BUSFILL_ERR_INVALID_ARG;
   if (r->tokens < 0 || r->q_heads < 1 || r->k_heads < 0 || r->q_heads > 65535 || r->k_heads > 65535 ||
       r->head_dim < 2 || r->head_dim > 512 || r->rot < 2 || (r->rot & 1) || r->rot > r->head_dim || r->axes < 1 ||
@@ -204,7 +206,7 @@ int busfill_rope_axes(const busfill_rope* r, void* stream) {
 int busfill_kv4_append(const busfill_kv4* cache, const busfill_kv4_rows* r, void* stream) {
   int st = check_cache(cache);
   if (st != BUSFILL_OK) return st;
-  if (!r || !r->k || !r->v || !is16bit(r->dtype)) return BUSFILL_ERR_INVALID_ARG;
+  if (!r || (r->tokens != 0 && (!r->k || !r->v)) || !is16bit(r->dtype)) return BUSFILL_ERR_INVALID_ARG;
   if (r->tokens < 0 || (!r->q_start && r->tokens != cache->batch)) return BUSFILL_ERR_SHAPE;
   if (!aligned(r->k, 2) || !aligned(r->v, 2) || !aligned(r->q_start, 4)) return BUSFILL_ERR_ALIGNMENT;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -241,7 +243,7 @@ int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_start, int token
                      void* stream) {
   int st = check_cache(cache);
   if (st != BUSFILL_OK) return st;
-  if (!k || !v) return BUSFILL_ERR_INVALID_ARG;
+  if (tokens != 0 && (!k || !v)) return BUSFILL_ERR_INVALID_ARG;
   if (tokens < 0 || (!q_start && tokens != cache->batch)) return BUSFILL_ERR_SHAPE;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(q_start, 4)) return BUSFILL_ERR_ALIGNMENT;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -261,7 +263,7 @@ int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_start, int token
 int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stream) {
   int st = check_cache(cache);
   if (st != BUSFILL_OK) return st;
-  if (!a || !a->q || !a->out || !is16bit(a->dtype) || (a->weights && !a->lse) || a->window < 0 ||
+  if (!a || (a->tokens != 0 && (!a->q || !a->out || (a->weights && !a->lse))) || !is16bit(a->dtype) || a->window < 0 ||
       (a->window > 0 && !a->causal) || !(a->scale == a->scale))
     return BUSFILL_ERR_INVALID_ARG;
   if (a->tokens < 0 || a->q_heads < 1 || a->q_heads % cache->heads != 0 || a->max_q < 1 ||

@@ -398,7 +398,8 @@ BUSFILL_API int busfill_dequant_q6k(const uint8_t* body, const uint16_t* d, uint
  * BUSFILL_ERR_DEVICE_INDEX; so it does for an attention call of more than
  * about 2^30 pages times groups of 8 rows, which then does nothing.
  * `dtype` is BUSFILL_TYPE_F16 or BUSFILL_TYPE_BF16 and holds for every 16-bit
- * tensor of the call; strides count elements, channels are contiguous.
+ * tensor of the call; strides count elements, channels are contiguous. A step
+ * of no tokens (tokens == 0) does nothing; its tensors may be NULL.
  * ------------------------------------------------------------------------- */
 #define BUSFILL_KV4_PAGE 64
 #define BUSFILL_KV4_MAX_BATCH 1024

@@ -42,3 +42,37 @@ def test_pages_before_the_window_are_not_looked_up(dim, new):
     assert torch.isfinite(results[0][0]).all()
     for x, y in zip(*results):
         assert torch.equal(x, y)
+
+
+# ---------------------------------------------------------------------------
+# steps without tokens
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_steps_of_no_tokens_do_nothing(dtype):
+    import torch
+    b = Batch([70, 5], 2, 128, seed=2)
+    pages, start = b.pages.clone(), b.starts([0, 0])
+    cache = (b.pages, b.table, b.kv_len)
+    q, k = _rand((0, 8, 128), 0, dtype), _rand((0, 2, 128), 0, dtype)
+    cos, sin = bf.rope_table(16, 128)
+    qo, ko = bf.rope_axes(q, k, torch.zeros((3, 0), dtype=torch.int32, device=DEV), cos, sin, [i % 3 for i in range(64)])
+    assert qo.shape == q.shape and ko.shape == k.shape
+    bf.kv4_append(*cache, k, k, q_start=start)
+    kk, vv = bf.kv4_read(*cache, q_start=start, tokens=0)
+    assert kk.shape == vv.shape == (0, 2, 128)
+    weights = torch.rand((2, 2, 64 * b.cols), device=DEV)
+    before = weights.clone()
+    assert bf.attn_kv4(q, *cache, q_start=start, weights=weights).shape == q.shape
+    assert torch.equal(weights, before) and torch.equal(b.pages, pages) and bf.stream_status() == 0
+
+
+@pytest.mark.parametrize("new", [(0, 0, 1), (0, 90, 0)])
+def test_steps_of_some_sequences_leave_the_others_alone(new):
+    import torch
+    b = Batch([70, 100, 5], 2, 128, seed=2)
+    q, start = _rand((sum(new), 16, 128), 3), b.starts(new)
+    weights = torch.zeros((3, 2, 64 * b.cols), device=DEV)
+    out = bf.attn_kv4(q, b.pages, b.table, b.kv_len, q_start=start, weights=weights)
+    assert bf.stream_status() == 0 and torch.isfinite(out).all()
+    for i, n in enumerate(new):
+        assert bool(weights[i].any()) == (n > 0)
