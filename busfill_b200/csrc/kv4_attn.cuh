@@ -130,7 +130,17 @@ __device__ __forceinline__ void sees(const AttnParams& p, const Span& s, int i, 
   lo = p.window > 0 ? max(0, s.len - s.n + i + 1 - p.window) : 0;
 }
 
-// pre[1 .. n] (each at most 2^30) to its running sum, pre[0] = 0 (one warp).
+// The warp's sum.
+__device__ __forceinline__ long long warp_total(long long x) {
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  return x;
+}
+// A sequence's units for running_sum: more than 2^30 as a number that it refuses.
+__device__ __forceinline__ int counted(long long units) {
+  return (int)min(units, (1ll << 30) + (1ll << 16));
+}
+// pre[1 .. n] (of `counted`) to its running sum, pre[0] = 0 (one warp).
 // More than about 2^30 in all is refused: no work, and reported.
 __device__ __forceinline__ void running_sum(int* pre, int n, int lane, bool& bad) {
   int total = 0, size = 0;
@@ -620,8 +630,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   for (int b = threadIdx.x; b < batch; b += W * 32) {
     const Span s = span_of(p, b, bad);
     const long long n = (long long)p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS) * s.pages;
-    if (n > (1 << 30)) bad = true;
-    pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
+    pre[b + 1] = counted(n);
     if (s.pages > 0) atomicAdd(&misc[126], p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS));
     if (n == 0 && blockIdx.x == 0) {   // rows that see nothing
       for (int i = 0; i < s.n; ++i)
@@ -926,8 +935,7 @@ __global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(
   pdl_launch_dependents();
   bool bad = false;
   for (int b = threadIdx.x; b < batch; b += W * 32) {
-    const long long n = (long long)p.c.heads * span_of(p, b, bad).pages;
-    pre[b + 1] = n > (1 << 30) ? 0 : (int)n;
+    pre[b + 1] = counted((long long)p.c.heads * span_of(p, b, bad).pages);
   }
   __syncthreads();
   if (warp == 0) running_sum(pre, batch, lane, bad);

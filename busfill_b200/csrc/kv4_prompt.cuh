@@ -255,11 +255,11 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   for (int b = warp; b < batch; b += kThreads / 32) {
     const Span s = span_of(p, b, bad);
     const int groups = groups_of<D>(p, s);
-    int n = 0, x;
+    long long n = 0;
+    int x;
     for (int t = lane; t < groups; t += 32) n += tiles_of<D>(p, s, t, x) + kItemCost;
-    const long long cost = (long long)__reduce_add_sync(0xffffffffu, n) * p.c.heads;
-    if (cost > (1 << 30)) bad = true;
-    if (lane == 0) pre[b + 1] = cost > (1 << 30) ? 0 : (int)cost;
+    const long long cost = warp_total(n) * p.c.heads;
+    if (lane == 0) pre[b + 1] = counted(cost);
     if (s.len == 0 && blockIdx.x == 0) {   // nothing cached: rows are 0
       for (int r = lane; r < s.n * p.q_heads; r += 32) {
         const int i = r / p.q_heads, h = r - i * p.q_heads;

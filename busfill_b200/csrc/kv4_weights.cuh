@@ -108,11 +108,10 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
     const Span s = span_of(p, b, bad);
     int t0, x;
     const int tiles = wsum::tiles_of<D>(s, t0);
-    int n = 0;
+    long long n = 0;
     for (int t = lane; t < tiles; t += 32) n += wsum::blocks_of<D>(p, s, t0 + t, x);
-    const long long cost = (long long)__reduce_add_sync(0xffffffffu, n) * p.c.heads;
-    if (cost > (1 << 30)) bad = true;
-    if (lane == 0) pre[b + 1] = cost > (1 << 30) ? 0 : (int)cost;
+    const long long cost = warp_total(n) * p.c.heads;
+    if (lane == 0) pre[b + 1] = counted(cost);
   }
   tc_fence_before();
   __syncthreads();

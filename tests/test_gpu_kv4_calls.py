@@ -76,3 +76,31 @@ def test_steps_of_some_sequences_leave_the_others_alone(new):
     assert bf.stream_status() == 0 and torch.isfinite(out).all()
     for i, n in enumerate(new):
         assert bool(weights[i].any()) == (n > 0)
+
+
+# ---------------------------------------------------------------------------
+# calls of more work than is counted
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cols", [(1 << 18, 1), (1 << 17, 2)])
+def test_a_call_of_too_much_work_does_nothing_and_is_reported(cols):
+    """2^23 query rows against 2^24 tokens, in one sequence or two: a sequence has 2^32 or 2^31 units
+    and a few, which in 32 bits are a small or a negative number."""
+    import torch
+    cols, batch = cols
+    new, heads, dim = (1 << 19) // batch, 16, 64
+    pages = torch.zeros((1, 1, 72 * dim), dtype=torch.uint8, device=DEV)
+    table = torch.zeros((batch, cols * batch), dtype=torch.int32, device=DEV)     # all of page 0
+    kv_len = torch.full((batch,), 64 * cols * batch, dtype=torch.int32, device=DEV)
+    start = torch.arange(0, (batch + 1) * new, new, dtype=torch.int32, device=DEV)
+    q = torch.zeros((batch * new, heads, dim), dtype=torch.float16, device=DEV)
+    out = torch.full_like(q, 5.0)
+    bf.attn_kv4(q, pages, table, kv_len, q_start=start, max_q=new, causal=False, out=out)
+    assert bf.stream_status_bits() == (-9, 256)
+    assert bool((out == 5.0).all())
+    # what comes after is right
+    b = Batch([3000], 1, dim, seed=1)
+    x = _rand((64, heads, dim), 4)
+    s = b.starts([64])
+    one = bf.attn_kv4(x, b.pages, b.table, b.kv_len, q_start=s, max_q=64)
+    two = bf.attn_kv4(x, b.pages, b.table, b.kv_len, q_start=s, max_q=64)
+    assert bf.stream_status() == 0 and torch.equal(one, two) and float(one.float().abs().max()) > 0
