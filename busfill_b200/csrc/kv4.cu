@@ -78,9 +78,10 @@ constexpr long long kMaxGrid = 2147483647;
 // of 4096, heads of 128: 32 rows 49 / 68).
 constexpr int kTwoTileRows = 25;
 
-// Workspace of the attention calls on a stream: a counter per CTA, then the
-// largest kernel's partial results.
+// Workspace of the attention calls on a stream: a counter per CTA, a word
+// between a call's two kernels, then the largest kernel's partial results.
 constexpr size_t kCounterBytes = 4096;
+constexpr int kMaxCtas = kCounterBytes / 4 - 1;
 size_t workspace_bytes(int sms) {
   size_t f = part_floats<64, 2>();
   f = std::max(f, part_floats<128, 1>());
@@ -294,9 +295,10 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.causal = a->causal != 0, p.window = a->window < (int64_t)kPage * cache->table_cols ? a->window : 0, p.bf16 = a->dtype == BUSFILL_TYPE_BF16;
   p.wide_out = aligned(a->out, 32) && (a->out_token | a->out_head) % 16 == 0;
   p.counters = static_cast<unsigned*>(work);
+  p.refused = p.counters + kMaxCtas;
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
   p.error = ctx.error;
-  if (ctx.sms > (int)(kCounterBytes / 4)) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
+  if (ctx.sms > kMaxCtas) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
   const int rows = p.max_q * p.group;
   st = by_dim(cache->head_dim, [&](auto d) {
     if (rows >= prompt_rows(d()) && (long long)p.tokens * p.q_heads >= kPromptTotal)

@@ -71,6 +71,7 @@ struct AttnParams {
   int causal, window, bf16;
   int wide_out;      // output rows start on 32 bytes
   unsigned* counters;   // one per CTA, zero between calls
+  unsigned* refused;    // whether the attention kernel refused the call, for the weights' pass behind it
   float* part;          // partial results (layout of the kernel)
   unsigned* error;
 };
@@ -141,11 +142,12 @@ __device__ __forceinline__ int counted(long long units) {
   return (int)min(units, (1ll << 30) + (1ll << 16));
 }
 // pre[1 .. n] (of `counted`) to its running sum, pre[0] = 0 (one warp).
-// More than about 2^30 in all is refused: no work, and reported.
-__device__ __forceinline__ void running_sum(int* pre, int n, int lane, bool& bad) {
+// More than about 2^30 in all is refused: no work, and reported; or all of it
+// is, if `refused` says so. Returns whether it was.
+__device__ __forceinline__ bool running_sum(int* pre, int n, int lane, bool& bad, bool refused = false) {
   int total = 0, size = 0;
   for (int i = lane; i < n; i += 32) size += (pre[i + 1] >> 16) + 1;
-  const bool over = __reduce_add_sync(0xffffffffu, size) > (1 << 14) + n;
+  const bool over = refused || __reduce_add_sync(0xffffffffu, size) > (1 << 14) + n;
   bad = bad || over;
   if (lane == 0) pre[0] = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
@@ -158,6 +160,12 @@ __device__ __forceinline__ void running_sum(int* pre, int n, int lane, bool& bad
     if (i0 + lane < n) pre[i0 + lane + 1] = total + x;
     total += __shfl_sync(0xffffffffu, x, 31);
   }
+  return over;
+}
+// running_sum in an attention kernel, which also tells the weights' pass.
+__device__ __forceinline__ void running_sum_first(const AttnParams& p, int* pre, int lane, bool& bad) {
+  const bool over = running_sum(pre, p.c.batch, lane, bad);
+  if (p.weights && blockIdx.x == 0 && lane == 0) *p.refused = over;
 }
 
 // Query operand of one row group of 8 rows, and per column pair (2j, 2j + 1)
@@ -641,7 +649,7 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
     }
   }
   __syncthreads();
-  if (warp == 0) running_sum(pre, batch, lane, bad);
+  if (warp == 0) running_sum_first(p, pre, lane, bad);
   __syncthreads();
   const int T = pre[batch], items = misc[126];
   // CTAs that share the list: every one gets a unit; where a warp would get
@@ -938,7 +946,7 @@ __global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(
     pre[b + 1] = counted((long long)p.c.heads * span_of(p, b, bad).pages);
   }
   __syncthreads();
-  if (warp == 0) running_sum(pre, batch, lane, bad);
+  if (warp == 0) running_sum(pre, batch, lane, bad, *p.refused != 0);
   __syncthreads();
   const long long T = pre[batch], all = (long long)gridDim.x * W, me = (long long)blockIdx.x * W + warp;
   const int u0 = (int)(T * me / all), u1 = (int)(T * (me + 1) / all);

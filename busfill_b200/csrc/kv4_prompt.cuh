@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) running_sum(pre, batch, lane, bad);
+  if (warp == 0) running_sum_first(p, pre, lane, bad);
   __syncthreads();
   const uint32_t tmem = misc[0];
 

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) running_sum(pre, batch, lane, bad);
+  if (warp == 0) running_sum(pre, batch, lane, bad, *p.refused != 0);
   __syncthreads();
   const uint32_t tmem = misc[0];
   const int T = pre[batch];

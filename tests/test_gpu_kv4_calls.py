@@ -104,3 +104,27 @@ def test_a_call_of_too_much_work_does_nothing_and_is_reported(cols):
     one = bf.attn_kv4(x, b.pages, b.table, b.kv_len, q_start=s, max_q=64)
     two = bf.attn_kv4(x, b.pages, b.table, b.kv_len, q_start=s, max_q=64)
     assert bf.stream_status() == 0 and torch.equal(one, two) and float(one.float().abs().max()) > 0
+
+
+@pytest.mark.parametrize("new,heads,batch,cols", [(632, 1, 1, 1 << 24), (1 << 15, 16, 1, 1 << 22)])
+def test_a_refused_call_adds_no_weights(new, heads, batch, cols):
+    """The attention kernel refuses (2^24 pages x 79 row groups; 2^21 tiles x 2^11 row groups), where
+    the weights' pass of the first call counts far fewer units and would go on."""
+    import torch
+    dim = 128
+    pages = torch.zeros((1, 1, 72 * dim), dtype=torch.uint8, device=DEV)
+    table = torch.zeros((batch, cols), dtype=torch.int32, device=DEV)
+    kv_len = torch.full((batch,), 64 * cols, dtype=torch.int32, device=DEV)
+    start = torch.tensor([0, new], dtype=torch.int32, device=DEV)
+    q = torch.zeros((new, heads, dim), dtype=torch.float16, device=DEV)
+    weights = torch.zeros((batch, 1, 64 * cols), device=DEV)
+    lse = torch.zeros((new, heads), device=DEV)
+    bf.attn_kv4(q, pages, table, kv_len, q_start=start, max_q=new, lse=lse, weights=weights)
+    assert bf.stream_status_bits() == (-9, 256)
+    assert not bool(weights.any()) and not bool(lse.any())
+    # the refusal is the call's own
+    b = Batch([3000, 70], 2, dim, seed=1)
+    x, w = _rand((2, 8, dim), 4), torch.zeros((2, 2, 64 * b.cols), device=DEV)
+    bf.attn_kv4(x, b.pages, b.table, b.kv_len, weights=w)
+    assert bf.stream_status() == 0
+    assert torch.allclose(w.sum(-1), torch.full((2, 2), 4.0, device=DEV), rtol=1e-4)
