@@ -252,9 +252,9 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   const int i = token - first;
   const int slot = len - n + i;
   const bool inside = i < n;
-  if (inside && slot < 0) bad = true;
+  if (i < 0 || (inside && slot < 0)) bad = true;   // i < 0: the starts do not rise
   int page = 0;
-  if (inside && slot >= 0) page = page_of(p.c, p.c.table, p.c.table_cols, b, slot / kPage, bad);
+  if (!bad && inside) page = page_of(p.c, p.c.table, p.c.table_cols, b, slot / kPage, bad);
   if (bad) {   // an index out of range: nothing is written
     if (lane == 0) atomicOr(p.error, kErrIndex);
     return;
@@ -316,9 +316,9 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadParams p) {
   const int i = token - first;
   const int slot = len - n + i;
   const bool inside = i < n;
-  if (inside && slot < 0) bad = true;
+  if (i < 0 || (inside && slot < 0)) bad = true;   // i < 0: the starts do not rise
   int page = 0;
-  if (inside && slot >= 0) page = page_of(p.c, p.c.table, p.c.table_cols, b, slot / kPage, bad);
+  if (!bad && inside) page = page_of(p.c, p.c.table, p.c.table_cols, b, slot / kPage, bad);
   if (bad) {
     if (lane == 0) atomicOr(p.error, kErrIndex);
     return;

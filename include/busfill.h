@@ -393,7 +393,8 @@ BUSFILL_API int busfill_dequant_q6k(const uint8_t* body, const uint16_t* d, uint
  * sequence with n rows belongs to slot kv_len - n + r; NULL means one row per
  * sequence. kv_len counts the step's tokens. Tables, lengths and starts are
  * read by the kernels: an entry out of range is not followed (a page index is
- * taken as page 0, a length is cut to the table, a row is left out or, for
+ * taken as page 0, a length is cut to the table, a row is left out (of starts
+ * that do not rise, those that a search does not find in their place) or, for
  * rope, written as NaN), and busfill_stream_status reports
  * BUSFILL_ERR_DEVICE_INDEX; so it does for an attention call of more than
  * about 2^30 pages times groups of 8 rows, which then does nothing.

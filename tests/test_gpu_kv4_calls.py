@@ -128,3 +128,23 @@ def test_a_refused_call_adds_no_weights(new, heads, batch, cols):
     bf.attn_kv4(x, b.pages, b.table, b.kv_len, weights=w)
     assert bf.stream_status() == 0
     assert torch.allclose(w.sum(-1), torch.full((2, 2), 4.0, device=DEV), rtol=1e-4)
+
+
+# ---------------------------------------------------------------------------
+# starts that do not rise
+# ---------------------------------------------------------------------------
+def test_rows_in_front_of_their_sequence_are_not_cached():
+    """Starts 0, 4, 6, 0, 8: the search for rows 0 to 3 ends at sequence 1, whose own start, 4, is
+    behind them. They are left out; what its older 28 tokens hold stays."""
+    import torch
+    b = Batch([20, 30, 9, 8], 2, 128, seed=4)
+    start = torch.tensor([0, 4, 6, 0, 8], dtype=torch.int32, device=DEV)
+    k = _rand((8, 2, 128), 5)
+    older = (b.pages, b.table[1:2].contiguous(), torch.tensor([28], dtype=torch.int32, device=DEV))
+    whole = torch.tensor([0, 28], dtype=torch.int32, device=DEV)
+    before = bf.kv4_read(*older, q_start=whole, tokens=28)
+    bf.kv4_append(b.pages, b.table, b.kv_len, k, k, q_start=start)
+    assert bf.stream_status_bits() == (-9, 256)
+    after = bf.kv4_read(*older, q_start=whole, tokens=28)
+    assert bf.stream_status() == 0
+    assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
