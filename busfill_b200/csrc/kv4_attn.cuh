@@ -511,6 +511,21 @@ __device__ __forceinline__ void store_lse(const AttnParams& p, const Span& s, in
       l > 0.0f ? (m + log2f(l)) * kLn2 : l == 0.0f ? -INFINITY : l;
 }
 
+// The rows [first, first + n) of a sequence with nothing cached: 0, lse -inf.
+// One warp of every CTA comes here, and the CTAs share the rows.
+template <int D>
+__device__ __forceinline__ void store_empty_rows(const AttnParams& p, int first, int n, int lane) {
+  constexpr int V = D / 8;   // 16-byte pieces of a row and head
+  const long long step = (long long)gridDim.x * 32, me = (long long)blockIdx.x * 32 + lane;
+  for (long long x = me; x < (long long)n * p.q_heads * V; x += step) {
+    const long long r = x / V, i = r / p.q_heads;
+    const size_t at = (size_t)(first + i) * p.o_token + (size_t)(r - i * p.q_heads) * p.o_head + 8 * (x - r * V);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = make_uint4(0, 0, 0, 0);
+  }
+  if (p.lse)
+    for (long long x = me; x < (long long)n * p.q_heads; x += step) p.lse[(size_t)first * p.q_heads + x] = -INFINITY;
+}
+
 // Position in the list of units.
 struct Cursor {
   int b, head, rg, page;    // page: index in the sequence
@@ -635,17 +650,17 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
   // units of every sequence, then their running sum (warp 0)
   bool bad = false;
   const int batch = p.c.batch;
-  for (int b = threadIdx.x; b < batch; b += W * 32) {
-    const Span s = span_of(p, b, bad);
-    const long long n = (long long)p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS) * s.pages;
-    pre[b + 1] = counted(n);
-    if (s.pages > 0) atomicAdd(&misc[126], p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS));
-    if (n == 0 && blockIdx.x == 0) {   // rows that see nothing
-      for (int i = 0; i < s.n; ++i)
-        for (int h = 0; h < p.q_heads; ++h) {
-          for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, p.by_group(h), i * p.group + h % p.group, ch, 0.0f);
-          store_lse(p, s, p.by_group(h), i * p.group + h % p.group, 0.0f, 0.0f);
-        }
+  for (int b0 = 32 * warp; b0 < batch; b0 += W * 32) {
+    const int b = b0 + lane;
+    Span s{};
+    if (b < batch) {
+      s = span_of(p, b, bad);
+      pre[b + 1] = counted((long long)p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS) * s.pages);
+      if (s.pages > 0) atomicAdd(&misc[126], p.c.heads * ((s.n * p.group + ROWS - 1) / ROWS));
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, s.n > 0 && s.pages == 0); left; left &= left - 1) {
+      const int from = __ffs(left) - 1;
+      store_empty_rows<D>(p, __shfl_sync(0xffffffffu, s.first, from), __shfl_sync(0xffffffffu, s.n, from), lane);
     }
   }
   __syncthreads();

@@ -260,13 +260,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
     for (int t = lane; t < groups; t += 32) n += tiles_of<D>(p, s, t, x) + kItemCost;
     const long long cost = warp_total(n) * p.c.heads;
     if (lane == 0) pre[b + 1] = counted(cost);
-    if (s.len == 0 && blockIdx.x == 0) {   // nothing cached: rows are 0
-      for (int r = lane; r < s.n * p.q_heads; r += 32) {
-        const int i = r / p.q_heads, h = r - i * p.q_heads;
-        for (int ch = 0; ch < D; ++ch) store_out<D>(p, s, p.by_group(h), i * p.group + h % p.group, ch, 0.0f);
-        store_lse(p, s, p.by_group(h), i * p.group + h % p.group, 0.0f, 0.0f);
-      }
-    }
+    if (s.len == 0) store_empty_rows<D>(p, s.first, s.n, lane);
   }
   tc_fence_before();
   __syncthreads();

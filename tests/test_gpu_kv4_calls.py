@@ -148,3 +148,45 @@ def test_rows_in_front_of_their_sequence_are_not_cached():
     after = bf.kv4_read(*older, q_start=whole, tokens=28)
     assert bf.stream_status() == 0
     assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
+
+
+# ---------------------------------------------------------------------------
+# batches padded with empty sequences
+# ---------------------------------------------------------------------------
+def _event_us(f, n=15):
+    import torch
+    times = []
+    for _ in range(n):
+        a, z = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        z.record()
+        z.synchronize()
+        times.append(a.elapsed_time(z) * 1e3)
+    return sorted(times)[n // 2]
+
+
+@pytest.mark.parametrize("dim,new,dtype", [(64, 1, "float16"), (128, 1, "bfloat16"), (256, 4, "float16"),
+                                           (128, 40, "float16"), (128, 700, "bfloat16")])
+def test_rows_of_empty_sequences_are_zero_and_cost_little(dim, new, dtype):
+    """The rows of empty sequences, whole and in strided outputs; 31 of 32 sequences of one token
+    cost no more than as many sequences of a page each."""
+    import torch
+    batch, heads = (32, 64) if new < 100 else (3, 64)
+    lens = [64 + new] + [0] * (batch - 1)
+    b = Batch(lens, 8, dim, seed=new)
+    q, start = _rand((batch * new, heads, dim), 1, dtype), b.starts([new] * batch)
+    wide = torch.full((batch * new, heads + 1, dim), 3.0, dtype=q.dtype, device=DEV)
+    lse = torch.full((batch * new, heads), 3.0, device=DEV)
+    args = dict(q_start=start, max_q=new)
+    bf.attn_kv4(q, b.pages, b.table, b.kv_len, out=wide[:, 1:], lse=lse, **args)
+    assert bf.stream_status() == 0
+    assert not bool(wide[new:, 1:].any()) and bool((wide[:, 0] == 3.0).all()) and bool((lse[new:] == -float("inf")).all())
+    alone = bf.attn_kv4(q[:new], b.pages, b.table[:1].contiguous(), b.kv_len[:1].contiguous(), q_start=start[:2].contiguous(),
+                        max_q=new)
+    assert bool(wide[:new, 1:].any()) and torch.allclose(wide[:new, 1:].float(), alone.float(), rtol=2e-2, atol=2e-3)
+    full = Batch([64 + new] * batch, 8, dim, seed=new)
+    out = torch.empty_like(q)
+    padded = _event_us(lambda: bf.attn_kv4(q, b.pages, b.table, b.kv_len, out=out, **args))
+    whole = _event_us(lambda: bf.attn_kv4(q, full.pages, full.table, full.kv_len, out=out, **args))
+    assert padded <= 1.5 * whole + 10.0, (padded, whole)
