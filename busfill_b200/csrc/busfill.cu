@@ -9,10 +9,13 @@
 #include <atomic>
 #include <cstdint>
 #include <cstring>
+#include <list>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <type_traits>
 #include <utility>
+#include <vector>
 
 #include "busfill.h"
 #include "decode_gemm.cuh"
@@ -280,9 +283,119 @@ unsigned* sweep_workspace(int dev, cudaStream_t s, int sm_count) {
   return w;
 }
 
-// The attention calls' workspace (host.h) and how many of its bytes are zero
-// between calls.
-std::map<std::pair<int, cudaStream_t>, std::pair<void*, size_t>> g_work;
+// The attention calls' workspaces (host.h), one per (device, stream), and how
+// many of their bytes are zero between calls. cudaStreamPerThread is another
+// stream in every thread, so its key is the stream's own number.
+struct Work {
+  void* ptr = nullptr;
+  size_t zeroed = 0;
+};
+using WorkKey = std::tuple<int, bool, unsigned long long>;
+std::map<WorkKey, Work> g_work;
+
+WorkKey work_key(int dev, cudaStream_t s) {
+  unsigned long long id = 0;
+  if (s == cudaStreamPerThread && cudaStreamGetId(s, &id) == cudaSuccess) return {dev, true, id};
+  return {dev, false, reinterpret_cast<uintptr_t>(s)};
+}
+
+// Captured calls: a graph runs on any stream, beside eager calls on the one it
+// was captured on and beside other graphs, so every capture has workspaces of
+// its own, one per stream that takes part in it (its calls on one stream run one
+// after another). The graph owns them through a user object; when it and what
+// was instantiated from it are gone, a later capture takes them over.
+struct CapturedWork {
+  int dev;
+  cudaStream_t stream;
+  unsigned long long capture;
+  size_t bytes;
+  Work work;
+};
+struct CapturedWorks {
+  std::mutex mu;   // no CUDA call under it: graphs give their workspaces back from a thread of the driver
+  std::list<CapturedWork> used, spare;
+};
+CapturedWorks& captured_works() {   // lives as long as any graph
+  static CapturedWorks& w = *new CapturedWorks;
+  return w;
+}
+void give_back(void* entry) {
+  CapturedWorks& all = captured_works();
+  std::lock_guard<std::mutex> lk(all.mu);
+  for (auto it = all.used.begin(); it != all.used.end(); ++it)
+    if (&*it == entry) {
+      all.spare.splice(all.spare.end(), all.used, it);
+      return;
+    }
+}
+
+// Zero the first `bytes` of p, waiting only for that.
+bool zero_apart(void* p, size_t bytes) {
+  cudaStream_t h;
+  if (cudaStreamCreateWithFlags(&h, cudaStreamNonBlocking) != cudaSuccess) return false;
+  const bool ok = cudaMemsetAsync(p, 0, bytes, h) == cudaSuccess && cudaStreamSynchronize(h) == cudaSuccess;
+  return cudaStreamDestroy(h) == cudaSuccess && ok;
+}
+
+int captured_workspace(int dev, cudaStream_t s, unsigned long long capture, cudaGraph_t graph, size_t bytes,
+                       size_t zeroed, void** out) {
+  CapturedWorks& all = captured_works();
+  std::list<CapturedWork> mine;
+  {
+    std::lock_guard<std::mutex> lk(all.mu);
+    for (const CapturedWork& w : all.used)
+      if (w.dev == dev && w.stream == s && w.capture == capture && w.bytes == bytes) {
+        *out = w.work.ptr;
+        return BUSFILL_OK;
+      }
+    for (auto it = all.spare.begin(); it != all.spare.end(); ++it)
+      if (it->dev == dev && it->bytes == bytes) {
+        mine.splice(mine.end(), all.spare, it);
+        break;
+      }
+  }
+  // allocations and waits that have nothing to do with the capture are let through
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) {
+    cudaGetLastError();
+    std::lock_guard<std::mutex> lk(all.mu);
+    all.spare.splice(all.spare.end(), mine);
+    return BUSFILL_ERR_CUDA;
+  }
+  int st = BUSFILL_OK;
+  if (mine.empty()) {
+    void* p = nullptr;
+    if (cudaMalloc(&p, bytes) == cudaSuccess) {
+      ++g_internal_allocs;
+      mine.push_back(CapturedWork{dev, s, capture, bytes, Work{p, zeroed}});
+    } else {
+      st = BUSFILL_ERR_ALLOC;
+    }
+  }
+  cudaUserObject_t owner = nullptr;
+  if (st == BUSFILL_OK) {
+    CapturedWork& w = mine.front();
+    w.stream = s;
+    w.capture = capture;
+    w.work.zeroed = zeroed;
+    if (!zero_apart(w.work.ptr, zeroed) ||
+        cudaUserObjectCreate(&owner, &w, give_back, 1, cudaUserObjectNoDestructorSync) != cudaSuccess)
+      st = BUSFILL_ERR_CUDA;
+  }
+  {
+    std::lock_guard<std::mutex> lk(all.mu);   // listed before the graph can give it back
+    if (st == BUSFILL_OK) *out = mine.front().work.ptr;
+    std::list<CapturedWork>& to = st == BUSFILL_OK ? all.used : all.spare;
+    to.splice(to.end(), mine);
+  }
+  if (st == BUSFILL_OK && cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaUserObjectRelease(owner, 1);   // back to the spare ones
+    st = BUSFILL_ERR_CUDA;
+  }
+  if (st != BUSFILL_OK) cudaGetLastError();
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return st;
+}
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -1084,10 +1197,18 @@ int context(cudaStream_t s, Context* out) {
   return get_error_words(out->dev, s, &out->error);
 }
 
-int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t zeroed, void** out) {
+int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t captured_bytes, size_t zeroed, void** out) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(s, &status, &capture, &graph) != cudaSuccess)
+    cudaGetLastError();
+  else if (status == cudaStreamCaptureStatusActive)
+    return captured_workspace(c.dev, s, capture, graph, captured_bytes, zeroed, out);
   std::lock_guard<std::mutex> lk(g_mu);
-  void*& w = g_work[{c.dev, s}].first;
-  g_work[{c.dev, s}].second = zeroed;
+  Work& work = g_work[work_key(c.dev, s)];
+  work.zeroed = zeroed;
+  void*& w = work.ptr;
   if (!w) {
     if (capturing(s)) return BUSFILL_ERR_ALLOC;
     if (cudaMalloc(&w, bytes) != cudaSuccess) {
@@ -1535,9 +1656,21 @@ int busfill_stream_status_ex(void* stream, unsigned* bits) {
   auto sw = g_sweep.find({dev, s});
   if (sw != g_sweep.end() && sw->second && cudaMemset(sw->second, 0, (size_t)sweep::kFlagWords * 4) != cudaSuccess)
     return BUSFILL_ERR_CUDA;
-  auto wk = g_work.find({dev, s});
-  if (wk != g_work.end() && wk->second.first && cudaMemset(wk->second.first, 0, wk->second.second) != cudaSuccess)
+  auto wk = g_work.find(work_key(dev, s));
+  if (wk != g_work.end() && wk->second.ptr && cudaMemset(wk->second.ptr, 0, wk->second.zeroed) != cudaSuccess)
     return BUSFILL_ERR_CUDA;
+  if (err & ~kErrIndex) {   // the graphs captured on the stream report here too, wherever they run
+    std::vector<Work> of_graphs;
+    {
+      CapturedWorks& all = captured_works();
+      std::lock_guard<std::mutex> lk2(all.mu);
+      for (const CapturedWork& w : all.used)
+        if (w.dev == dev && w.stream == s) of_graphs.push_back(w.work);
+    }
+    if (!of_graphs.empty() && cudaDeviceSynchronize() != cudaSuccess) return BUSFILL_ERR_CUDA;
+    for (const Work& w : of_graphs)
+      if (cudaMemset(w.ptr, 0, w.zeroed) != cudaSuccess) return BUSFILL_ERR_CUDA;
+  }
   return err == kErrIndex ? BUSFILL_ERR_DEVICE_INDEX : BUSFILL_ERR_DEVICE_TIMEOUT;
 }
 

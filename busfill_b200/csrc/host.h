@@ -24,10 +24,10 @@ struct Context {
 // Current device (must be sm_100) and the stream's error words; a busfill_status.
 int context(cudaStream_t s, Context* out);
 
-// The stream's workspace of the attention calls: `bytes` are the same in
-// every call, and the first `zeroed` of them are zero when it is made. Never
-// made while the stream is capturing (BUSFILL_ERR_ALLOC).
-int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t zeroed, void** out);
+// The workspace of an attention call: the stream's, of `bytes` in every call,
+// or, while the stream is capturing, one of `captured_bytes` that belongs to the
+// graph. The first `zeroed` bytes are zero when it is made.
+int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t captured_bytes, size_t zeroed, void** out);
 
 int launch(const void* kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, void** args);
 

@@ -82,14 +82,19 @@ constexpr int kTwoTileRows = 25;
 // between a call's two kernels, then the largest kernel's partial results.
 constexpr size_t kCounterBytes = 4096;
 constexpr int kMaxCtas = kCounterBytes / 4 - 1;
-size_t workspace_bytes(int sms) {
+// What calls that do not take prompt_kernel need of it (2.4 MB), and all calls (39 MB).
+size_t few_rows_bytes(int sms) {
   size_t f = part_floats<64, 2>();
   f = std::max(f, part_floats<128, 1>());
   f = std::max(f, part_floats<256, 1>());
-  f = std::max(f, (size_t)2 * prompt::Geo<64>::kPartFloats);
+  f = std::max(f, (size_t)2 * wsum::Geo<128>::kTokens);
+  return kCounterBytes + (size_t)sms * f * sizeof(float);
+}
+size_t workspace_bytes(int sms) {
+  size_t f = (size_t)2 * prompt::Geo<64>::kPartFloats;
   f = std::max(f, (size_t)2 * prompt::Geo<128>::kPartFloats);
   f = std::max(f, (size_t)2 * prompt::Geo<256>::kPartFloats);
-  return kCounterBytes + (size_t)sms * f * sizeof(float);
+  return std::max(few_rows_bytes(sms), kCounterBytes + (size_t)sms * f * sizeof(float));
 }
 
 template <int D, int NT>
@@ -279,8 +284,11 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   host::Context ctx;
   st = host::context(s, &ctx);
   if (st != BUSFILL_OK || a->tokens == 0) return st;
+  const int max_q = a->q_start ? a->max_q : 1, rows = max_q * (a->q_heads / cache->heads);
+  const bool many = rows >= prompt_rows(cache->head_dim) && (long long)a->tokens * a->q_heads >= kPromptTotal;
   void* work = nullptr;
-  st = host::workspace(ctx, s, workspace_bytes(ctx.sms), kCounterBytes, &work);
+  st = host::workspace(ctx, s, workspace_bytes(ctx.sms), many ? workspace_bytes(ctx.sms) : few_rows_bytes(ctx.sms),
+                       kCounterBytes, &work);
   if (st != BUSFILL_OK) return st;
   AttnParams p{};
   p.c = view_of(cache);
@@ -290,7 +298,7 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.scale_log2 = a->scale * kLog2e;
   p.tokens = a->tokens, p.q_heads = a->q_heads, p.group = a->q_heads / cache->heads;
   p.by_group = divide_by((unsigned)p.group);
-  p.max_q = a->q_start ? a->max_q : 1;
+  p.max_q = max_q;
   // a window as long as the table can hold is none (and stays clear of the end of int)
   p.causal = a->causal != 0, p.window = a->window < (int64_t)kPage * cache->table_cols ? a->window : 0, p.bf16 = a->dtype == BUSFILL_TYPE_BF16;
   p.wide_out = aligned(a->out, 32) && (a->out_token | a->out_head) % 16 == 0;
@@ -299,10 +307,8 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounterBytes);
   p.error = ctx.error;
   if (ctx.sms > kMaxCtas) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
-  const int rows = p.max_q * p.group;
   st = by_dim(cache->head_dim, [&](auto d) {
-    if (rows >= prompt_rows(d()) && (long long)p.tokens * p.q_heads >= kPromptTotal)
-      return launch_prompt<d()>(p, ctx, s);
+    if (many) return launch_prompt<d()>(p, ctx, s);
     if constexpr (d() == 64) {
       if (rows >= kTwoTileRows) return launch_attn<d(), 2>(p, ctx, s);
     }

@@ -471,8 +471,14 @@ BUSFILL_API int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_star
  * call's rows give slot s of their sequence, summed over rows and over the
  * heads of the group, is added to weights[.][.][s]; needs lse, and
  * weights_cols >= 64 * table_cols. All results are bitwise repeatable. The
- * first call on a stream makes its workspace (not inside a graph capture:
- * BUSFILL_ERR_ALLOC). */
+ * first call on a stream makes its workspace (39 MB); calls on one stream share
+ * it in stream order. Captured calls do not: each capture gets a workspace of
+ * its own per capturing stream (2.4 MB, 39 MB for calls of many rows), which
+ * goes back to the library with the graph, so a graph may run on any stream,
+ * beside other graphs and calls. (Two instances of one graph share theirs and
+ * must not overlap.) Failures of captured calls show in the status of the
+ * stream that they were captured on; that stream needs one call of the library
+ * before the capture (BUSFILL_ERR_ALLOC without). */
 typedef struct busfill_attn {
   const void* q;
   void* out;

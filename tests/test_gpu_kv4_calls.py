@@ -190,3 +190,131 @@ def test_rows_of_empty_sequences_are_zero_and_cost_little(dim, new, dtype):
     padded = _event_us(lambda: bf.attn_kv4(q, b.pages, b.table, b.kv_len, out=out, **args))
     whole = _event_us(lambda: bf.attn_kv4(q, full.pages, full.table, full.kv_len, out=out, **args))
     assert padded <= 1.5 * whole + 10.0, (padded, whole)
+
+
+# ---------------------------------------------------------------------------
+# graphs and streams side by side
+# ---------------------------------------------------------------------------
+def _captured(stream, calls):
+    import torch
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(g, stream=stream):
+            for f in calls:
+                f()
+    return g
+
+
+def test_every_capture_has_a_workspace_of_its_own_and_gives_it_back():
+    import gc
+    import time
+    import torch
+    b = Batch([5000], 2, 128, seed=1)
+    q, out = _rand((1, 16, 128), 2), torch.empty((1, 16, 128), dtype=torch.float16, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    call = [lambda: bf.attn_kv4(q, b.pages, b.table, b.kv_len, out=out, stream=side)]
+    call[0]()
+    side.synchronize()
+    want = out.clone()
+    gc.collect()
+    time.sleep(0.5)
+    count, held = bf.internal_allocations(), []
+    while bf.internal_allocations() == count and len(held) < 100:    # what earlier graphs gave back
+        held.append(_captured(side, call))
+    count = bf.internal_allocations()
+    one = _captured(side, call * 3)          # one for all of a capture's calls
+    two = _captured(side, call)
+    assert bf.internal_allocations() == count + 2
+    for g in (one, two):
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    del one, g
+    gc.collect()
+    torch.cuda.synchronize()
+    count = bf.internal_allocations()
+    for _ in range(50):                      # the driver gives it back from a thread of its own
+        time.sleep(0.1)
+        three = _captured(side, call)
+        if bf.internal_allocations() == count:
+            break
+        held.append(three)
+        count = bf.internal_allocations()
+    else:
+        pytest.fail("no workspace came back")
+    out.zero_()
+    torch.cuda.synchronize()
+    three.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and bf.stream_status(side) == 0
+
+
+@pytest.mark.parametrize("new", [1, 80])
+def test_graphs_of_one_stream_run_beside_each_other_and_beside_its_calls(new):
+    import torch
+    side, others = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    b = [Batch([9000 + 700 * i, 40 + new, 3000], 2, 128, seed=i) for i in range(3)]
+    q = [_rand((3 * new, 16, 128), 5 + i) for i in range(3)]
+    start = b[0].starts([new] * 3)
+    out = [torch.empty_like(x) for x in q]
+    lse = [torch.zeros((3 * new, 16), device=DEV) for _ in q]
+    w = [torch.zeros((3, 2, 64 * x.cols), device=DEV) for x in b]
+    torch.cuda.synchronize()
+
+    def call(i):
+        return lambda: bf.attn_kv4(q[i], b[i].pages, b[i].table, b[i].kv_len, q_start=start, max_q=new, out=out[i],
+                                   lse=lse[i], weights=w[i], stream=side)
+
+    want, total = [], []          # of the same calls one after another
+    for i in range(3):
+        for _ in range(80):
+            call(i)()
+        side.synchronize()
+        want.append(out[i].clone())
+        total.append(w[i].clone())
+        w[i].zero_()
+    torch.cuda.synchronize()
+    graphs = [_captured(side, [call(0)] * 4), _captured(side, [call(1)] * 4)]
+    for _ in range(20):
+        for s, g in zip(others, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        for _ in range(4):
+            call(2)()
+    torch.cuda.synchronize()
+    assert bf.stream_status(side) == 0
+    for i in range(3):
+        assert torch.equal(out[i], want[i]) and torch.equal(w[i], total[i])
+
+
+def test_threads_on_their_own_default_streams_share_no_workspace():
+    """cudaStreamPerThread is one handle and a stream in every thread."""
+    import threading
+    import torch
+    b = [Batch([9000 + 700 * i, 3000], 2, 128, seed=i) for i in range(2)]
+    q = [_rand((2, 16, 128), 5 + i) for i in range(2)]
+    out = [torch.empty_like(x) for x in q]
+    want = [bf.attn_kv4(q[i], b[i].pages, b[i].table, b[i].kv_len) for i in range(2)]
+    torch.cuda.synchronize()
+    per_thread = torch.cuda.ExternalStream(2)
+    wrong = []
+
+    def work(i):
+        for _ in range(60):
+            for _ in range(5):
+                bf.attn_kv4(q[i], b[i].pages, b[i].table, b[i].kv_len, out=out[i], stream=per_thread)
+            per_thread.synchronize()
+            if not torch.equal(out[i], want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    before = bf.internal_allocations()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and bf.stream_status(per_thread) == 0
+    assert bf.internal_allocations() == before + 3      # two workspaces and the handle's error words
