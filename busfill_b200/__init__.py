@@ -23,7 +23,7 @@ __all__ = [
     "gemm_q4_0", "gemm_q4k", "gemm_q4_0_ggml", "gemm_q4k_swiglu", "gemm_q4k_sweep", "SweepOp", "gemm_q4k_noalloc", "gemm_q5k", "gemm_q6k", "repack_q6k",
     "busfill_q4", "repack_q4k_planar", "gemm_q4k_planar", "Tensor", "tensor_desc", "mul_mat", "dequant_q4_0", "dequant_q4_0_ggml", "dequant_q4k", "dequant_q5k", "dequant_q6k",
     "stream_status", "stream_status_bits", "noalloc_status", "internal_allocations", "set_pdl", "set_ksplit", "set_prefill_min_m", "set_exact_kquant", "uses_prefill", "gemm_launches", "probe_umma", "version",
-    "KV4_PAGE", "kv4_page_bytes", "kv4_pool", "rope_table", "rope_axes", "kv4_append", "kv4_read", "attn_kv4", "kv4_evict",
+    "KV4_PAGE", "kv4_page_bytes", "kv4_pool", "rope_table", "rope_axes", "kv4_append", "kv4_read", "attn_kv4", "attn_kv4_kernel", "kv4_evict",
 ]
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -103,6 +103,7 @@ _SIGS = {
     "busfill_kv4_append": [_P, _P, _P],
     "busfill_kv4_read": [_P, _P, _I, _P, _P, _P],
     "busfill_attn_kv4": [_P, _P, _P],
+    "busfill_attn_kv4_kernel_for": [_I, _I, _I, _I, _I],
     "busfill_kv4_evict": [_P, _P, _P],
 }
 
@@ -558,5 +559,5 @@ def probe_umma(a, b, nb, stream=None):
     return d
 
 
-from .kv4 import (KV4_PAGE, attn_kv4, kv4_append, kv4_evict, kv4_page_bytes, kv4_pool, kv4_read, rope_axes,  # noqa: E402
-                  rope_table)
+from .kv4 import (KV4_PAGE, attn_kv4, attn_kv4_kernel, kv4_append, kv4_evict, kv4_page_bytes, kv4_pool,  # noqa: E402
+                  kv4_read, rope_axes, rope_table)

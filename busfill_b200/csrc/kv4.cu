@@ -78,6 +78,14 @@ constexpr long long kMaxGrid = 2147483647;
 // of 4096, heads of 128: 32 rows 49 / 68).
 constexpr int kTwoTileRows = 25;
 
+// The kernels of a call: busfill_attn_kv4_kernel_for.
+enum { kFewRows = 0, kFewRowsTwoTiles = 1, kManyRows = 2, kWeightsManyRows = 4 };
+int choose(long long all_rows, int rows, int head_dim) {
+  const int weights = rows >= kWeightsRows ? kWeightsManyRows : 0;
+  if (rows >= prompt_rows(head_dim) && all_rows >= kPromptTotal) return kManyRows | weights;
+  return (head_dim == 64 && rows >= kTwoTileRows ? kFewRowsTwoTiles : kFewRows) | weights;
+}
+
 // Workspace of the attention calls on a stream: a counter per CTA, a word
 // between a call's two kernels, then the largest kernel's partial results.
 constexpr size_t kCounterBytes = 4096;
@@ -285,10 +293,10 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   st = host::context(s, &ctx);
   if (st != BUSFILL_OK || a->tokens == 0) return st;
   const int max_q = a->q_start ? a->max_q : 1, rows = max_q * (a->q_heads / cache->heads);
-  const bool many = rows >= prompt_rows(cache->head_dim) && (long long)a->tokens * a->q_heads >= kPromptTotal;
+  const int kernels = choose((long long)a->tokens * a->q_heads, rows, cache->head_dim);
   void* work = nullptr;
-  st = host::workspace(ctx, s, workspace_bytes(ctx.sms), many ? workspace_bytes(ctx.sms) : few_rows_bytes(ctx.sms),
-                       kCounterBytes, &work);
+  const size_t bytes = workspace_bytes(ctx.sms);
+  st = host::workspace(ctx, s, bytes, kernels & kManyRows ? bytes : few_rows_bytes(ctx.sms), kCounterBytes, &work);
   if (st != BUSFILL_OK) return st;
   AttnParams p{};
   p.c = view_of(cache);
@@ -308,14 +316,22 @@ int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stre
   p.error = ctx.error;
   if (ctx.sms > kMaxCtas) return BUSFILL_ERR_UNSUPPORTED_DEVICE;
   st = by_dim(cache->head_dim, [&](auto d) {
-    if (many) return launch_prompt<d()>(p, ctx, s);
+    if (kernels & kManyRows) return launch_prompt<d()>(p, ctx, s);
     if constexpr (d() == 64) {
-      if (rows >= kTwoTileRows) return launch_attn<d(), 2>(p, ctx, s);
+      if (kernels & kFewRowsTwoTiles) return launch_attn<d(), 2>(p, ctx, s);
     }
     return launch_attn<d(), 1>(p, ctx, s);
   });
   if (st != BUSFILL_OK || !a->weights) return st;
-  return by_dim(cache->head_dim, [&](auto d) { return launch_weights<d()>(p, ctx, s, rows >= kWeightsRows); });
+  const bool many = (kernels & kWeightsManyRows) != 0;
+  return by_dim(cache->head_dim, [&](auto d) { return launch_weights<d()>(p, ctx, s, many); });
+}
+
+int busfill_attn_kv4_kernel_for(int tokens, int q_heads, int heads, int head_dim, int max_q) {
+  if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || tokens < 0 || heads < 1 || heads > 65535 ||
+      q_heads < 1 || q_heads % heads != 0 || max_q < 1 || (long long)max_q * (q_heads / heads) > (1 << 30))
+    return BUSFILL_ERR_SHAPE;
+  return choose((long long)tokens * q_heads, max_q * (q_heads / heads), head_dim);
 }
 
 int busfill_kv4_evict(const busfill_kv4* cache, const busfill_kv4_eviction* e, void* stream) {

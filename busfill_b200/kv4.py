@@ -322,6 +322,14 @@ def attn_kv4(q, pages, table, kv_len, q_start=None, max_q=None, scale=None, caus
     return out
 
 
+def attn_kv4_kernel(tokens: int, q_heads: int, kv_heads: int, head_dim: int, max_q: int) -> tuple:
+    """(row tiles of a warp, or 0 for the kernel of many rows; whether the kernel of many rows sums the
+    weights) of an :func:`attn_kv4` call of that shape (busfill_attn_kv4_kernel_for)."""
+    n = _lib().busfill_attn_kv4_kernel_for(int(tokens), int(q_heads), int(kv_heads), int(head_dim), int(max_q))
+    _check(min(n, 0), "busfill_attn_kv4_kernel_for")
+    return (1, 2, 0)[n & 3], bool(n & 4)
+
+
 def kv4_evict(pages, table, kv_len, weights, keep, recent, out_table=None, weights_out=None, stream=None):
     """Bring every sequence longer than ``keep`` down to ``keep`` tokens, head by head: the last
     ``recent`` stay, and of the others those with the largest accumulated weights (the lower slot of

@@ -494,6 +494,14 @@ typedef struct busfill_attn {
 } busfill_attn;
 BUSFILL_API int busfill_attn_kv4(const busfill_kv4* cache, const busfill_attn* a, void* stream);
 
+/* Which kernel an attention call of `tokens` rows and q_heads query heads over
+ * `heads` key/value heads of head_dim, with at most max_q rows a sequence,
+ * runs: 0 = few rows (mma.sync), 1 = few rows in two row tiles (heads of 64),
+ * 2 = many rows (tcgen05); 4 is added where its weights are summed by the
+ * kernel of many rows. BUSFILL_ERR_SHAPE for shapes that busfill_attn_kv4
+ * refuses. Diagnostic; no reference counterpart. */
+BUSFILL_API int busfill_attn_kv4_kernel_for(int tokens, int q_heads, int heads, int head_dim, int max_q);
+
 /* Eviction by accumulated attention weight, for each sequence and head by
  * itself: of a sequence longer than `keep`, the last `recent` tokens stay and
  * of the others the keep - recent with the largest weights (the lower slot of
