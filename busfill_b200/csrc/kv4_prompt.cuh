@@ -104,7 +104,7 @@ __device__ __forceinline__ void normalize_query8(uint4& v, int bf16, float sign,
     const int ex = e == 0 || e == 255 ? 0 : max(-126, min(126, 136 - (int)e));
     const __nv_bfloat162 up = __bfloat162bfloat162(
         __ushort_as_bfloat16((unsigned short)((127 + ex) << 7 | (sign < 0.0f ? 0x8000 : 0))));
-    fac *= __uint_as_float((unsigned)(127 - ex) << 23);
+    fac = fmaxf(fac * __uint_as_float((unsigned)(127 - ex) << 23), 1e-37f);   // not 0: -inf * fac stays -inf
     auto half = [&](uint32_t u) {
       const uint32_t x = bits(__hmul2(pair(u), up));   // exact
       return h2_as_u32(__floats2half2_rn(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)));
