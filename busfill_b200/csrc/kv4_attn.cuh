@@ -108,27 +108,29 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 // What a sequence asks for: its rows, and the pages that some row of it sees.
 struct Span {
-  int first, n;     // rows of the step's tensors
+  int first, n;     // rows of the step's tensors, max_q at most
   int len;          // cached tokens
+  int past;         // cached tokens before the first row's own (negative: rows that see nothing)
   int page0, pages; // pages [page0, page0 + pages)
 };
 __device__ __forceinline__ Span span_of(const AttnParams& p, int b, bool& bad) {
   Span s;
   rows_of(p.q_start, b, p.tokens, s.first, s.n, bad);
+  s.len = cached(p.c, b, bad);
+  s.past = s.len - s.n;
   if (s.n > p.max_q) {
     bad = true;
     s.n = p.max_q;
   }
-  s.len = cached(p.c, b, bad);
-  const int lo = p.window > 0 ? max(0, s.len - s.n + 1 - p.window) : 0;
+  const int lo = p.window > 0 ? max(0, min(s.past + 1 - p.window, s.len - 1)) : 0;
   s.page0 = lo / kPage;
   s.pages = s.n > 0 && s.len > 0 ? (s.len + kPage - 1) / kPage - s.page0 : 0;
   return s;
 }
 // slots [lo, hi) that row i of the span sees
 __device__ __forceinline__ void sees(const AttnParams& p, const Span& s, int i, int& lo, int& hi) {
-  hi = p.causal ? min(s.len, s.len - s.n + i + 1) : s.len;
-  lo = p.window > 0 ? max(0, s.len - s.n + i + 1 - p.window) : 0;
+  hi = p.causal ? min(s.len, s.past + i + 1) : s.len;
+  lo = p.window > 0 ? max(0, s.past + i + 1 - p.window) : 0;
 }
 
 // The warp's sum.
@@ -999,7 +1001,7 @@ __global__ void __launch_bounds__(WeightsGeo<D>::kWarps * 32, 1) weights_kernel(
     int stage = 0;
     uint32_t parity = 0;
     for (int u = u0; u < u1; ++u) {
-      const int base = c.page * kPage, past = c.s.len - c.s.n;
+      const int base = c.page * kPage, past = c.s.past;
       // lane 4r's slots, read ahead
       float* out = p.weights + ((size_t)c.b * p.c.heads + c.head) * p.weights_cols + base + tile_perm(lane >> 2);
       float sum[4][2];

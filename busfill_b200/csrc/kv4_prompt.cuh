@@ -180,7 +180,7 @@ struct Item {
 struct Work {
   int b, head, first, n;         // first row and rows of the sequence
   int len, row0, tile0, tiles;   // tiles 0: the end
-  int page0;                     // the first page that some row of the sequence sees
+  int page0, past;               // of the sequence's Span
   int kind, c_first, c_last, row_tiles;
 };
 enum { kWhole = 0, kTail = 1, kHead = 2 };   // kTail: began in an earlier CTA; kHead: goes on in the next
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           if (to > from) {
             Work y;
             y.b = it.b, y.head = it.head, y.first = it.s.first, y.n = it.s.n, y.len = it.s.len;
-            y.page0 = it.s.page0;
+            y.page0 = it.s.page0, y.past = it.s.past;
             y.row0 = it.t * G::kRows, y.tile0 = it.tile0 + from, y.tiles = to - from;
             y.kind = from > 0 ? kTail : to < it.tiles ? kHead : kWhole;
             y.c_first = cta_of(x + near_start(c)), y.c_last = cta_of(x + c - kSnap - 1);
@@ -685,8 +685,8 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
         // slots seen, from the piece's first token on
         int lo = 0, hi = 0x7fffffff;
         if (live) {
-          hi = (p.causal ? min(x.len, x.len - x.n + tok + 1) : x.len) - x.tile0 * K;
-          lo = (p.window > 0 ? max(0, x.len - x.n + tok + 1 - p.window) : 0) - x.tile0 * K;
+          hi = (p.causal ? min(x.len, x.past + tok + 1) : x.len) - x.tile0 * K;
+          lo = (p.window > 0 ? max(0, x.past + tok + 1 - p.window) : 0) - x.tile0 * K;
         }
         for (int j = 0; j < x.tiles; ++j, ++done, lo -= K, hi -= K) {
           if (!wait(G::bS + i, done)) break;

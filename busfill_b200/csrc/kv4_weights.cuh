@@ -66,7 +66,7 @@ __device__ __forceinline__ int tiles_of(const Span& s, int& tile0) {
 template <int D>
 __device__ __forceinline__ int blocks_of(const AttnParams& p, const Span& s, int t, int& block0) {
   constexpr int T = Geo<D>::kTokens;
-  const int base = t * T, past = s.len - s.n;
+  const int base = t * T, past = s.past;
   const int i0 = p.causal ? max(0, base - past) : 0;
   const int i1 = p.window > 0 ? min(s.n, base + T - 1 + p.window - past) : s.n;
   block0 = i0 * p.group / 128;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(wsum::kThreads, 1) weights_prompt_kernel(const
     for_pieces([&](const Item& it, int from, int blocks, int u) {
       const int slot = (it.tile0 + it.t) * G::kTokens + mine;
       // the rows that see the thread's token: [row_a, row_z)
-      const long long at = slot - (it.s.len - it.s.n);   // the row that stands at it
+      const long long at = slot - it.s.past;   // the row that stands at it
       const int row_a = p.causal ? (int)max(0ll, min(at, (long long)it.s.n)) * p.group : 0;
       const int row_z = slot >= it.s.len ? 0
                         : p.window > 0   ? (int)max(0ll, min(at + p.window, (long long)it.s.n)) * p.group

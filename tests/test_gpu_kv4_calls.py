@@ -318,3 +318,32 @@ def test_threads_on_their_own_default_streams_share_no_workspace():
         t.join()
     assert not wrong and bf.stream_status(per_thread) == 0
     assert bf.internal_allocations() == before + 3      # two workspaces and the handle's error words
+
+
+# ---------------------------------------------------------------------------
+# more rows than the caller's bound
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("new,max_q,many", [([2, 7, 1], 3, False), ([60, 150, 31], 80, True)])
+def test_rows_beyond_max_q_are_left_out_and_the_others_stay_in_place(dim, window, new, max_q, many):
+    import torch
+    lens, heads = [300, 400, 90], 16
+    b = Batch(lens, 2, dim, seed=dim)
+    assert (bf.attn_kv4_kernel(sum(new), heads, 2, dim, max_q)[0] == 0) == many
+    q, start = _rand((sum(new), heads, dim), 3), b.starts(new)
+    cut = list(range(new[0])) + list(range(new[0], new[0] + max_q)) + list(range(new[0] + new[1], sum(new)))
+    gone = list(range(new[0] + max_q, new[0] + new[1]))
+    want = bf.attn_kv4(q, b.pages, b.table, b.kv_len, q_start=start, max_q=max(new), window=window).float()
+    assert bf.stream_status() == 0
+    out, lse = torch.full_like(q, 5.0), torch.full((sum(new), heads), 5.0, device=DEV)
+    w = torch.zeros((3, 2, 64 * b.cols), device=DEV)
+    bf.attn_kv4(q, b.pages, b.table, b.kv_len, q_start=start, max_q=max_q, window=window, out=out, lse=lse, weights=w)
+    assert bf.stream_status_bits() == (-9, 256)
+    assert bool((out[gone] == 5.0).all()) and bool((lse[gone] == 5.0).all())
+    # another bound may choose another kernel: fp16 roundings apart
+    assert torch.allclose(out[cut].float(), want[cut], rtol=4e-3, atol=2e-3)
+    # every row that is there gives each of its heads a weight of 1, up to its own slot
+    rows = torch.tensor([new[0], max_q, new[2]], device=DEV)
+    assert torch.allclose(w.sum(-1), (rows * (heads // 2)).float()[:, None].expand(3, 2), rtol=1e-4)
+    assert not bool(w[1, :, lens[1] - new[1] + max_q:].any())
