@@ -18,15 +18,11 @@
 //     more matrix instruction per block (an operand of ones) adds up from
 //     the same rounded products.
 //   * Scales never touch the codes: the keys' multiply the finished block
-//     sums in fp32, the values' multiply p. p is rounded to fp16 (the
-//     transposition between the two products moves 16-bit pairs) and p d again:
-//     two roundings of 2^-11, independent from token to token. Both use fp16's
-//     whole range, so that they stay relative ones: p is at most 2^(kLift +
-//     kLag), 2^kLift at the row's reference maximum, and d is brought below 1
-//     by a power of two that follows the largest scale of the pages read. Only
-//     terms 2^-24 below the largest one lose bits (d alone at the values' own
-//     size, p at most 2^4: values of 2^-10 behind a token of weight 0.1 were
-//     off by 0.7 %, of 2^-13 by 4 %).
+//     sums in fp32, the values' multiply p, in fp32 too. p d is rounded to
+//     fp16 once (the matrix operand, and the transposition between the two
+//     products moves 16-bit pairs). It uses fp16's whole range: the row's
+//     reference is set by the largest p d of a page, so only terms 2^-25 below
+//     the largest one lose bits, whatever the size of the values.
 // The matrix instruction is m16n8k16 with the tokens (scores) or channels
 // (output) as its 16 rows and the query rows as its 8 columns, so that a
 // group of 8 query heads fills it.
@@ -41,7 +37,7 @@
 // the workspace; always in the order of the ranges, so results repeat bit for
 // bit.
 //
-// Measured, 64 query heads over 8 of 128: 32 sequences to 16000 tokens 82 us
+// Measured, 64 query heads over 8 of 128: 32 sequences to 16000 tokens 84 us
 // (353 MB, 4.3 TB/s; bulk copies of that size alone 64-74 us), one of 131071
 // 44 us (106 MB), one of 300 9 us.
 #pragma once
@@ -53,7 +49,7 @@ namespace kv4 {
 
 constexpr int kMaxBatch = 1024;
 constexpr float kLag = 4.0f;    // log2 growth of a row's maximum that is not followed
-constexpr float kLift = 11.0f;  // log2 of p at the row's reference maximum; p < 2^(kLift + kLag), with room in fp16
+constexpr float kLift = 11.0f;  // log2 of p d at the row's reference; p d < 2^(kLift + kLag), with room in fp16
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -291,19 +287,16 @@ __device__ __forceinline__ void scores_16(const uint8_t* page, int mt, int lane,
 // Running output of NT row tiles: o is channels x rows. Lane (c = lane / 4,
 // j = lane % 4) holds, of block b and half u, the channels 32b + 8(c/2) + 4u +
 // (c%2) (regs 0, 1: rows 2j, 2j + 1; in 2^24 ths) and the same + 2 (regs 2, 3; in
-// 2^20 ths); pd: sum of p d per block. Scales d enter o and pd times
-// 2^(-1 - top_d), where 2^top_d <= the largest |d| so far < 2^(top_d + 1).
-// m is the row's reference: its maximum (as far as that is followed) - kLift.
-constexpr int kLeastTopD = -15;   // 2^(-1 - top_d) is an fp16 number; smaller scales stay below 1/2
+// 2^20 ths); pd: sum of p d per block. m is the row's reference: the largest
+// log2 of a page's greatest p and greatest |d| together, as far as that is
+// followed, less kLift.
 template <int D, int NT>
 struct Running {
   float o[NT][Fmt<D>::kBlocks][2][4];
   float pd[NT][Fmt<D>::kBlocks][4];   // every row alike: a whole accumulator
   float m[NT][2], l[NT][2];
-  int top_d;
 
   __device__ __forceinline__ void clear() {
-    top_d = kLeastTopD;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -318,10 +311,11 @@ struct Running {
   }
 };
 
-// Exponent (floor of log2, within fp16's) of the largest |d| among the value
-// scales of a page's `left` first tokens. What lies behind them may be anything.
+// 2^x of it is above the largest |d| among the value scales of a page's `left`
+// first tokens (what lies behind them may be anything): -14 for fp16's
+// subnormals, or none.
 template <int D>
-__device__ __forceinline__ int top_value_scale(const uint8_t* scales, int left, int lane) {
+__device__ __forceinline__ int above_value_scales(const uint8_t* scales, int left, int lane) {
   constexpr int NB = Fmt<D>::kBlocks;
   uint32_t w[NB];   // columns 2 NB lane .. of the blocks' 64 each
   load_words<NB>(scales + lane * 4 * NB, w);
@@ -336,7 +330,7 @@ __device__ __forceinline__ int top_value_scale(const uint8_t* scales, int left, 
 #pragma unroll
   for (int i = 1; i < NB; ++i) top = __hmax2(top, __habs2(u32_as_h2(w[i])));
   const unsigned bits = __reduce_max_sync(0xffffffffu, (unsigned)__half_as_ushort(__hmax(top.x, top.y)));
-  return max(kLeastTopD, min(10, (int)(bits >> 10) - 15));
+  return min(11, (int)(bits >> 10) - 14);
 }
 
 // One page (64 tokens, slots base .. base + 63) into the running output.
@@ -346,7 +340,7 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
   using F = Fmt<D>;
   constexpr int NB = F::kBlocks;
   const int c = lane >> 2, j = lane & 3;
-  const int top_d = max(run.top_d, top_value_scale<D>(page + F::kValueScale, len - base, lane));
+  const float lift = (float)above_value_scales<D>(page + F::kValueScale, len - base, lane) - kLift;
   float s[4][NT][4];
 #pragma unroll
   for (int mt = 0; mt < 4; ++mt) scores_16<D, NT>(page, mt, lane, q, s[mt]);
@@ -374,20 +368,17 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
     for (int k = 0; k < 2; ++k) {
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], x));
-      top[k] = fmaf(top[k], q[nt].factor[k], -kLift);
+      top[k] = fmaf(top[k], q[nt].factor[k], lift);
     }
-    // The reference m follows the maximum only when that has grown by more
-    // than kLag, as most pages change some row's maximum a little.
-    if (top_d > run.top_d ||
-        __any_sync(0xffffffffu, top[0] > run.m[nt][0] + kLag || top[1] > run.m[nt][1] + kLag)) {
-      const float shrink = __uint_as_float((unsigned)(127 + run.top_d - top_d) << 23);
+    // The reference m follows only what has grown by more than kLag, as most
+    // pages change some row's maximum a little.
+    if (__any_sync(0xffffffffu, top[0] > run.m[nt][0] + kLag || top[1] > run.m[nt][1] + kLag)) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float m = fmaxf(run.m[nt][k], top[k]);
-        float f = m == run.m[nt][k] ? 1.0f : exp2_approx(run.m[nt][k] - m);
+        const float f = m == run.m[nt][k] ? 1.0f : exp2_approx(run.m[nt][k] - m);
         run.m[nt][k] = m;
         run.l[nt][k] *= f;
-        f *= shrink;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -407,18 +398,10 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
         run.l[nt][e & 1] += s[mt][nt][e];
       }
   }
-  run.top_d = top_d;
-  const __half2 lift_d = __half2half2(__ushort_as_half((unsigned short)((14 - top_d) << 10)));   // 2^(-1 - top_d)
   const uint8_t* vals = page + F::kValue;
   const uint8_t* vsc = page + F::kValueScale;
 #pragma unroll
   for (int mt = 0; mt < 4; ++mt) {
-    uint32_t p0[NT], p1[NT];   // rows (columns of the operand) x tokens 2j, 2j + 1 of each 8-token tile
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      p0[nt] = transpose_8x8(h2_as_u32(__floats2half2_rn(s[mt][nt][0], s[mt][nt][1])));
-      p1[nt] = transpose_8x8(h2_as_u32(__floats2half2_rn(s[mt][nt][2], s[mt][nt][3])));
-    }
     const int ta = 16 * mt + tile_perm(2 * j), tb = 16 * mt + tile_perm(2 * j + 1);
     uint32_t w[4][NB / 2];
     load_words<NB / 2>(vals + ta * F::kRow + (c ^ value_swizzle<D>(ta)) * 2 * NB, w[0]);
@@ -429,14 +412,13 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
     const int left = len - base - 16 * mt;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      uint32_t d0 = *reinterpret_cast<const uint32_t*>(vsc + (b * kPage + 16 * mt + 2 * j) * 2);
-      uint32_t d1 = *reinterpret_cast<const uint32_t*>(vsc + (b * kPage + 16 * mt + 8 + 2 * j) * 2);
+      // scales of the tokens whose scores the lane holds (column c: token tile_perm(c))
+      const __half* sc = reinterpret_cast<const __half*>(vsc) + b * kPage + 16 * mt + c;
+      float d0 = __half2float(sc[0]), d1 = __half2float(sc[8]);
       if (left < 16) {
-        const int a = tile_perm(2 * j), bb = tile_perm(2 * j + 1);
-        d0 &= (a < left ? 0xffffu : 0u) | (bb < left ? 0xffff0000u : 0u);
-        d1 &= (a + 8 < left ? 0xffffu : 0u) | (bb + 8 < left ? 0xffff0000u : 0u);
+        if (tile_perm(c) >= left) d0 = 0.0f;
+        if (tile_perm(c) + 8 >= left) d1 = 0.0f;
       }
-      const __half2 e0 = __hmul2(u32_as_h2(d0), lift_d), e1 = __hmul2(u32_as_h2(d1), lift_d);
       const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
       const uint32_t x0 = prmt(w[0][b / 2], w[1][b / 2], sel), x1 = prmt(w[2][b / 2], w[3][b / 2], sel);
       const uint32_t a0[4] = {x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u};
@@ -445,8 +427,12 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
       const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const uint32_t pb[2] = {h2_as_u32(__hmul2(u32_as_h2(p0[nt]), e0)),
-                                h2_as_u32(__hmul2(u32_as_h2(p1[nt]), e1))};
+        // rows (columns of the operand) x tokens 2j, 2j + 1 of each 8-token tile
+        float x[4] = {s[mt][nt][0], s[mt][nt][1], s[mt][nt][2], s[mt][nt][3]};
+        mul_f32x2(x[0], x[1], d0);
+        mul_f32x2(x[2], x[3], d1);
+        const uint32_t pb[2] = {transpose_8x8(h2_as_u32(__floats2half2_rn(x[0], x[1]))),
+                                transpose_8x8(h2_as_u32(__floats2half2_rn(x[2], x[3])))};
         mma_16816(run.o[nt][b][0], a0, pb);
         mma_16816(run.o[nt][b][1], a1, pb);
         mma_16816(run.pd[nt][b], ones, pb);
@@ -459,7 +445,6 @@ __device__ __forceinline__ void attend_page(const uint8_t* page, int base, int l
 // row sums l over the warp.
 template <int D, int NT>
 __device__ __forceinline__ void settle(Running<D, NT>& run) {
-  const float unit = __uint_as_float((unsigned)(128 + run.top_d) << 23);   // of o and pd
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -471,8 +456,7 @@ __device__ __forceinline__ void settle(Running<D, NT>& run) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         run.o[nt][b][e >> 2][e & 3] =
-            fmaf(run.o[nt][b][e >> 2][e & 3], (e & 2 ? 1048576.0f : 16777216.0f) * unit,
-                 -8.0f * unit * run.pd[nt][b][e & 1]);
+            fmaf(run.o[nt][b][e >> 2][e & 3], e & 2 ? 1048576.0f : 16777216.0f, -8.0f * run.pd[nt][b][e & 1]);
   }
 }
 template <int D>

@@ -138,7 +138,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool h
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// (a, b) = (a, b) * s + t and (a, b) += t as packed fp32 pairs (sm_100)
+// (a, b) = (a, b) * s + t, (a, b) * s and (a, b) += t as packed fp32 pairs (sm_100)
 __device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float t) {
   asm("{\n\t.reg .b64 x, y, z;\n\t"
       "mov.b64 x, {%0, %1};\n\t"
@@ -148,6 +148,15 @@ __device__ __forceinline__ void fma_f32x2(float& a, float& b, float s, float t) 
       "mov.b64 {%0, %1}, x;\n\t}"
       : "+f"(a), "+f"(b)
       : "f"(s), "f"(t));
+}
+__device__ __forceinline__ void mul_f32x2(float& a, float& b, float s) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %2};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(s));
 }
 __device__ __forceinline__ void add_f32x2(float& a, float& b, float x, float y) {
   asm("{\n\t.reg .b64 x, y;\n\t"

@@ -110,3 +110,26 @@ def test_rows_keep_what_lies_far_below_a_sink_without_value(dim, rows, n, causal
     out = bf.attn_kv4(wide, pages, table, kv_len, q_start=start, max_q=rows, causal=causal)
     assert bf.stream_status() == 0
     _check_wide(q, out, k, v, causal, 100 if rows < 8 else 3)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 5, 100])
+def test_products_are_rounded_once(dim, rows):
+    """Where the sum of p v nearly cancels, the output's own rounding is small and the rms error against
+    the root of the sum of (p v)^2 is that of p v's roundings. One to fp16, of log-uniform mantissas m
+    in [1, 2): 2^-10 / sqrt(12) * sqrt(E[1 / m^2]) with E = 3 / (8 ln 2), 2.07e-4; two: sqrt(2) more."""
+    import torch
+    n, batch = 400, 600 // rows
+    one = 2.0 ** -10 / 12 ** 0.5 * (3 / (8 * np.log(2))) ** 0.5
+    _, pages, table, kv_len, k, v = _sequence(n, dim, 1, 1, 0, seed=dim + rows)
+    q = torch.randn((batch * rows, HEADS, dim), generator=torch.Generator().manual_seed(rows)).half()
+    _, table, kv_len, start = _wide(q[:rows], table, kv_len, batch)
+    out = bf.attn_kv4(q.to(DEV), pages, table, kv_len, q_start=start, max_q=rows, causal=False).double().cpu().numpy()
+    assert bf.stream_status() == 0
+    x = q.double().numpy().reshape(-1, dim)
+    ref, _, p = orc.attention(x, k, v, dim ** -0.5, orc.seen(len(x), n, False))
+    spread = np.sqrt((p * p) @ (v * v))
+    near = np.abs(ref) < spread / 16
+    assert near.sum() > 5000
+    rms = np.sqrt(np.mean(((out.reshape(-1, dim) - ref) / spread)[near] ** 2))
+    assert 0.5 * one < rms < 1.2 * one, rms / one
