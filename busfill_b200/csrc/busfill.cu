@@ -12,6 +12,7 @@
 #include <list>
 #include <map>
 #include <mutex>
+#include <new>
 #include <tuple>
 #include <type_traits>
 #include <utility>
@@ -354,21 +355,23 @@ int captured_workspace(int dev, cudaStream_t s, unsigned long long capture, cuda
         break;
       }
   }
+  if (mine.empty()) mine.push_back(CapturedWork{dev, s, capture, bytes, Work{}});
   // allocations and waits that have nothing to do with the capture are let through
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
   if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) {
     cudaGetLastError();
-    std::lock_guard<std::mutex> lk(all.mu);
-    all.spare.splice(all.spare.end(), mine);
+    if (mine.front().work.ptr) {
+      std::lock_guard<std::mutex> lk(all.mu);
+      all.spare.splice(all.spare.end(), mine);
+    }
     return BUSFILL_ERR_CUDA;
   }
   int st = BUSFILL_OK;
-  if (mine.empty()) {
-    void* p = nullptr;
-    if (cudaMalloc(&p, bytes) == cudaSuccess) {
+  if (!mine.front().work.ptr) {
+    if (cudaMalloc(&mine.front().work.ptr, bytes) == cudaSuccess) {
       ++g_internal_allocs;
-      mine.push_back(CapturedWork{dev, s, capture, bytes, Work{p, zeroed}});
     } else {
+      mine.clear();
       st = BUSFILL_ERR_ALLOC;
     }
   }
@@ -1188,16 +1191,22 @@ int gemm_sweep_impl(const busfill_sweep_op* ops, int nops, int M, cudaStream_t s
 namespace busfill {
 namespace host {
 
-int context(cudaStream_t s, Context* out) {
-  DeviceInfo di;
-  const int st = current_device(&di, &out->dev);
-  if (st != BUSFILL_OK) return st;
-  out->sms = di.sm_count;
-  std::lock_guard<std::mutex> lk(g_mu);
-  return get_error_words(out->dev, s, &out->error);
+namespace {
+
+// f() as a C entry point may return it: what is thrown (host memory that has
+// run out) is a status too.
+template <typename Fn>
+int guarded(Fn f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return BUSFILL_ERR_ALLOC;
+  } catch (...) {
+    return BUSFILL_ERR_CUDA;
+  }
 }
 
-int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t captured_bytes, size_t zeroed, void** out) {
+int make_workspace(const Context& c, cudaStream_t s, size_t bytes, size_t captured_bytes, size_t zeroed, void** out) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long capture = 0;
   cudaGraph_t graph = nullptr;
@@ -1226,6 +1235,23 @@ int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t captured_by
   }
   *out = w;
   return BUSFILL_OK;
+}
+
+}  // namespace
+
+int context(cudaStream_t s, Context* out) {
+  return guarded([&] {
+    DeviceInfo di;
+    const int st = current_device(&di, &out->dev);
+    if (st != BUSFILL_OK) return st;
+    out->sms = di.sm_count;
+    std::lock_guard<std::mutex> lk(g_mu);
+    return get_error_words(out->dev, s, &out->error);
+  });
+}
+
+int workspace(const Context& c, cudaStream_t s, size_t bytes, size_t captured_bytes, size_t zeroed, void** out) {
+  return guarded([&] { return make_workspace(c, s, bytes, captured_bytes, zeroed, out); });
 }
 
 int launch(const void* kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t s, void** args) {
@@ -1661,11 +1687,13 @@ int busfill_stream_status_ex(void* stream, unsigned* bits) {
     return BUSFILL_ERR_CUDA;
   if (err & ~kErrIndex) {   // the graphs captured on the stream report here too, wherever they run
     std::vector<Work> of_graphs;
-    {
+    try {
       CapturedWorks& all = captured_works();
       std::lock_guard<std::mutex> lk2(all.mu);
       for (const CapturedWork& w : all.used)
         if (w.dev == dev && w.stream == s) of_graphs.push_back(w.work);
+    } catch (const std::bad_alloc&) {
+      return BUSFILL_ERR_ALLOC;
     }
     if (!of_graphs.empty() && cudaDeviceSynchronize() != cudaSuccess) return BUSFILL_ERR_CUDA;
     for (const Work& w : of_graphs)
