@@ -23,6 +23,11 @@
 //     products moves 16-bit pairs). It uses fp16's whole range: the row's
 //     reference is set by the largest p d of a page, so only terms 2^-25 below
 //     the largest one lose bits, whatever the size of the values.
+//   * The tensor core lines a subnormal's products up as if it were 2^-14, so
+//     what is added up is good to about 2^-14 of a code step: an element whose
+//     sum cancels is off by up to 1e-5 of its block's largest value (the rows'
+//     error against 64 bits is that of one fp16 rounding, 2.6e-4, up to 131071
+//     tokens of like weight).
 // The matrix instruction is m16n8k16 with the tokens (scores) or channels
 // (output) as its 16 rows and the query rows as its 8 columns, so that a
 // group of 8 query heads fills it.
@@ -37,9 +42,9 @@
 // the workspace; always in the order of the ranges, so results repeat bit for
 // bit.
 //
-// Measured, 64 query heads over 8 of 128: 32 sequences to 16000 tokens 84 us
-// (353 MB, 4.3 TB/s; bulk copies of that size alone 64-74 us), one of 131071
-// 44 us (106 MB), one of 300 9 us.
+// Measured, 64 query heads over 8 of 128: 32 sequences to 16000 tokens 86 us
+// (353 MB, 4.1 TB/s; bulk copies of that size alone 64-74 us), one of 131071
+// 46 us (151 MB, 3.3 TB/s), one of 300 9 us.
 #pragma once
 
 #include "kv4_format.cuh"
@@ -915,8 +920,8 @@ __global__ void __launch_bounds__(Geo<D, NT>::kWarps * 32, 1) attn_kernel(const 
 // exp(score[r,s] - lse[r]). Keys only, so half the bytes of the attention. A
 // warp streams whole pages (ranges of the list of all pages, as above) and
 // walks over the rows that see each, so every sum has one owner and one order.
-// One sequence of 131071 tokens, 8 heads of 128, one row of 64 heads: 26 us for
-// 61 MB.
+// One sequence of 131071 tokens, 8 heads of 128, one row of 64 heads: 27 us for
+// 84 MB (75.5 of keys, the sums in and out), 3.1 TB/s.
 template <int D>
 struct WeightsGeo {
   static constexpr int kWarps = D == 256 ? 8 : 16;

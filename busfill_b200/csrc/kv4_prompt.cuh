@@ -34,8 +34,9 @@
 // (repeatable). Warp 2 walks the list and hands out what comes next as
 // descriptors in shared memory: the index arithmetic stays off the other warps.
 //
-// Measured, 64 query heads over 8 of 128: one prompt of 8000 tokens 1060 us
-// (990 TFLOP/s; sustained 1150 us at the power cap), 3 of 1000 104 us. A pair
+// Measured, 64 query heads over 8 of 128: one prompt of 8000 tokens 1020 us
+// (1030 TFLOP/s) after a pause, 1140 us sustained at the power cap; 3 of 1000
+// 104 us. A pair
 // of tiles takes 4500 cycles where its MMAs take 2080: the chain of score,
 // softmax and P V that the two row tiles take turns in bounds it, not the
 // exponentials (without a quarter of them 5 % less). An item's start and end
@@ -409,8 +410,9 @@ __global__ void __launch_bounds__(prompt::kThreads, 1) prompt_kernel(const __gri
           const uint8_t* src[G::kTilePages];
 #pragma unroll
           for (int k = 0; k < G::kTilePages; ++k)
-            src[k] = p.c.pages + ((size_t)(there(k) ? page_of(p.c, p.c.table, p.c.table_cols, x.b, page0 + k, bad) : 0) *
-                                      p.c.heads + x.head) * F::kPageBytes;
+            src[k] = p.c.pages +
+                     ((size_t)(there(k) ? page_of(p.c, p.c.table, p.c.table_cols, x.b, page0 + k, bad) : 0) * p.c.heads +
+                      x.head) * F::kPageBytes;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int st = n % G::kRawStages;

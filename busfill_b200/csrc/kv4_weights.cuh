@@ -6,7 +6,7 @@
 // so a TMEM lane, and with it a thread, owns a token and adds up its row of
 // S^T in registers; no reduction crosses threads. Half the MMAs of the
 // attention itself (2 R L D flops) and one exp2 per score (16 a clock and SM).
-// Measured, 3 prompts of 1000 tokens, 64 heads over 8 of 128: 80 us, where the
+// Measured, 3 prompts of 1000 tokens, 64 heads over 8 of 128: 82 us, where the
 // exponentials alone are 27; the rest is the first keys and queries of a range
 // (5 us) and the loaders, which 16 warps keep just ahead of the sums (8 warps,
 // with the masks read from shared memory: 10 us more).

@@ -287,7 +287,8 @@ def attn_kv4(q, pages, table, kv_len, q_start=None, max_q=None, scale=None, caus
 
     A row sees its whole sequence, with ``causal`` the slots up to its own, with window > 0 the last
     ``window`` of these; a row that sees nothing gives 0. ``max_q`` bounds the rows of one sequence
-    (default: all rows); a sequence with more is cut and reported. scale defaults to D ** -0.5.
+    (default: all rows, which for a ragged step of few rows a sequence chooses the slower kernel:
+    give it); a sequence with more is cut and reported. scale defaults to D ** -0.5.
     ``lse`` fp32 [tokens, q_heads] gets each row's log-sum-exp (-inf for a row that sees nothing).
     To ``weights`` fp32 [batch, kv_heads, cols >= 64 * table columns] the attention weight of every
     cached token, summed over the call's rows and the group's heads, is added."""
@@ -334,7 +335,7 @@ def kv4_evict(pages, table, kv_len, weights, keep, recent, out_table=None, weigh
     """Bring every sequence longer than ``keep`` down to ``keep`` tokens, head by head: the last
     ``recent`` stay, and of the others those with the largest accumulated weights (the lower slot of
     equals), in their order. ``out_table`` int32 [batch, cols] names the pages they move to (default:
-    the same table, in place). Returns (index, weights_out, new kv_len): index int32 [batch,
+    the same table, in place; then no page may be shared between sequences). Returns (index, weights_out, new kv_len): index int32 [batch,
     kv_heads, keep] holds the slots they came from (-1 behind a shorter sequence's)."""
     c, batch, heads, _, cols = _cache(pages, table, kv_len)
     w_ptr, w_cols = _weights(weights, "weights", batch, heads, cols)

@@ -465,7 +465,9 @@ BUSFILL_API int busfill_kv4_read(const busfill_kv4* cache, const int32_t* q_star
  * over the slots that a row sees: all of its sequence, with `causal` those up
  * to its own, with window > 0 (needs causal) the last `window` of these; pages
  * that lie before the windows of all of a sequence's rows are not looked up. A
- * row that sees nothing is 0 (its lse -inf). Scores, softmax statistics and
+ * row that sees nothing is 0 (its lse -inf). A sequence with more than max_q
+ * rows is cut to its first max_q, each at its own slot, and reported. out must
+ * not overlap q. Scores, softmax statistics and
  * sums are fp32. lse (optional, [tokens][q_heads]) gets log(sum exp(score)).
  * weights (optional, fp32 [batch][heads][weights_cols]): the weight that the
  * call's rows give slot s of their sequence, summed over rows and over the
@@ -508,7 +510,8 @@ BUSFILL_API int busfill_attn_kv4_kernel_for(int tokens, int q_heads, int heads, 
  * equals; NaN counts as the least). The kept tokens move, in their order, to
  * slots 0 .. keep - 1 of out_table (the same table as the cache's: in place,
  * with out_cols == table_cols; or pages that the cache's sequences do not
- * use). index [batch][heads][keep] gets the slots they came from (-1 behind a
+ * use). In place, a page must belong to one sequence alone: one that several
+ * share (a common prefix) would be overwritten for the others too. index [batch][heads][keep] gets the slots they came from (-1 behind a
  * shorter sequence's), weights_out [batch][heads][weights_cols] their weights
  * with zeros behind (it may be `weights`), kv_len_out [batch] the new lengths
  * (not the cache's kv_len). */
